@@ -3,8 +3,11 @@
 Produces, inside ``sm120_rmsnorm/``:
   * ``libsm120norm_b200.so`` -- the C-ABI library (include/sm120norm_b200.h):
     all CUDA kernels, compiled for sm_100a only, every non-ABI symbol hidden;
-  * ``_C<ext suffix>``       -- the PyTorch binding (csrc/torch_binding.cpp),
-    linked against the library through an ``$ORIGIN`` rpath.
+  * ``libsm120norm_b200_serving.so`` -- the serving operators
+    (include/sm120norm_b200_serving.h), linked against the first;
+  * ``_C<ext suffix>``       -- the PyTorch binding (csrc/torch_binding.cpp,
+    csrc/serving_binding.cpp), linked against both libraries through an
+    ``$ORIGIN`` rpath.
 
 Usage: ``python build.py [--force] [--verbose]`` (``--verbose`` prints
 ``ptxas -v`` register / spill / shared-memory reports).
@@ -30,13 +33,19 @@ BUILD = ROOT / "_build"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CUDA_SOURCES = ["runtime.cu", "row_norm.cu", "head_norm_rope.cu", "head_cache.cu", "norm_quant.cu", "norm_fp4.cu", "qkv_gemm.cu"]
+SHARED_SOURCES = ["device_caches.cu", "cache_args.cu"]  # in both libraries
+NORM_SOURCES = ["runtime.cu", "row_norm.cu", "head_norm_rope.cu", "head_cache.cu", "norm_quant.cu",
+                "norm_fp4.cu", "qkv_gemm.cu", *SHARED_SOURCES]
+SERVING_SOURCES = ["serving_runtime.cu", "step_plan.cu", "head_mrope.cu", "attention.cu",
+                   "attention_mma.cu", *SHARED_SOURCES]
+BINDING_SOURCES = ["torch_binding.cpp", "serving_binding.cpp"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     f"-I{INCLUDE}", f"-I{CSRC}",
 ]
 LIBRARY = PACKAGE / "libsm120norm_b200.so"
+SERVING_LIBRARY = PACKAGE / "libsm120norm_b200_serving.so"
 
 
 def _headers() -> list[Path]:
@@ -70,11 +79,28 @@ def _torch_cudart_dirs() -> list[Path]:
     return [d for d in [site / "nvidia" / "cuda_runtime" / "lib"] if (d / "libcudart.so.12").exists()]
 
 
+def _objects(sources: list[str]) -> list[Path]:
+    return [BUILD / (Path(n).stem + ".o") for n in sources]
+
+
+def _link(target: Path, sources: list[str], extra: list[str], verbose: bool) -> None:
+    tmp = BUILD / target.name
+    # The CUDA runtime is linked as a shared library so that, inside a
+    # PyTorch process, the libraries and PyTorch share one runtime instance
+    # (one current device, one set of streams). The rpath prefers the
+    # runtime PyTorch ships with, then the toolkit's.
+    rpaths = [str(p) for p in _torch_cudart_dirs()] + [str(CUDA_HOME / "lib64")]
+    _run([NVCC, *ARCH, "-shared", "-cudart", "shared", *map(str, _objects(sources)), "-o", str(tmp),
+          *extra, "-Xlinker", "--exclude-libs,ALL", "-Xlinker", "-Bsymbolic",
+          *[f"-Xlinker=-rpath,{r}" for r in rpaths]], verbose)
+    os.replace(tmp, target)
+
+
 def build_library(force: bool = False, verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     headers = _headers()
     jobs = []
-    for name in CUDA_SOURCES:
+    for name in dict.fromkeys([*NORM_SOURCES, *SERVING_SOURCES]):
         src = CSRC / name
         obj = BUILD / (Path(name).stem + ".o")
         if force or _stale(obj, [src, *headers]):
@@ -87,18 +113,11 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
             for out in pool.map(lambda c: _run(c, verbose), jobs):
                 if verbose and out:
                     print(out)
-    objects = [BUILD / (Path(n).stem + ".o") for n in CUDA_SOURCES]
-    if force or jobs or _stale(LIBRARY, objects):
-        tmp = BUILD / LIBRARY.name
-        # The CUDA runtime is linked as a shared library so that, inside a
-        # PyTorch process, this library and PyTorch share one runtime instance
-        # (one current device, one set of streams). The rpath prefers the
-        # runtime PyTorch ships with, then the toolkit's.
-        rpaths = [str(p) for p in _torch_cudart_dirs()] + [str(CUDA_HOME / "lib64")]
-        _run([NVCC, *ARCH, "-shared", "-cudart", "shared", *map(str, objects), "-o", str(tmp),
-              "-Xlinker", "--exclude-libs,ALL", "-Xlinker", "-Bsymbolic",
-              *[f"-Xlinker=-rpath,{r}" for r in rpaths]], verbose)
-        os.replace(tmp, LIBRARY)
+    if force or _stale(LIBRARY, _objects(NORM_SOURCES)):
+        _link(LIBRARY, NORM_SOURCES, [], verbose)
+    if force or _stale(SERVING_LIBRARY, [*_objects(SERVING_SOURCES), LIBRARY]):
+        _link(SERVING_LIBRARY, SERVING_SOURCES,
+              [f"-L{PACKAGE}", "-l:" + LIBRARY.name, "-Xlinker", "-rpath,$ORIGIN"], verbose)
     return LIBRARY
 
 
@@ -119,15 +138,21 @@ def _torch_flags() -> tuple[list[str], list[str]]:
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     target = PACKAGE / f"_C{suffix}"
-    src = CSRC / "torch_binding.cpp"
-    if not force and not _stale(target, [src, LIBRARY, *INCLUDE.glob("*.h")]):
+    sources = [CSRC / name for name in BINDING_SOURCES]
+    headers = list(INCLUDE.glob("*.h"))
+    if not force and not _stale(target, [*sources, LIBRARY, SERVING_LIBRARY, *headers]):
         return target
     compile_flags, link_flags = _torch_flags()
     BUILD.mkdir(exist_ok=True)
     tmp = BUILD / target.name
     cxx = shutil.which("g++") or "g++"
-    _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", *compile_flags, str(src), "-o", str(tmp),
-          *link_flags, f"-L{PACKAGE}", "-l:libsm120norm_b200.so", "-Wl,-rpath,$ORIGIN"], verbose)
+    objects = [BUILD / (src.stem + ".o") for src in sources]
+    jobs = [[cxx, "-O2", "-std=c++17", "-fPIC", *compile_flags, "-c", str(src), "-o", str(obj)]
+            for src, obj in zip(sources, objects) if force or _stale(obj, [src, *headers])]
+    with ThreadPoolExecutor(max_workers=2) as pool:
+        list(pool.map(lambda c: _run(c, verbose), jobs))
+    _run([cxx, "-shared", *map(str, objects), "-o", str(tmp), *link_flags, f"-L{PACKAGE}",
+          "-l:" + LIBRARY.name, "-l:" + SERVING_LIBRARY.name, "-Wl,-rpath,$ORIGIN"], verbose)
     os.replace(tmp, target)
     return target
 

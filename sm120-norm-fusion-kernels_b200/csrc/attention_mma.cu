@@ -1,0 +1,982 @@
+// attention_mma.cu -- attention on warp-level matrix instructions: the pass of
+// a decode step over each request's own cached tokens, and prompts and shared
+// prefixes with the head size that has no tensor-memory form.
+//
+//   o_i = sum_j softmax_j(scale * q_i . k_j) v_j
+// with the running maximum m and sum l of a row's exponentials: a tile of keys
+// with scores s gives m' = max(m, max s), p = 2^(s - m'), l' = l 2^(m - m') +
+// sum p, o' = o 2^(m - m') + p v. Scores, p's sum, o and all states are fp32;
+// p is rounded to the 16-bit operand type of the second product only.
+//
+// The query heads of one key head are rows of one tile, so K and V are read
+// once for all of them. A warp owns 16 rows. Where there are few rows (one
+// token per request) the four warps of a block share the rows and split the
+// 64 keys of a tile; otherwise each has rows of its own. K and V tiles go
+// from global to shared memory by cp.async, kStages tiles deep, 16-byte
+// chunks swizzled so that every matrix load is free of bank conflicts. Keys
+// behind the end of the sequence, or in a block that does not exist, are
+// filled with zeros and masked, so nothing stored there can reach a result.
+//
+// fp8 caches: e4m3 to fp16 is exact and one instruction for two values, so
+// these run the fp16 instruction, with each row of q scaled by a power of two
+// into [1, 2) first (exact but for elements 2^14 below the row's largest) and
+// the power folded into the row's score scale.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "attention.h"
+#include "device_utils.cuh"
+
+namespace sm120n {
+namespace {
+
+constexpr int kTileKeys = 64;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * kWarpSize;
+
+enum Pass : int { kPrompt, kPrefix, kOwn };
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__nv_bfloat16> {
+  __device__ __forceinline__ static void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Mma<__half> {
+  __device__ __forceinline__ static void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(address)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(address)
+               : "memory");
+}
+
+// 16 bytes from global to shared memory, zeros where `real` is false.
+__device__ __forceinline__ void copy16(uint32_t smem, const void* gmem, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem),
+               "r"(real ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two e4m3 bytes (low half of `b`) as two fp16 values.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(b), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+// Geometry of a pass: kRowWarps warps with rows of their own, the others
+// (kOwn) split the keys of a tile.
+template <typename T, bool kFp8, int D, int kPass>
+struct Form {
+  static constexpr int kElem = kFp8 ? 1 : 2;
+  static constexpr int kRowBytes = D * kElem;
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kRows = kPass == kOwn ? 16 : 16 * kWarps;
+  static constexpr int kWarpKeys = kPass == kOwn ? kTileKeys / kWarps : kTileKeys;
+  static constexpr int kTileBytes = kTileKeys * kRowBytes;
+  static constexpr int kQBytes = kRows * D * 2;
+  // Three tiles of K and V in flight, two for 512-byte rows: with two or
+  // three blocks to an SM that is 100 KB and more, past the 50 KB that
+  // latency times bandwidth asks of an SM.
+  static constexpr int kStages = kRowBytes > 256 ? 2 : 3;
+  static constexpr size_t kSmem = kQBytes + kStages * 2 * kTileBytes;
+};
+
+// Where 16-byte chunk c of a row lies. 16-bit tiles: the 8 rows of a matrix
+// hit 8 different chunks. fp8 tiles: two neighbouring rows read 64 bytes each
+// (K) and rows 0, 2, 4, 6 read 32 bytes each (V) at once.
+template <int kChunks, bool kFp8>
+__device__ __forceinline__ int chunk_at(int row, int c) {
+  if constexpr (!kFp8) return row * kChunks + (c ^ (row & 7));
+  if constexpr (kChunks == 4) return row * kChunks + (c ^ (((row >> 1) & 1) << 1));
+  return row * kChunks + (c ^ ((((row ^ (row >> 1)) & 1) << 2) | (((row >> 2) & 1) << 1)));
+}
+
+// A block's piece of work: rows of one key head against keys [key_first, key_last).
+struct Piece {
+  int64_t first_row;  // kPrompt: packed row (token, head of the group) of the sequence
+  int rows;
+  int key_first;
+  int key_last;
+  int kv_head;
+  int64_t token0;  // kPrompt: the sequence's first token
+  int request;     // kOwn
+};
+
+// Row `row` of a piece: its token and query head, as an offset into q or out.
+template <int kPass, typename Args>
+__device__ __forceinline__ int64_t row_offset(const Args& a, const Piece& p, int64_t row, int64_t stride,
+                                              int d) {
+  if constexpr (kPass == kOwn) {
+    return static_cast<int64_t>(p.request) * stride +
+           (static_cast<int64_t>(p.kv_head) * a.group + p.first_row + row) * d;
+  } else {
+    const int64_t r = p.first_row + row;
+    const int64_t token = r / a.group;
+    const int64_t head = static_cast<int64_t>(p.kv_head) * a.group + (r - token * a.group);
+    return (p.token0 + token) * stride + head * d;
+  }
+}
+
+template <typename TQ, typename T, bool kFp8, int D, int kPass, typename Args>
+struct Worker {
+  using F = Form<T, kFp8, D, kPass>;
+  const Args& a;
+  unsigned char* smem;
+  uint32_t* live;     // [kStages + 1][2] which keys of a tile exist, one bit each
+  int64_t* offsets;   // [kStages + 1][kTileKeys] elements from the head's first, -1: no such key
+  float* row_factor;  // fp8: power of two taken out of q
+
+  int warp, lane;
+  float o[D / 8][4];
+  float m[2], l[2];
+
+  __device__ __forceinline__ unsigned char* k_tile(int stage) const {
+    return smem + F::kQBytes + stage * 2 * F::kTileBytes;
+  }
+
+  // Where key `j` is: its token (kPrompt) or its offset within the head, in
+  // elements; -1 where there is none.
+  __device__ __forceinline__ int64_t key_offset(const Piece& p, int64_t j) const {
+    if (j >= p.key_last) return -1;
+    if constexpr (kPass == kPrompt) {
+      return p.token0 + j;
+    } else {
+      const int block = static_cast<int>(j / a.kv.block_size);
+      const int id = kPass == kPrefix
+                         ? a.prefix_blocks[block]
+                         : a.table[static_cast<int64_t>(p.request) * a.table_stride + block];
+      if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.kv.num_blocks)) return -1;
+      return id * a.kv.block_stride + (j - static_cast<int64_t>(block) * a.kv.block_size) * a.kv.slot_stride;
+    }
+  }
+
+  // Threads 0-63 place a tile's rows; `found` was computed ahead of the wait.
+  __device__ __forceinline__ void publish(int slot, int64_t found) {
+    if (threadIdx.x < kTileKeys) {
+      offsets[slot * kTileKeys + threadIdx.x] = found;
+      const uint32_t bits = __ballot_sync(kFullMask, found >= 0);
+      if (lane == 0) live[slot * 2 + warp] = bits;
+    }
+  }
+
+  __device__ __forceinline__ void load_tile(const Piece& p, int stage, int slot) {
+    const unsigned char *key, *value;
+    int64_t key_step, value_step, head;  // elements
+    if constexpr (kPass == kPrompt) {
+      key = static_cast<const unsigned char*>(a.key);
+      value = static_cast<const unsigned char*>(a.value);
+      key_step = a.key_stride;
+      value_step = a.value_stride;
+      head = static_cast<int64_t>(p.kv_head) * D;
+    } else {
+      key = static_cast<const unsigned char*>(a.kv.key);
+      value = static_cast<const unsigned char*>(a.kv.value);
+      key_step = value_step = 1;
+      head = p.kv_head * a.kv.head_stride;
+    }
+    const uint32_t k = shared_address(k_tile(stage));
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kTileKeys * F::kChunks; i += kThreads) {
+      const int row = i / F::kChunks;
+      const int c = i % F::kChunks;
+      const int64_t at = offsets[slot * kTileKeys + row];
+      const int64_t place = max(at, int64_t{0});
+      const uint32_t to = k + chunk_at<F::kChunks, kFp8>(row, c) * 16;
+      copy16(to, key + (place * key_step + head) * F::kElem + c * 16, at >= 0);
+      copy16(to + F::kTileBytes, value + (place * value_step + head) * F::kElem + c * 16, at >= 0);
+    }
+  }
+
+  // Q of the piece's rows into shared memory, as T; rows that do not exist are zeros.
+  __device__ __forceinline__ void load_query(const Piece& p) {
+    const TQ* query = static_cast<const TQ*>(a.query);
+    constexpr int kQChunks = D / 8;
+    const uint32_t base = shared_address(smem);
+    if constexpr (!kFp8) {
+      for (int i = threadIdx.x; i < F::kRows * kQChunks; i += kThreads) {
+        const int row = i / kQChunks, c = i % kQChunks;
+        const bool real = row < p.rows;
+        const TQ* from = real ? query + row_offset<kPass>(a, p, row, a.query_stride, D) + c * 8 : query;
+        copy16(base + (row * kQChunks + (c ^ (row & 7))) * 16, from, real);
+      }
+    } else {
+      // a warp to a row: its largest element, then the scaled row
+      for (int row = warp; row < F::kRows; row += kWarps) {
+        float v[D / kWarpSize];
+        float top = 0.0f;
+        const bool real = row < p.rows;
+        const TQ* from = query + (real ? row_offset<kPass>(a, p, row, a.query_stride, D) : 0);
+#pragma unroll
+        for (int i = 0; i < D / kWarpSize; ++i) {
+          const int e = lane * (D / kWarpSize) + i;
+          v[i] = real ? static_cast<float>(from[e]) : 0.0f;
+          top = fmaxf(top, fabsf(v[i]));
+        }
+#pragma unroll
+        for (int d = kWarpSize / 2; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+        // 2^-e and 2^e with e the exponent of the largest element, kept normal
+        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 2), 252);
+        const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+        if (lane == 0) row_factor[row] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+        for (int i = 0; i < D / kWarpSize; ++i) {
+          const int el = lane * (D / kWarpSize) + i;
+          T* to = reinterpret_cast<T*>(smem) + row * D + (((el / 8) ^ (row & 7)) * 8 + el % 8);
+          *to = static_cast<T>(v[i] * down);
+        }
+      }
+    }
+  }
+
+  // Scores of this warp's 16 rows x kWarpKeys keys of the tile in `stage`.
+  __device__ __forceinline__ void scores(int stage, float (*s)[4]) {
+    constexpr int kNt = F::kWarpKeys / 8;
+    const int key0 = kPass == kOwn ? warp * F::kWarpKeys : 0;
+    const int row0 = kPass == kOwn ? 0 : warp * 16;
+    const uint32_t q = shared_address(smem);
+    const uint32_t k = shared_address(k_tile(stage));
+#pragma unroll
+    for (int n = 0; n < kNt; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    if constexpr (!kFp8) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t qa[4];
+        const int qr = row0 + (lane & 15);
+        ldmatrix4(qa, q + (qr * (D / 8) + ((2 * kk + (lane >> 4)) ^ (qr & 7))) * 16);
+#pragma unroll
+        for (int n = 0; n < kNt; n += 2) {
+          uint32_t b[4];
+          const int r = key0 + n * 8 + (lane & 7) + ((lane >> 4) << 3);
+          ldmatrix4(b, k + chunk_at<F::kChunks, false>(r, 2 * kk + ((lane >> 3) & 1)) * 16);
+          Mma<T>::mma(s[n], qa, b[0], b[1]);
+          Mma<T>::mma(s[n + 1], qa, b[2], b[3]);
+        }
+      }
+    } else {
+      // The order of the summed index is free: in each run of 64 elements,
+      // step i of four takes elements 16t + 4i .. + 3 of lane t, so that a
+      // lane's bytes for four steps are one 16-byte load.
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int run = 0; run < D / 64; ++run) {
+        uint32_t qa[4][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // rows g and g + 8
+          const int r = row0 + g + 8 * half;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // 16 elements = two 16-byte chunks of T
+            const int chunk = run * 8 + 2 * t + c;
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + (r * (D / 8) + (chunk ^ (r & 7))) * 16);
+            qa[2 * c][half] = v.x;
+            qa[2 * c][2 + half] = v.y;
+            qa[2 * c + 1][half] = v.z;
+            qa[2 * c + 1][2 + half] = v.w;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) {
+          const int r = key0 + n * 8 + g;
+          const uint4 v = *reinterpret_cast<const uint4*>(
+              k_tile(stage) + chunk_at<F::kChunks, true>(r, run * 4 + t) * 16);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            Mma<T>::mma(s[n], qa[i], e4m3_pair(w[i] & 0xffffu), e4m3_pair(w[i] >> 16));
+          }
+        }
+      }
+    }
+  }
+
+  // o += p v over this warp's keys; p as operand registers, 16 keys each.
+  __device__ __forceinline__ void weigh(int stage, const uint32_t (*p)[4]) {
+    const int key0 = kPass == kOwn ? warp * F::kWarpKeys : 0;
+    unsigned char* tile = k_tile(stage) + F::kTileBytes;
+    const uint32_t v = shared_address(tile);
+#pragma unroll
+    for (int kk = 0; kk < F::kWarpKeys / 16; ++kk) {
+      if constexpr (!kFp8) {
+        const int r = key0 + kk * 16 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < D / 8; n += 2) {
+          uint32_t b[4];
+          ldmatrix4_trans(b, v + chunk_at<F::kChunks, false>(r, n + (lane >> 4)) * 16);
+          Mma<T>::mma(o[n], p[kk], b[0], b[1]);
+          Mma<T>::mma(o[n + 1], p[kk], b[2], b[3]);
+        }
+      } else {
+        // The order of the columns is free: of a run of 32, lane group g
+        // holds 4g .. 4g + 3, the i-th of them in product i of four.
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int run = 0; run < D / 32; ++run) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = key0 + kk * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
+            w[j] = *reinterpret_cast<const uint32_t*>(
+                tile + chunk_at<F::kChunks, true>(r, run * 2 + (g >> 2)) * 16 + (g & 3) * 4);
+          }
+          const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5140), hi0 = __byte_perm(w[0], w[1], 0x7362);
+          const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5140), hi1 = __byte_perm(w[2], w[3], 0x7362);
+          Mma<T>::mma(o[run * 4], p[kk], e4m3_pair(lo0 & 0xffffu), e4m3_pair(lo1 & 0xffffu));
+          Mma<T>::mma(o[run * 4 + 1], p[kk], e4m3_pair(lo0 >> 16), e4m3_pair(lo1 >> 16));
+          Mma<T>::mma(o[run * 4 + 2], p[kk], e4m3_pair(hi0 & 0xffffu), e4m3_pair(hi1 & 0xffffu));
+          Mma<T>::mma(o[run * 4 + 3], p[kk], e4m3_pair(hi0 >> 16), e4m3_pair(hi1 >> 16));
+        }
+      }
+    }
+  }
+
+  // Column of o[n][c] (c = 0 or 1 of the row's pair).
+  __device__ __forceinline__ int column(int n, int c) const {
+    const int t = lane & 3;
+    if constexpr (kFp8) return (n / 4) * 32 + 4 * (2 * t + c) + n % 4;
+    return n * 8 + 2 * t + c;
+  }
+
+  __device__ __forceinline__ uint32_t pack(float x, float y) const {
+    return Pack<T>::f32_to_word(x, y);
+  }
+
+  // One row of a prompt by plain arithmetic, one warp, keys one by one: used
+  // for blocks of rows that have an infinite or NaN value among the keys that
+  // some of them must not see (a matrix product would multiply it by zero).
+  __device__ __noinline__ void plain_row(const Piece& p, int64_t row, float scale_log2, TQ* out) {
+    const int64_t r = p.first_row + row;
+    const int64_t last = min(r / a.group, static_cast<int64_t>(p.key_last) - 1);
+    const TQ* q = static_cast<const TQ*>(a.query) + row_offset<kPass>(a, p, row, a.query_stride, D);
+    float acc[D / kWarpSize] = {};
+    float top = -INFINITY, sum = 0.0f;
+    for (int64_t j = 0; j <= last; ++j) {
+      const int64_t head = static_cast<int64_t>(p.kv_head) * D;
+      const TQ* k = static_cast<const TQ*>(a.key) + (p.token0 + j) * a.key_stride + head;
+      const TQ* v = static_cast<const TQ*>(a.value) + (p.token0 + j) * a.value_stride + head;
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / kWarpSize; ++i) {
+        s += static_cast<float>(q[lane + i * kWarpSize]) * static_cast<float>(k[lane + i * kWarpSize]);
+      }
+#pragma unroll
+      for (int d = kWarpSize / 2; d > 0; d /= 2) s += __shfl_xor_sync(kFullMask, s, d);
+      s *= scale_log2;
+      const float next = fmaxf(top, s);
+      const float keep = next == -INFINITY ? 1.0f : exp2_approx(top - next);
+      const float e = next == -INFINITY ? 0.0f : exp2_approx(s - next);
+      top = next;
+      sum = sum * keep + e;
+#pragma unroll
+      for (int i = 0; i < D / kWarpSize; ++i) {
+        acc[i] = acc[i] * keep + e * static_cast<float>(v[lane + i * kWarpSize]);
+      }
+    }
+    TQ* to = out + row_offset<kPass>(a, p, row, a.out_stride, D);
+#pragma unroll
+    for (int i = 0; i < D / kWarpSize; ++i) to[lane + i * kWarpSize] = static_cast<TQ>(acc[i] / sum);
+  }
+
+  // Whether a value of the tile in `stage` is infinite or NaN (16-bit tiles, whole block).
+  __device__ __forceinline__ bool unsafe_values(int stage) {
+    constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    const uint4* v = reinterpret_cast<const uint4*>(k_tile(stage) + F::kTileBytes);
+    bool bad = false;
+    for (int i = threadIdx.x; i < kTileKeys * F::kChunks; i += kThreads) {
+      const uint4 x = v[i];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bad |= (w[j] & kExponent) == kExponent || ((w[j] >> 16) & kExponent) == kExponent;
+      }
+    }
+    return __syncthreads_or(bad);
+  }
+
+  // Runs over the piece's keys. kPrompt: true when a value that some rows
+  // must not see was infinite or NaN.
+  __device__ __forceinline__ bool run(const Piece& p, float scale_log2) {
+    constexpr int kNt = F::kWarpKeys / 8;
+    constexpr int kRing = F::kStages + 1;
+    const int tiles = (p.key_last - p.key_first + kTileKeys - 1) / kTileKeys;
+    bool unsafe = false;
+    __syncthreads();  // the piece before is done with shared memory
+    load_query(p);
+#pragma unroll
+    for (int t = 0; t < F::kStages; ++t) {
+      publish(t, threadIdx.x < kTileKeys ? key_offset(p, p.key_first + int64_t{t} * kTileKeys + threadIdx.x) : -1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < F::kStages; ++t) {
+      if (t < tiles) load_tile(p, t, t);
+      copies_commit();
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.0f;
+    const int row0 = (kPass == kOwn ? 0 : warp * 16) + (lane >> 2);
+    int64_t limit[2] = {0, 0};  // kPrompt: last key of the row
+    if constexpr (kPass == kPrompt) {
+      limit[0] = (p.first_row + row0) / a.group;
+      limit[1] = (p.first_row + row0 + 8) / a.group;
+    }
+    for (int t = 0; t < tiles; ++t) {
+      const int stage = t % F::kStages;
+      const int slot = t % kRing;
+      const int64_t ahead =
+          threadIdx.x < kTileKeys
+              ? key_offset(p, p.key_first + (int64_t{t} + F::kStages) * kTileKeys + threadIdx.x)
+              : -1;
+      copies_wait<F::kStages - 1>();
+      __syncthreads();
+      const int64_t key0 = p.key_first + int64_t{t} * kTileKeys;
+      if constexpr (kPass == kPrompt) {
+        // the last rows see all keys up to key_last; the first stop at theirs
+        if (key0 + kTileKeys - 1 > p.first_row / a.group) unsafe = unsafe_values(stage) || unsafe;
+      }
+      float s[kNt][4];
+      scores(stage, s);
+      float f0 = scale_log2, f1 = scale_log2;
+      if constexpr (kFp8) {
+        f0 *= row_factor[row0];
+        f1 *= row_factor[row0 + 8];
+      }
+      const uint32_t live0 = live[slot * 2], live1 = live[slot * 2 + 1];
+      const bool whole = (live0 & live1) == kFullMask;
+      const int warp_key = kPass == kOwn ? warp * F::kWarpKeys : 0;
+      float top0 = m[0], top1 = m[1];
+#pragma unroll
+      for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int key = warp_key + n * 8 + 2 * (lane & 3) + c;
+          s[n][c] *= f0;
+          s[n][2 + c] *= f1;
+          const bool there = whole || (((key < 32 ? live0 : live1) >> (key & 31)) & 1u);
+          if (!there || (kPass == kPrompt && key0 + key > limit[0])) s[n][c] = -INFINITY;
+          if (!there || (kPass == kPrompt && key0 + key > limit[1])) s[n][2 + c] = -INFINITY;
+          top0 = fmaxf(top0, s[n][c]);
+          top1 = fmaxf(top1, s[n][2 + c]);
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d *= 2) {
+        top0 = fmaxf(top0, __shfl_xor_sync(kFullMask, top0, d));
+        top1 = fmaxf(top1, __shfl_xor_sync(kFullMask, top1, d));
+      }
+      // a row that has seen nothing yet keeps everything at zero
+      const float base0 = top0 == -INFINITY ? 0.0f : top0;
+      const float base1 = top1 == -INFINITY ? 0.0f : top1;
+      const float keep0 = exp2_approx(m[0] - base0);
+      const float keep1 = exp2_approx(m[1] - base1);
+      m[0] = top0;
+      m[1] = top1;
+      float sum0 = 0.0f, sum1 = 0.0f;
+      uint32_t pr[kNt / 2][4];
+#pragma unroll
+      for (int n = 0; n < kNt; ++n) {
+        const float x0 = exp2_approx(s[n][0] - base0), y0 = exp2_approx(s[n][1] - base0);
+        const float x1 = exp2_approx(s[n][2] - base1), y1 = exp2_approx(s[n][3] - base1);
+        sum0 += x0 + y0;
+        sum1 += x1 + y1;
+        pr[n / 2][(n & 1) * 2] = pack(x0, y0);
+        pr[n / 2][(n & 1) * 2 + 1] = pack(x1, y1);
+      }
+      l[0] = l[0] * keep0 + sum0;
+      l[1] = l[1] * keep1 + sum1;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][0] *= keep0;
+        o[n][1] *= keep0;
+        o[n][2] *= keep1;
+        o[n][3] *= keep1;
+      }
+      weigh(stage, pr);
+      publish((t + F::kStages) % kRing, ahead);
+      __syncthreads();
+      if (t + F::kStages < tiles) load_tile(p, stage, (t + F::kStages) % kRing);
+      copies_commit();
+    }
+    copies_wait<0>();
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+      l[0] += __shfl_xor_sync(kFullMask, l[0], d);
+      l[1] += __shfl_xor_sync(kFullMask, l[1], d);
+    }
+    return unsafe;
+  }
+};
+
+#define SM120S_WORKER(FORM)                                                           \
+  extern __shared__ __align__(128) unsigned char dynamic_smem[];                      \
+  __shared__ uint32_t live[(FORM::kStages + 1) * 2];                                  \
+  __shared__ int64_t offsets[(FORM::kStages + 1) * kTileKeys];                        \
+  __shared__ float row_factor[FORM::kRows]
+
+// ---- prompts -----------------------------------------------------------------
+
+// The sequence and tile of its rows that block `index` of the tile list works
+// on: tiles of `rows` (token, head) rows, sequence after sequence. Whole block.
+struct SequenceTile {
+  int64_t first_token;
+  int64_t length;
+  int64_t tile;  // -1: the list is shorter
+  int64_t tiles;
+};
+
+__device__ __forceinline__ int64_t clamp_start(int32_t v, int64_t tokens) {
+  return min(max(static_cast<int64_t>(v), int64_t{0}), tokens);
+}
+
+template <int kBlockThreads>
+__device__ __forceinline__ SequenceTile find_tile(const int32_t* query_start, int sequences,
+                                                  int64_t tokens, int group, int rows,
+                                                  int64_t index) {
+  __shared__ int64_t totals[kBlockThreads / kWarpSize];
+  __shared__ SequenceTile found;
+  const int lane = threadIdx.x & (kWarpSize - 1);
+  const int warp = threadIdx.x / kWarpSize;
+  if (threadIdx.x == 0) found.tile = -1;
+  int64_t before = 0;
+  for (int base = 0; base < sequences; base += kBlockThreads) {
+    const int i = base + threadIdx.x;
+    int64_t first = 0, length = 0;
+    if (i < sequences) {
+      first = clamp_start(query_start[i], tokens);
+      length = max(clamp_start(query_start[i + 1], tokens) - first, int64_t{0});
+    }
+    const int64_t mine = (length * group + rows - 1) / rows;
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < kWarpSize; d *= 2) {
+      const int64_t x = __shfl_up_sync(kFullMask, upto, d);
+      if (lane >= d) upto += x;
+    }
+    __syncthreads();
+    if (lane == kWarpSize - 1) totals[warp] = upto;
+    __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < kBlockThreads / kWarpSize; ++w) {
+      if (w < warp) upto += totals[w];
+      all += totals[w];
+    }
+    upto += before;
+    if (index < upto && index >= upto - mine) {
+      // the last rows of a sequence have the most keys: first
+      found = SequenceTile{first, length, upto - 1 - index, mine};
+    }
+    before += all;
+    if (index < before) break;
+  }
+  __syncthreads();
+  return found;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) prompt_mma_kernel(PromptArgs a) {
+  using F = Form<T, false, D, kPrompt>;
+  SM120S_WORKER(F);
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  const SequenceTile tile = find_tile<kThreads>(a.query_start, a.sequences, a.tokens, a.group,
+                                                F::kRows, blockIdx.x / a.key_heads);
+  if (tile.tile < 0) return;
+  Worker<T, T, false, D, kPrompt, PromptArgs> w{a, dynamic_smem, live, offsets, row_factor};
+  w.warp = threadIdx.x / kWarpSize;
+  w.lane = threadIdx.x & (kWarpSize - 1);
+  Piece p{};
+  p.first_row = tile.tile * F::kRows;
+  p.rows = static_cast<int>(min(int64_t{F::kRows}, tile.length * a.group - p.first_row));
+  p.key_last = static_cast<int>((p.first_row + p.rows - 1) / a.group + 1);
+  p.kv_head = static_cast<int>(blockIdx.x % a.key_heads);
+  p.token0 = tile.first_token;
+  T* out = static_cast<T*>(a.out);
+  if (w.run(p, a.scale_log2)) {
+    for (int row = w.warp; row < p.rows; row += kWarps) w.plain_row(p, row, a.scale_log2, out);
+    return;
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = w.warp * 16 + (w.lane >> 2) + 8 * half;
+    if (row >= p.rows) continue;
+    const float inv = 1.0f / w.l[half];
+    T* to = out + row_offset<kPrompt>(a, p, row, a.out_stride, D);
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      *reinterpret_cast<uint32_t*>(to + n * 8 + 2 * (w.lane & 3)) =
+          Pack<T>::f32_to_word(w.o[n][2 * half] * inv, w.o[n][2 * half + 1] * inv);
+    }
+  }
+}
+
+// ---- the shared prefix of a decode batch ----------------------------------------
+// Rows: (request, head of the group) of one key head; keys: one part of the prefix.
+template <typename TQ, typename T, bool kFp8, int D>
+__global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(DecodeArgs a) {
+  using F = Form<T, kFp8, D, kPrefix>;
+  SM120S_WORKER(F);
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  Worker<TQ, T, kFp8, D, kPrefix, DecodeArgs> w{a, dynamic_smem, live, offsets, row_factor};
+  w.warp = threadIdx.x / kWarpSize;
+  w.lane = threadIdx.x & (kWarpSize - 1);
+  Piece p{};
+  p.first_row = static_cast<int64_t>(blockIdx.x) * F::kRows;
+  p.rows = static_cast<int>(min(int64_t{F::kRows}, int64_t{a.batch} * a.group - p.first_row));
+  p.kv_head = blockIdx.y;
+  const int64_t tiles = (a.prefix_tokens + kTileKeys - 1) / kTileKeys;
+  const int split = blockIdx.z;
+  p.key_first = static_cast<int>(tiles * split / a.prefix_splits * kTileKeys);
+  p.key_last = static_cast<int>(min(tiles * (split + 1) / a.prefix_splits * kTileKeys,
+                                    int64_t{a.prefix_tokens}));
+  const float scale = kFp8 ? a.scale_log2 * *a.k_scale : a.scale_log2;
+  w.run(p, scale);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = w.warp * 16 + (w.lane >> 2) + 8 * half;
+    if (row >= p.rows) continue;
+    const int64_t r = p.first_row + row;
+    const int64_t request = r / a.group;
+    const int64_t at = (static_cast<int64_t>(split) * a.batch + request) * a.query_heads +
+                       static_cast<int64_t>(p.kv_head) * a.group + (r - request * a.group);
+    if ((w.lane & 3) == 0) a.prefix_state[at] = make_float2(w.m[half], w.l[half]);
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      a.prefix_values[at * D + w.column(n, 0)] = w.o[n][2 * half];
+      a.prefix_values[at * D + w.column(n, 1)] = w.o[n][2 * half + 1];
+    }
+  }
+}
+
+// ---- each request's own tokens ------------------------------------------------------
+// The key tiles of all (request, key head, row tile) triples stand in one
+// list, cut into min(own_grid, tiles) equal runs, none empty: a block's run may
+// end one triple and begin others, and every triple it touches gets one
+// partial result, at index triple + block, which no other (triple, block) of
+// the list shares.
+__device__ __forceinline__ int own_tokens(const DecodeArgs& a, int request, int* first_block) {
+  const int64_t cap = static_cast<int64_t>(a.table_width) * a.kv.block_size;
+  const int64_t n = min(static_cast<int64_t>(max(a.seq_lens[request], 0)), cap);
+  const bool shares = n >= a.prefix_tokens;
+  *first_block = shares ? a.prefix_tokens : 0;
+  return static_cast<int>(n) - *first_block;
+}
+
+template <typename TQ, typename T, bool kFp8, int D>
+__global__ void __launch_bounds__(kThreads, 1) own_mma_kernel(DecodeArgs a) {
+  using F = Form<T, kFp8, D, kOwn>;
+  SM120S_WORKER(F);
+  __shared__ int32_t warp_totals[kWarps];
+  __shared__ int64_t found_start;
+  __shared__ int found_request;
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  Worker<TQ, T, kFp8, D, kOwn, DecodeArgs> w{a, dynamic_smem, live, offsets, row_factor};
+  w.warp = threadIdx.x / kWarpSize;
+  w.lane = threadIdx.x & (kWarpSize - 1);
+  const int triples = a.key_heads * a.row_tiles;  // of one request
+  const float scale = kFp8 ? a.scale_log2 * *a.k_scale : a.scale_log2;
+
+  auto tiles_of = [&](int request) {
+    int first;
+    return (own_tokens(a, request, &first) + kTileKeys - 1) / kTileKeys;
+  };
+  // sums of the requests' tiles, chunk by chunk; f(request, tiles before, tiles)
+  auto over_requests = [&](auto f) {
+    int64_t before = 0;
+    for (int base = 0; base < a.batch; base += kThreads) {
+      const int i = base + threadIdx.x;
+      const int mine = i < a.batch ? tiles_of(i) : 0;
+      int upto = mine;
+#pragma unroll
+      for (int d = 1; d < kWarpSize; d *= 2) {
+        const int x = __shfl_up_sync(kFullMask, upto, d);
+        if (w.lane >= d) upto += x;
+      }
+      __syncthreads();
+      if (w.lane == kWarpSize - 1) warp_totals[w.warp] = upto;
+      __syncthreads();
+      int64_t all = 0;
+      for (int k = 0; k < kWarps; ++k) {
+        if (k < w.warp) upto += warp_totals[k];
+        all += warp_totals[k];
+      }
+      if (i < a.batch) f(i, before + upto - mine, mine);
+      before += all;
+    }
+    return before;
+  };
+  const int64_t total = over_requests([&](int i, int64_t start, int) {
+                          if (blockIdx.x == 0) a.tile_start[i] = static_cast<int32_t>(start);
+                        }) * triples;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = static_cast<int32_t>(total / triples);
+  const int64_t runs = min(total, int64_t{a.own_grid});
+  if (blockIdx.x >= runs) return;
+  int64_t at = total * blockIdx.x / runs;
+  const int64_t end = total * (blockIdx.x + 1) / runs;
+  over_requests([&](int i, int64_t start, int n) {
+    if (at >= start * triples && at < (start + n) * triples) {
+      found_request = i;
+      found_start = start * triples;
+    }
+  });
+  __syncthreads();
+  int request = found_request;
+  int64_t request_start = found_start;
+  while (at < end) {
+    int first_key;
+    const int keys = own_tokens(a, request, &first_key);
+    const int n = (keys + kTileKeys - 1) / kTileKeys;
+    if (n == 0) {
+      ++request;
+      continue;
+    }
+    const int triple = static_cast<int>((at - request_start) / n);
+    const int64_t triple_start = request_start + static_cast<int64_t>(triple) * n;
+    const int tile0 = static_cast<int>(at - triple_start);
+    const int tile1 = static_cast<int>(min(end - triple_start, int64_t{n}));
+    Piece p{};
+    p.request = request;
+    p.kv_head = triple / a.row_tiles;
+    p.first_row = static_cast<int64_t>(triple % a.row_tiles) * 16;
+    p.rows = min(16, a.group - static_cast<int>(p.first_row));
+    p.key_first = first_key + tile0 * kTileKeys;
+    p.key_last = first_key + min(tile1 * kTileKeys, keys);
+    w.run(p, scale);
+
+    // The four warps' states of the same rows become one; their values pass
+    // through the K / V stages, which the run has left.
+    __shared__ float2 states[kWarps][16];
+    float* values = reinterpret_cast<float*>(dynamic_smem + F::kQBytes);  // [kWarps][16][D]
+    static_assert(static_cast<size_t>(kWarps) * 16 * D * 4 <= F::kStages * 2 * F::kTileBytes,
+                  "the warps' partial values fit the stages");
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = (w.lane >> 2) + 8 * half;
+      if ((w.lane & 3) == 0) states[w.warp][row] = make_float2(w.m[half], w.l[half]);
+      if (row < p.rows) {
+        float* to = values + (w.warp * 16 + row) * D;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          to[w.column(i, 0)] = w.o[i][2 * half];
+          to[w.column(i, 1)] = w.o[i][2 * half + 1];
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t slot = (static_cast<int64_t>(request) * triples + triple + blockIdx.x) * 16;
+    for (int i = threadIdx.x; i < p.rows * (D / 4); i += kThreads) {
+      const int row = i / (D / 4), c = i % (D / 4);
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, states[k][row].x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float2 st = states[k][row];
+        const float f = exp2_approx(st.x - base);
+        sum += st.y * f;
+        const float4 x = *reinterpret_cast<const float4*>(values + (k * 16 + row) * D + 4 * c);
+        v.x += x.x * f;
+        v.y += x.y * f;
+        v.z += x.z * f;
+        v.w += x.w * f;
+      }
+      *reinterpret_cast<float4*>(a.own_values + (slot + row) * D + 4 * c) = v;
+      if (c == 0) a.own_state[slot + row] = make_float2(top, sum);
+    }
+    at = triple_start + tile1;
+    if (at >= request_start + static_cast<int64_t>(n) * triples) {
+      request_start += static_cast<int64_t>(n) * triples;
+      ++request;
+    }
+  }
+}
+
+// ---- the parts of a row joined ---------------------------------------------------
+// One warp to a (request, query head): the parts of the prefix, then the runs
+// that touched the row's triple, always in this order.
+template <typename TQ, int D>
+__global__ void __launch_bounds__(kThreads) merge_kernel(DecodeArgs a) {
+  constexpr int kPer = D / kWarpSize;
+  const int lane = threadIdx.x & (kWarpSize - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / kWarpSize;
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  if (row >= static_cast<int64_t>(a.batch) * a.query_heads) return;
+  const int request = static_cast<int>(row / a.query_heads);
+  const int head = static_cast<int>(row - static_cast<int64_t>(request) * a.query_heads);
+  const int kv_head = head / a.group;
+  const int in_group = head - kv_head * a.group;
+  float top = -INFINITY, sum = 0.0f;
+  float acc[kPer] = {};
+  auto add = [&](float2 state, const float* values) {
+    // nothing seen; a sum that is not zero has seen a NaN and passes it on
+    if (state.x == -INFINITY && state.y == 0.0f) return;
+    const float next = fmaxf(top, state.x);
+    const float keep = exp2_approx(top - next);
+    const float f = exp2_approx(state.x - next);
+    top = next;
+    sum = sum * keep + state.y * f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * keep + values[lane * kPer + i] * f;
+  };
+  int first_key;
+  const int keys = own_tokens(a, request, &first_key);
+  if (first_key > 0) {  // the request shares the prefix
+    for (int s = 0; s < a.prefix_splits; ++s) {
+      const int64_t at = static_cast<int64_t>(s) * a.batch * a.query_heads + row;
+      add(a.prefix_state[at], a.prefix_values + at * D);
+    }
+  }
+  if (keys > 0) {
+    const int triples = a.key_heads * a.row_tiles;
+    const int triple = kv_head * a.row_tiles + in_group / 16;
+    const int64_t total = static_cast<int64_t>(a.tile_start[a.batch]) * triples;
+    const int64_t n = a.tile_start[request + 1] - a.tile_start[request];
+    const int64_t t0 = static_cast<int64_t>(a.tile_start[request]) * triples + triple * n;
+    // the runs that hold the triple's first and last tile
+    const int64_t runs = min(total, int64_t{a.own_grid});
+    const int64_t from = ((t0 + 1) * runs - 1) / total;
+    const int64_t to = ((t0 + n) * runs - 1) / total;
+    for (int64_t run = from; run <= to; ++run) {
+      const int64_t at = (static_cast<int64_t>(request) * triples + triple + run) * 16 + in_group % 16;
+      add(a.own_state[at], a.own_values + at * D);
+    }
+  }
+  const float v_scale = a.v_scale ? *a.v_scale : 1.0f;
+  const float inv = sum == 0.0f ? 0.0f : v_scale / sum;
+  TQ* out = static_cast<TQ*>(a.out) + request * a.out_stride + static_cast<int64_t>(head) * D + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer; i += 2) {
+    *reinterpret_cast<uint32_t*>(out + i) = Pack<TQ>::f32_to_word(acc[i] * inv, acc[i + 1] * inv);
+  }
+}
+
+template <typename T, int D>
+int run_prompt(const PromptArgs& a, cudaStream_t stream) {
+  using F = Form<T, false, D, kPrompt>;
+  auto kernel = prompt_mma_kernel<T, D>;
+  int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), F::kSmem);
+  if (rc != SM120N_OK) return rc;
+  const int64_t tiles = (a.tokens * a.group + F::kRows - 1) / F::kRows + a.sequences;
+  return launch(kernel, dim3(static_cast<unsigned>(tiles * a.key_heads)), dim3(kThreads), F::kSmem,
+                stream, a);
+}
+
+template <typename TQ, typename T, bool kFp8, int D>
+int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
+  using F = Form<T, kFp8, D, kPrefix>;
+  auto kernel = prefix_mma_kernel<TQ, T, kFp8, D>;
+  int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), F::kSmem);
+  if (rc != SM120N_OK) return rc;
+  const int64_t tiles = (static_cast<int64_t>(a.batch) * a.group + F::kRows - 1) / F::kRows;
+  return launch(kernel,
+                dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.key_heads),
+                     static_cast<unsigned>(a.prefix_splits)),
+                dim3(kThreads), F::kSmem, stream, a);
+}
+
+template <typename TQ, typename T, bool kFp8, int D>
+int run_own(const DecodeArgs& a, cudaStream_t stream) {
+  using F = Form<T, kFp8, D, kOwn>;
+  auto kernel = own_mma_kernel<TQ, T, kFp8, D>;
+  int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), F::kSmem);
+  if (rc != SM120N_OK) return rc;
+  return launch(kernel, dim3(static_cast<unsigned>(a.own_grid)), dim3(kThreads), F::kSmem, stream, a);
+}
+
+}  // namespace
+
+// As many as shared memory holds (100 KB a block for 256-byte rows), at most four.
+int own_blocks_per_sm(int row_bytes) {
+  const int stages = row_bytes > 256 ? 2 : 3;
+  return std::min(4, 220 * 1024 / (stages * 2 * kTileKeys * row_bytes + 12 * 1024));
+}
+
+#define SM120S_BY_HEAD_DIM(CALL)      \
+  switch (head_dim) {                 \
+    case 64: return CALL(64);         \
+    case 128: return CALL(128);       \
+    default: return CALL(256);        \
+  }
+
+int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream) {
+#define CALL(D) \
+  dtype == SM120N_F16 ? run_prompt<__half, D>(a, stream) : run_prompt<__nv_bfloat16, D>(a, stream)
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
+                      cudaStream_t stream) {
+  const bool fp8 = cache_dtype == SM120N_CACHE_FP8_E4M3;
+#define CALL(D)                                                                          \
+  dtype == SM120N_F16 ? (fp8 ? run_prefix<__half, __half, true, D>(a, stream)            \
+                             : run_prefix<__half, __half, false, D>(a, stream))          \
+                      : (fp8 ? run_prefix<__nv_bfloat16, __half, true, D>(a, stream)     \
+                             : run_prefix<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream))
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+int launch_own_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
+                   cudaStream_t stream) {
+  const bool fp8 = cache_dtype == SM120N_CACHE_FP8_E4M3;
+#define CALL(D)                                                                       \
+  dtype == SM120N_F16 ? (fp8 ? run_own<__half, __half, true, D>(a, stream)            \
+                             : run_own<__half, __half, false, D>(a, stream))          \
+                      : (fp8 ? run_own<__nv_bfloat16, __half, true, D>(a, stream)     \
+                             : run_own<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream))
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+int launch_merge(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.query_heads;
+  const dim3 grid(static_cast<unsigned>((rows + kWarps - 1) / kWarps));
+#define CALL(D)                                                                                \
+  dtype == SM120N_F16 ? launch(merge_kernel<__half, D>, grid, dim3(kThreads), 0, stream, a)    \
+                      : launch(merge_kernel<__nv_bfloat16, D>, grid, dim3(kThreads), 0, stream, a)
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+}  // namespace sm120n

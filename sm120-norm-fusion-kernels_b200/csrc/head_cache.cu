@@ -26,13 +26,12 @@
 
 #include <algorithm>
 
+#include "cache_args.h"
 #include "head_utils.cuh"
 #include "runtime.h"
 
 namespace sm120n {
 namespace {
-
-enum CacheKind : int { kNoCache = 0, kSameType = 1, kFp8 = 2 };
 
 template <typename T>
 struct CacheArgs {
@@ -96,18 +95,6 @@ __device__ __forceinline__ uint2 chunk_to_fp8(const Half8<T>& h, float scale) {
     b[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3));
   }
   return make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
-}
-
-template <bool kVector>
-__device__ __forceinline__ void store_fp8_chunk(uint8_t* p, uint2 v) {
-  if constexpr (kVector) {
-    *reinterpret_cast<uint2*>(p) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = static_cast<uint8_t>(v.x >> (8 * i));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[4 + i] = static_cast<uint8_t>(v.y >> (8 * i));
-  }
 }
 
 // kFullNeox: rotary over the whole head with NEOX (half-split) pairs, the
@@ -290,10 +277,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 2) head_cache_kernel
   }
 }
 
-bool aligned_to(const void* p, uintptr_t bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
-}
-
 template <typename T, int D, int kCache>
 int run_cache(CacheArgs<T> a, cudaStream_t stream) {
   const int64_t cache_elem = a.cache_kind == kFp8 ? 1 : sizeof(T);
@@ -395,81 +378,6 @@ int run_cache_typed(const sm120n_qk_cache_args& in, int cache_kind, cudaStream_t
     case 128: return run_cache_kind<T, 128>(a, stream);
     default: return run_cache_kind<T, 256>(a, stream);
   }
-}
-
-int check_cache_args(const sm120n_qk_cache_args* a, int* cache_kind) {
-  if (a == nullptr) return fail(SM120N_ERR_INVALID_ARGUMENT, "args must be non-null");
-  if (a->struct_size != sizeof(sm120n_qk_cache_args)) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT,
-                "struct_size %u does not match this library's sm120n_qk_cache_args (%zu)",
-                a->struct_size, sizeof(sm120n_qk_cache_args));
-  }
-  if (dtype_size(a->dtype) == 0) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "supported dtypes are float16, bfloat16, and float32");
-  }
-  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) {
-    return fail(SM120N_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256 (got %lld)",
-                static_cast<long long>(a->head_dim));
-  }
-  if (a->rotary_dim < 16 || a->rotary_dim > a->head_dim || a->rotary_dim % 16 != 0) {
-    return fail(SM120N_ERR_UNSUPPORTED,
-                "rotary_dim must be a multiple of 16 in [16, head_dim] (got %lld)",
-                static_cast<long long>(a->rotary_dim));
-  }
-  if (a->rope_style != SM120N_ROPE_NEOX && a->rope_style != SM120N_ROPE_INTERLEAVED) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "unknown rope_style %d", a->rope_style);
-  }
-  if (a->cache_dtype != SM120N_CACHE_AUTO && a->cache_dtype != SM120N_CACHE_FP8_E4M3) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "unknown cache_dtype %d", a->cache_dtype);
-  }
-  if (a->tokens < 0 || a->query_heads < 0 || a->key_heads < 0 || a->rope_positions < 0) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT,
-                "tokens, head counts and rope_positions must be non-negative");
-  }
-  const int64_t heads = a->query_heads + a->key_heads;
-  if (heads > (1 << 20)) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "at most 2^20 heads per token are supported");
-  }
-  if (a->tokens > (int64_t{1} << 40) / std::max<int64_t>(1, heads)) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "too many tokens");
-  }
-  const bool store = a->key_cache != nullptr || a->value_cache != nullptr;
-  *cache_kind = !store ? kNoCache : a->cache_dtype == SM120N_CACHE_FP8_E4M3 ? kFp8 : kSameType;
-  if (a->tokens == 0 || heads == 0) return SM120N_OK;
-  if (a->query_token_stride < a->query_heads * a->head_dim ||
-      a->key_token_stride < a->key_heads * a->head_dim) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT,
-                "token strides must cover heads * head_dim elements (rows may not overlap)");
-  }
-  if ((a->query_heads > 0 && !a->query) || (a->key_heads > 0 && !a->key) || !a->query_weight ||
-      !a->key_weight || !a->positions || !a->cos_sin_cache) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "tensor pointers must be non-null");
-  }
-  if (store) {
-    if (!a->key_cache || !a->value_cache) {
-      return fail(SM120N_ERR_INVALID_ARGUMENT, "key_cache and value_cache go together");
-    }
-    if (a->key_heads > 0 && (!a->value || !a->slot_mapping)) {
-      return fail(SM120N_ERR_INVALID_ARGUMENT, "a KV store needs value and slot_mapping");
-    }
-    if (a->value_token_stride < a->key_heads * a->head_dim) {
-      return fail(SM120N_ERR_INVALID_ARGUMENT,
-                  "token strides must cover heads * head_dim elements (rows may not overlap)");
-    }
-    if (a->num_blocks < 0 || a->block_size < 1 || a->block_size > INT32_MAX ||
-        a->cache_block_stride < 0 || a->cache_slot_stride < 0 || a->cache_head_stride < 0) {
-      return fail(SM120N_ERR_INVALID_ARGUMENT,
-                  "cache geometry must have num_blocks >= 0, block_size >= 1 and "
-                  "non-negative strides");
-    }
-    if (a->num_blocks > (int64_t{1} << 31) / a->block_size) {
-      return fail(SM120N_ERR_INVALID_ARGUMENT, "num_blocks * block_size must be at most 2^31");
-    }
-    if (*cache_kind == kFp8 && (!a->k_scale || !a->v_scale)) {
-      return fail(SM120N_ERR_INVALID_ARGUMENT, "fp8 caches need k_scale and v_scale");
-    }
-  }
-  return SM120N_OK;
 }
 
 }  // namespace

@@ -229,4 +229,17 @@ __device__ __forceinline__ void load8_pairs(const float* p, float2* f) {
   }
 }
 
+// Eight fp8 bytes, element 0 lowest, at `p`.
+template <bool kVector>
+__device__ __forceinline__ void store_fp8_chunk(uint8_t* p, uint2 v) {
+  if constexpr (kVector) {
+    *reinterpret_cast<uint2*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = static_cast<uint8_t>(v.x >> (8 * i));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[4 + i] = static_cast<uint8_t>(v.y >> (8 * i));
+  }
+}
+
 }  // namespace sm120n

@@ -19,32 +19,16 @@
 // the C ABI in include/sm120norm_b200.h, on the tensors' device and on the
 // current PyTorch stream. No host synchronisation; only rms_norm and
 // fused_add_rms_norm allocate (their outputs).
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/extension.h>
-#include <torch/library.h>
-
 #include <vector>
 
-#include "sm120norm_b200.h"
+#include "binding_utils.h"
+
+using namespace sm120n_binding;
 
 namespace {
 
-int dtype_code(const torch::Tensor& t) {
-  switch (t.scalar_type()) {
-    case torch::kFloat32: return SM120N_F32;
-    case torch::kFloat16: return SM120N_F16;
-    case torch::kBFloat16: return SM120N_BF16;
-    default: return -1;
-  }
-}
-
 void raise_if_failed(int status) {
   TORCH_CHECK(status == SM120N_OK, sm120n_last_error());
-}
-
-void* current_stream() {
-  return static_cast<void*>(c10::cuda::getCurrentCUDAStream().stream());
 }
 
 void check_activation_and_weight(const torch::Tensor& input, const torch::Tensor& weight) {
@@ -246,36 +230,14 @@ TORCH_LIBRARY_IMPL(sm120_norm, CUDA, m) {
 // ---------------------------------------------------------------------------
 // Extensions
 // ---------------------------------------------------------------------------
-namespace {
-
-bool is_fp8_storage(const torch::Tensor& t) {
-  return t.scalar_type() == torch::kFloat8_e4m3fn || t.scalar_type() == torch::kByte;
-}
-
-// [tokens, heads, head_dim] with adjacent heads and elements; any token stride.
-void check_head_rows(const torch::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.dim() == 3, name, " must have shape [tokens, heads, head_dim]");
-  TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, name, " must have unit element stride");
-  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == t.size(2), name,
-              " heads must be adjacent (head stride == head_dim)");
-}
-
-int64_t token_stride(const torch::Tensor& t) {
-  return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
-}
-
-}  // namespace
-
-void b200_qk_norm_rope_cache(torch::Tensor query, torch::Tensor key,
-                             c10::optional<torch::Tensor> value, torch::Tensor query_weight,
-                             torch::Tensor key_weight, torch::Tensor positions,
-                             torch::Tensor cos_sin_cache, c10::optional<torch::Tensor> key_cache,
-                             c10::optional<torch::Tensor> value_cache,
-                             c10::optional<torch::Tensor> slot_mapping,
-                             c10::optional<torch::Tensor> k_scale,
-                             c10::optional<torch::Tensor> v_scale, bool is_neox,
-                             c10::string_view kv_cache_layout, double epsilon) {
+void sm120n_binding::fill_qk_cache_args(
+    sm120n_qk_cache_args& a, const torch::Tensor& query, const torch::Tensor& key,
+    const c10::optional<torch::Tensor>& value, const torch::Tensor& query_weight,
+    const torch::Tensor& key_weight, const torch::Tensor& cos_sin_cache,
+    const c10::optional<torch::Tensor>& key_cache, const c10::optional<torch::Tensor>& value_cache,
+    const c10::optional<torch::Tensor>& slot_mapping, const c10::optional<torch::Tensor>& k_scale,
+    const c10::optional<torch::Tensor>& v_scale, bool is_neox, c10::string_view kv_cache_layout,
+    double epsilon) {
   check_head_rows(query, "query");
   check_head_rows(key, "key");
   TORCH_CHECK(query.size(0) == key.size(0), "query and key token counts must match");
@@ -291,20 +253,15 @@ void b200_qk_norm_rope_cache(torch::Tensor query, torch::Tensor key,
   TORCH_CHECK(query_weight.scalar_type() == query.scalar_type() &&
                   key_weight.scalar_type() == query.scalar_type(),
               "Q/K weight dtypes must match activations");
-  TORCH_CHECK(positions.is_cuda() && positions.is_contiguous() &&
-                  positions.scalar_type() == torch::kInt64 && positions.numel() == query.size(0),
-              "positions must be contiguous CUDA int64 with one entry per token");
   TORCH_CHECK(cos_sin_cache.is_cuda() && cos_sin_cache.is_contiguous() &&
                   cos_sin_cache.scalar_type() == torch::kFloat32 && cos_sin_cache.dim() >= 1,
               "cos/sin cache must be a contiguous CUDA float32 tensor");
   const int64_t rotary_dim = cos_sin_cache.size(-1);
   const auto device = query.device();
   TORCH_CHECK(key.device() == device && query_weight.device() == device &&
-                  key_weight.device() == device && positions.device() == device &&
-                  cos_sin_cache.device() == device,
+                  key_weight.device() == device && cos_sin_cache.device() == device,
               "all tensors must be on the same CUDA device");
 
-  sm120n_qk_cache_args a{};
   a.struct_size = sizeof(a);
   a.dtype = dtype_code(query);
   a.tokens = query.size(0);
@@ -320,7 +277,6 @@ void b200_qk_norm_rope_cache(torch::Tensor query, torch::Tensor key,
   a.key_token_stride = token_stride(key);
   a.query_weight = query_weight.data_ptr();
   a.key_weight = key_weight.data_ptr();
-  a.positions = positions.data_ptr<int64_t>();
   a.cos_sin_cache = cos_sin_cache.data_ptr<float>();
   a.rope_positions = rotary_dim == 0 ? 0 : cos_sin_cache.numel() / rotary_dim;
   a.epsilon = static_cast<float>(epsilon);
@@ -380,7 +336,27 @@ void b200_qk_norm_rope_cache(torch::Tensor query, torch::Tensor key,
     a.cache_slot_stride = kc.stride(slot_axis);
     a.cache_head_stride = kc.stride(head_axis);
   }
-  c10::cuda::CUDAGuard guard(device);
+}
+
+void b200_qk_norm_rope_cache(torch::Tensor query, torch::Tensor key,
+                             c10::optional<torch::Tensor> value, torch::Tensor query_weight,
+                             torch::Tensor key_weight, torch::Tensor positions,
+                             torch::Tensor cos_sin_cache, c10::optional<torch::Tensor> key_cache,
+                             c10::optional<torch::Tensor> value_cache,
+                             c10::optional<torch::Tensor> slot_mapping,
+                             c10::optional<torch::Tensor> k_scale,
+                             c10::optional<torch::Tensor> v_scale, bool is_neox,
+                             c10::string_view kv_cache_layout, double epsilon) {
+  TORCH_CHECK(positions.is_cuda() && positions.is_contiguous() &&
+                  positions.scalar_type() == torch::kInt64 && positions.numel() == query.size(0),
+              "positions must be contiguous CUDA int64 with one entry per token");
+  TORCH_CHECK(positions.device() == query.device(), "all tensors must be on the same CUDA device");
+  sm120n_qk_cache_args a{};
+  fill_qk_cache_args(a, query, key, value, query_weight, key_weight, cos_sin_cache, key_cache,
+                     value_cache, slot_mapping, k_scale, v_scale, is_neox, kv_cache_layout,
+                     epsilon);
+  a.positions = positions.data_ptr<int64_t>();
+  c10::cuda::CUDAGuard guard(query.device());
   raise_if_failed(sm120n_qk_norm_rope_cache(&a, current_stream()));
 }
 

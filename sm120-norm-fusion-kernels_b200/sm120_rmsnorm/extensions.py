@@ -10,6 +10,9 @@ kernels' numerics (csrc/head_cache.cu, csrc/norm_quant.cu):
   any block size, and fp8 e4m3 caches with per-tensor scales. With
   head_dim = rotary_dim = 128, NEOX, a same-dtype NHD cache and dense inputs it
   is bit-identical to ``ops.fused_qk_rms_norm_rope_kv``.
+* :func:`qk_norm_mrope_cache_` -- the same with positions of several axes (time,
+  height and width of images and video), optionally out of place; rounded once
+  (csrc/head_mrope.cu).
 * :func:`rms_norm_static_fp8_quant`, :func:`fused_add_rms_norm_static_fp8_quant`,
   :func:`rms_norm_dynamic_per_token_quant` -- RMSNorm (after the optional
   residual add) with an fp8 e4m3 output: the row y is computed with the
@@ -66,6 +69,45 @@ def qk_norm_rope_cache_(
     torch.ops.sm120_norm_ext.qk_norm_rope_cache_(
         query, key, value, query_weight, key_weight, positions, cos_sin_cache, key_cache,
         value_cache, slot_mapping, k_scale, v_scale, is_neox, kv_cache_layout, epsilon)
+
+
+def qk_norm_mrope_cache_(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor | None,
+    query_weight: torch.Tensor,
+    key_weight: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin_cache: torch.Tensor,
+    sections: list[int],
+    key_cache: torch.Tensor | None = None,
+    value_cache: torch.Tensor | None = None,
+    slot_mapping: torch.Tensor | None = None,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    is_neox: bool = True,
+    interleaved_sections: bool = False,
+    kv_cache_layout: str = "NHD",
+    epsilon: float = 1e-6,
+    query_out: torch.Tensor | None = None,
+    key_out: torch.Tensor | None = None,
+) -> None:
+    """As :func:`qk_norm_rope_cache_`, with ``positions`` (int64 [axes, T], 1 to 4
+    axes, any axis stride) and ``sections`` (one entry per axis, adding up to half
+    the rotary width): the first ``sections[0]`` pairs of a head turn by axis 0,
+    the next ``sections[1]`` by axis 1, and so on; with ``interleaved_sections``
+    pair i turns by axis ``k = i % axes`` if ``k > 0`` and ``i < axes *
+    sections[k]``, else by axis 0. A token with a position outside the table on
+    any axis is left untouched. In place, or into ``query_out`` / ``key_out``
+    (shapes of the inputs, any token stride). Computed in fp32 and rounded once,
+    to the activation dtype and separately to an fp8 cache, so a result may
+    differ in its last place from :func:`qk_norm_rope_cache_`, which rounds after
+    each stage."""
+    _extension()
+    torch.ops.sm120_norm_ext.qk_norm_mrope_cache_(
+        query, key, value, query_weight, key_weight, positions, cos_sin_cache, sections,
+        key_cache, value_cache, slot_mapping, k_scale, v_scale, is_neox, interleaved_sections,
+        kv_cache_layout, epsilon, query_out, key_out)
 
 
 def rms_norm_static_fp8_quant(result: torch.Tensor, input: torch.Tensor, weight: torch.Tensor,
@@ -154,6 +196,14 @@ if _C is not None:
                                  cos_sin_cache, key_cache, value_cache, slot_mapping, k_scale,
                                  v_scale, is_neox=True, kv_cache_layout="NHD",
                                  epsilon=1e-6) -> None:
+        return None
+
+    @torch.library.register_fake("sm120_norm_ext::qk_norm_mrope_cache_")
+    def _qk_norm_mrope_cache_meta(query, key, value, query_weight, key_weight, positions,
+                                  cos_sin_cache, sections, key_cache=None, value_cache=None,
+                                  slot_mapping=None, k_scale=None, v_scale=None, is_neox=True,
+                                  interleaved_sections=False, kv_cache_layout="NHD",
+                                  epsilon=1e-6, query_out=None, key_out=None) -> None:
         return None
 
     @torch.library.register_fake("sm120_norm_ext::rms_norm_static_fp8_quant")
