@@ -34,6 +34,14 @@ SM120N_API int sm120s_abi_version(void);
 SM120N_API const char* sm120s_last_error(void);
 
 /*
+ * Number of bounded waits that expired in these kernels on the current device
+ * since the last reset. Zero in correct operation; a block that gave up left
+ * its rows unwritten. Both synchronise the current device.
+ */
+SM120N_API int sm120s_get_device_faults(uint32_t* out_count);
+SM120N_API int sm120s_reset_device_faults(void);
+
+/*
  * Plans one serving step. With c = max(context_lens[r], 0) tokens of request r
  * in the cache, q = max(query_lens[r], 0) new ones and B = block_size:
  *   held = ceil(c / B), want = ceil((c + q) / B), end_r = q_0 + ... + q_r

@@ -43,6 +43,13 @@ int check_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int
   return SM120N_OK;
 }
 
+// Whether the prefix runs on tensor memory: 256 rows and 128 keys to a tile
+// there, 64 and 64 otherwise.
+bool prefix_on_tensor_memory(const sm120s_decode_args& a) {
+  return a.head_dim <= 128 && a.cache_dtype == SM120N_CACHE_AUTO &&
+         block_fills_tiles(a.block_size) && a.num_blocks > 0;
+}
+
 struct Plan {
   int row_tiles;
   int own_grid;
@@ -100,11 +107,13 @@ int plan_decode(const sm120s_decode_args& a, Plan* plan) {
                            triples * most_tiles)));
   plan->prefix_splits = 0;
   if (a.prefix_blocks_count > 0) {
-    const int64_t row_tiles = (a.batch * group + 63) / 64;
-    const int64_t tiles = (a.prefix_blocks_count * a.block_size + 63) / 64;
+    const bool tc = prefix_on_tensor_memory(a);
+    const int64_t tile_rows = tc ? 256 : 64, tile_keys = tc ? 128 : 64;
+    const int64_t row_tiles = (a.batch * group + tile_rows - 1) / tile_rows;
+    const int64_t tiles = (a.prefix_blocks_count * a.block_size + tile_keys - 1) / tile_keys;
     const int64_t blocks = std::max<int64_t>(1, row_tiles * a.key_heads);
-    plan->prefix_splits = static_cast<int>(
-        std::max<int64_t>(1, std::min<int64_t>(tiles, 2 * dev.sm_count / blocks)));
+    plan->prefix_splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>(tiles, (tc ? 1 : 2) * dev.sm_count / blocks)));
   }
   size_t at = (static_cast<size_t>(a.batch + 1) * sizeof(int32_t) + 15) / 16 * 16;
   const size_t own_rows = static_cast<size_t>(triples + plan->own_grid) * 16;
@@ -169,7 +178,10 @@ extern "C" int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
   a.key_heads = static_cast<int32_t>(in.key_heads);
   a.group = static_cast<int32_t>(group);
   a.scale_log2 = in.scale * kLog2e;
-  return launch_prompt_mma(a, in.dtype, static_cast<int>(in.head_dim), static_cast<cudaStream_t>(stream));
+  const int head_dim = static_cast<int>(in.head_dim);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return head_dim <= 128 ? launch_prompt_tc(a, in.dtype, head_dim, s)
+                         : launch_prompt_mma(a, in.dtype, head_dim, s);
 }
 
 extern "C" int sm120s_paged_decode_workspace(const sm120s_decode_args* args, size_t* bytes) {
@@ -257,7 +269,8 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
   const int head_dim = static_cast<int>(in.head_dim);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.prefix_splits > 0) {
-    rc = launch_prefix_mma(a, in.dtype, in.cache_dtype, head_dim, s);
+    rc = prefix_on_tensor_memory(in) ? launch_prefix_tc(a, in.dtype, head_dim, s)
+                                     : launch_prefix_mma(a, in.dtype, in.cache_dtype, head_dim, s);
     if (rc != SM120N_OK) return rc;
   }
   rc = launch_own_mma(a, in.dtype, in.cache_dtype, head_dim, s);

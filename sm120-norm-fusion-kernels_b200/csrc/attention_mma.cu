@@ -26,7 +26,7 @@
 #include <algorithm>
 
 #include "attention.h"
-#include "device_utils.cuh"
+#include "attention_utils.cuh"
 
 namespace sm120n {
 namespace {
@@ -83,12 +83,6 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int kPending>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Two e4m3 bytes (low half of `b`) as two fp16 values.
@@ -373,42 +367,6 @@ struct Worker {
     return Pack<T>::f32_to_word(x, y);
   }
 
-  // One row of a prompt by plain arithmetic, one warp, keys one by one: used
-  // for blocks of rows that have an infinite or NaN value among the keys that
-  // some of them must not see (a matrix product would multiply it by zero).
-  __device__ __noinline__ void plain_row(const Piece& p, int64_t row, float scale_log2, TQ* out) {
-    const int64_t r = p.first_row + row;
-    const int64_t last = min(r / a.group, static_cast<int64_t>(p.key_last) - 1);
-    const TQ* q = static_cast<const TQ*>(a.query) + row_offset<kPass>(a, p, row, a.query_stride, D);
-    float acc[D / kWarpSize] = {};
-    float top = -INFINITY, sum = 0.0f;
-    for (int64_t j = 0; j <= last; ++j) {
-      const int64_t head = static_cast<int64_t>(p.kv_head) * D;
-      const TQ* k = static_cast<const TQ*>(a.key) + (p.token0 + j) * a.key_stride + head;
-      const TQ* v = static_cast<const TQ*>(a.value) + (p.token0 + j) * a.value_stride + head;
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / kWarpSize; ++i) {
-        s += static_cast<float>(q[lane + i * kWarpSize]) * static_cast<float>(k[lane + i * kWarpSize]);
-      }
-#pragma unroll
-      for (int d = kWarpSize / 2; d > 0; d /= 2) s += __shfl_xor_sync(kFullMask, s, d);
-      s *= scale_log2;
-      const float next = fmaxf(top, s);
-      const float keep = next == -INFINITY ? 1.0f : exp2_approx(top - next);
-      const float e = next == -INFINITY ? 0.0f : exp2_approx(s - next);
-      top = next;
-      sum = sum * keep + e;
-#pragma unroll
-      for (int i = 0; i < D / kWarpSize; ++i) {
-        acc[i] = acc[i] * keep + e * static_cast<float>(v[lane + i * kWarpSize]);
-      }
-    }
-    TQ* to = out + row_offset<kPass>(a, p, row, a.out_stride, D);
-#pragma unroll
-    for (int i = 0; i < D / kWarpSize; ++i) to[lane + i * kWarpSize] = static_cast<TQ>(acc[i] / sum);
-  }
-
   // Whether a value of the tile in `stage` is infinite or NaN (16-bit tiles, whole block).
   __device__ __forceinline__ bool unsafe_values(int stage) {
     constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
@@ -549,63 +507,6 @@ struct Worker {
 
 // ---- prompts -----------------------------------------------------------------
 
-// The sequence and tile of its rows that block `index` of the tile list works
-// on: tiles of `rows` (token, head) rows, sequence after sequence. Whole block.
-struct SequenceTile {
-  int64_t first_token;
-  int64_t length;
-  int64_t tile;  // -1: the list is shorter
-  int64_t tiles;
-};
-
-__device__ __forceinline__ int64_t clamp_start(int32_t v, int64_t tokens) {
-  return min(max(static_cast<int64_t>(v), int64_t{0}), tokens);
-}
-
-template <int kBlockThreads>
-__device__ __forceinline__ SequenceTile find_tile(const int32_t* query_start, int sequences,
-                                                  int64_t tokens, int group, int rows,
-                                                  int64_t index) {
-  __shared__ int64_t totals[kBlockThreads / kWarpSize];
-  __shared__ SequenceTile found;
-  const int lane = threadIdx.x & (kWarpSize - 1);
-  const int warp = threadIdx.x / kWarpSize;
-  if (threadIdx.x == 0) found.tile = -1;
-  int64_t before = 0;
-  for (int base = 0; base < sequences; base += kBlockThreads) {
-    const int i = base + threadIdx.x;
-    int64_t first = 0, length = 0;
-    if (i < sequences) {
-      first = clamp_start(query_start[i], tokens);
-      length = max(clamp_start(query_start[i + 1], tokens) - first, int64_t{0});
-    }
-    const int64_t mine = (length * group + rows - 1) / rows;
-    int64_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < kWarpSize; d *= 2) {
-      const int64_t x = __shfl_up_sync(kFullMask, upto, d);
-      if (lane >= d) upto += x;
-    }
-    __syncthreads();
-    if (lane == kWarpSize - 1) totals[warp] = upto;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < kBlockThreads / kWarpSize; ++w) {
-      if (w < warp) upto += totals[w];
-      all += totals[w];
-    }
-    upto += before;
-    if (index < upto && index >= upto - mine) {
-      // the last rows of a sequence have the most keys: first
-      found = SequenceTile{first, length, upto - 1 - index, mine};
-    }
-    before += all;
-    if (index < before) break;
-  }
-  __syncthreads();
-  return found;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) prompt_mma_kernel(PromptArgs a) {
   using F = Form<T, false, D, kPrompt>;
@@ -626,7 +527,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_mma_kernel(PromptArgs a) {
   p.token0 = tile.first_token;
   T* out = static_cast<T*>(a.out);
   if (w.run(p, a.scale_log2)) {
-    for (int row = w.warp; row < p.rows; row += kWarps) w.plain_row(p, row, a.scale_log2, out);
+    for (int row = w.warp; row < p.rows; row += kWarps) {
+      plain_prompt_row<T, D>(a, p.token0, p.first_row + row, p.kv_head);
+    }
     return;
   }
 #pragma unroll

@@ -1,0 +1,757 @@
+// attention_tc.cu -- attention on the fifth-generation tensor cores, for head
+// sizes 64 and 128: causal attention of packed prompts, and the shared prefix
+// of a decode batch.
+//
+// A block works on 256 rows of one key head -- (token, head of the group) of a
+// prompt, or (request, head of the group) of a decode batch -- as two tiles of
+// 128, against tiles of 128 keys:
+//   S_i = Q_i K^T      tcgen05.mma, both operands in shared memory -> TMEM
+//   P_i = 2^(scale S_i - m_i)   one thread per row; TMEM -> registers -> TMEM
+//   O_i += P_i V       tcgen05.mma, P from TMEM, V in shared memory -> TMEM
+// S_i and P_i share 128 columns of tensor memory, O_i has D of its own: at
+// D = 128 all 512 columns. While the 128 threads of one tile exponentiate,
+// the tensor cores work on the other tile. Both products of a tile pair take
+// 2048 cycles at D = 128, and so do the pair's 32768 exponentials on the
+// special-function units (16 a cycle): neither may wait for the other.
+//
+// Warps 0-3 and 4-7: softmax and epilogue of tile 0 and 1, a thread to a row, so
+// that no reduction crosses threads. Warp 8: issues every matrix instruction.
+// Warp 9: loads K and V tiles by TMA into kStages shared-memory stages. Warps
+// 10-11 (prompts): look for infinite or NaN values in the V tiles that some
+// rows must not see, where a product would multiply them by zero; a block
+// that meets one does its rows by plain arithmetic instead.
+//
+// The running maximum of a row follows the true one only when that has grown
+// by more than 2^8 (kSlack): p then stays below 256, exact enough in 16 bits
+// at any scale, and O is hardly ever rescaled; the softmax threads do it
+// themselves, between S_j (whose completion implies that of the product
+// before it) and the release of P_j.
+//
+// Every wait on an mbarrier is bounded; one that runs out is counted
+// (sm120s_get_device_faults) and ends the block without results.
+#include <algorithm>
+
+#include "attention.h"
+#include "attention_utils.cuh"
+#include "tensor_core.cuh"
+#include "tensor_map.h"
+
+namespace sm120n {
+
+__device__ unsigned int g_attention_expired_waits = 0;
+
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kTileKeys = 128;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kMmaWarp = 8;
+constexpr int kLoadWarp = 9;
+constexpr int kGuardWarps = 2;  // 10, 11
+constexpr int kThreads = 12 * kWarpSize;
+constexpr uint32_t kBoxBytes = kTileKeys * 128;  // 64 elements of 128 rows
+constexpr float kSlack = 8.0f;                   // log2 of how far a maximum may lag
+
+enum Pass : int { kPrompt, kPrefix };
+
+template <int D>
+struct TcShape {
+  static constexpr int kStages = D == 64 ? 8 : 4;  // K and V tiles alternate: even
+  static constexpr uint32_t kTileBytes = kTileKeys * D * 2;
+  static constexpr uint32_t kQBytes = kTileRows * D * 2;
+  static constexpr size_t kSmem = 2 * kQBytes + kStages * kTileBytes + 1024;
+  static constexpr uint32_t kOutColumn = 256;  // of tile 0; tile 1 is D further
+  static constexpr uint32_t kTmemColumns = 512;
+};
+
+// Instruction descriptor of tcgen05.mma.kind::f16: fp32 accumulator (bit 4), the
+// operands' type (bits 7 and 10: 0 fp16, 1 bf16), B with its outer dimension
+// contiguous (bit 16), N >> 3 at bit 17, M >> 4 at bit 24.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool outer_b) {
+  const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | (outer_b ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileRows >> 4) << 24);
+}
+
+// Descriptor of a V tile as B of the second product: d contiguous (64 of them
+// in a 128-byte swizzled row, the next 64 a box further: leading offset), keys
+// in groups of 8 rows, 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t value_descriptor(const void* tile) {
+  const uint64_t address = shared_address(tile);
+  return ((address & 0x3FFFFull) >> 4) | (uint64_t{kBoxBytes >> 4} << 16) |
+         (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+
+__device__ __forceinline__ void mma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                              uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 columns of this thread's TMEM lane; the values may be used after tmem_wait_load.
+__device__ __forceinline__ void tmem_load32_async(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
+        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+
+// Waits for this thread's TMEM loads; the empty statements keep every use of
+// the loaded values behind the wait.
+template <int N>
+__device__ __forceinline__ void tmem_wait_load(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y,
+                                            int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(shared_address(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(shared_address(bar))
+      : "memory");
+}
+
+template <int kRegisters>
+__device__ __forceinline__ void grow_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+template <int kRegisters>
+__device__ __forceinline__ void shrink_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+// 384 threads launch with 168 registers each: 2 x 208 + 88 = 3 x 168.
+constexpr int kSoftmaxRegisters = 208;
+constexpr int kOtherRegisters = 88;
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// What a block works on.
+struct Work {
+  int64_t first_row;  // of the sequence, or of the batch
+  int64_t rows;       // up to 256
+  int64_t token0;     // kPrompt: the sequence's first token
+  int key_first;      // kPrefix: first key of its part of the prefix
+  int key_last;
+  int kv_head;
+  int split;  // kPrefix
+};
+
+struct Barriers {
+  uint64_t full[8];
+  uint64_t empty[8];
+  uint64_t q_full;
+  uint64_t s_full[2];
+  uint64_t p_ready[2];
+  uint64_t o_full[2];
+  uint64_t guarded;
+  uint64_t done;
+};
+
+struct Control {
+  Barriers bar;
+  uint32_t tmem;
+  int aborted;
+  int unsafe;  // a value that some rows must not see is infinite or NaN
+  int holes;   // kPrefix: a block of the prefix does not exist
+};
+
+__device__ __forceinline__ bool wait_in(Control& c, uint64_t* bar, uint32_t parity) {
+  if (mbarrier_wait_bounded(bar, parity)) return true;
+  atomicAdd(&g_attention_expired_waits, 1u);
+  atomicExch(&c.aborted, 1);
+  return false;
+}
+
+// Offset of a row of q or out, in elements.
+template <int kPass, int D, typename Args>
+__device__ __forceinline__ int64_t row_at(const Args& a, const Work& w, int64_t row, int64_t stride) {
+  const int64_t r = w.first_row + row;
+  const int64_t token = r / a.group;
+  const int64_t head = static_cast<int64_t>(w.kv_head) * a.group + (r - token * a.group);
+  return (w.token0 + token) * stride + head * D;
+}
+
+template <typename T, int D, int kPass, typename Args>
+__device__ __forceinline__ void attend(const Args& a, const Work& w, const CUtensorMap* key_map,
+                                       const CUtensorMap* value_map, Control& c, unsigned char* smem) {
+  using S = TcShape<D>;
+  constexpr int kStages = S::kStages;
+  const int warp = threadIdx.x / kWarpSize;
+  const int lane = threadIdx.x & (kWarpSize - 1);
+  unsigned char* stages = smem + 2 * S::kQBytes;
+
+  // key tiles of each row tile
+  int n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t rows = min(w.rows - i * kTileRows, int64_t{kTileRows});
+    if (rows <= 0) {
+      n[i] = 0;
+    } else if constexpr (kPass == kPrompt) {
+      n[i] = static_cast<int>((w.first_row + i * kTileRows + rows - 1) / a.group / kTileKeys + 1);
+    } else {
+      n[i] = (w.key_last - w.key_first + kTileKeys - 1) / kTileKeys;
+    }
+  }
+  const int tiles = max(n[0], n[1]);
+
+  if (warp < kSoftmaxWarps) {
+    grow_registers<kSoftmaxRegisters>();
+    const int i = warp / 4;
+    const int row = i * kTileRows + (warp % 4) * kWarpSize + lane;
+    const T* query = static_cast<const T*>(a.query);
+    // Q of the warp's 32 rows into the swizzled operand layout
+    {
+      constexpr int kChunks = D / 8;
+#pragma unroll 8
+      for (int t = lane; t < kWarpSize * kChunks; t += kWarpSize) {
+        const int r = (warp % 4) * kWarpSize + t / kChunks;
+        const int chunk = t % kChunks;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (i * kTileRows + r < w.rows) {
+          v = load16(query + row_at<kPass, D>(a, w, i * kTileRows + r, a.query_stride) + chunk * 8);
+        }
+        *reinterpret_cast<uint4*>(smem + i * S::kQBytes + (chunk / 8) * kBoxBytes + r * 128 +
+                                  ((chunk % 8) ^ (r & 7)) * 16) = v;
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&c.bar.q_full);
+    }
+    const uint32_t lane_base = c.tmem + (static_cast<uint32_t>((warp % 4) * kWarpSize) << 16);
+    const uint32_t s_at = lane_base + i * kTileKeys;
+    const uint32_t o_at = lane_base + S::kOutColumn + i * D;
+    const float scale = a.scale_log2;
+    float top = -INFINITY;   // true maximum of the raw scores
+    float base = 0.0f;       // scale * the maximum in use
+    float sum = 0.0f;
+    // last key of the row, counted from the first key tile's first
+    const int64_t limit = kPass == kPrompt ? (w.first_row + row) / a.group
+                                           : int64_t{w.key_last} - w.key_first - 1;
+    const int64_t first_limit =  // smallest of the tile: tiles behind it need no mask
+        kPass == kPrompt ? (w.first_row + i * kTileRows) / a.group : limit;
+    bool ok = true;
+    for (int j = 0; j < n[i]; ++j) {
+      if (!wait_in(c, &c.bar.s_full[i], j & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t raw[kTileKeys];
+#pragma unroll
+      for (int q = 0; q < kTileKeys / 32; ++q) tmem_load32_async(s_at + 32 * q, raw + 32 * q);
+      tmem_wait_load<kTileKeys>(raw);
+      float* s = reinterpret_cast<float*>(raw);
+      const int64_t key0 = int64_t{j} * kTileKeys;
+      if (key0 + kTileKeys - 1 > first_limit) {
+        const int last = static_cast<int>(min(limit - key0, int64_t{kTileKeys}));
+#pragma unroll
+        for (int k = 0; k < kTileKeys; ++k) {
+          if (k > last) s[k] = -INFINITY;
+        }
+      }
+      if constexpr (kPass == kPrefix) {
+        if (c.holes) {
+#pragma unroll
+          for (int k = 0; k < kTileKeys; ++k) {
+            const int64_t key = min(w.key_first + key0 + k, int64_t{a.prefix_tokens} - 1);
+            const int id = a.prefix_blocks[key / a.kv.block_size];
+            if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.kv.num_blocks)) s[k] = -INFINITY;
+          }
+        }
+      }
+      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+      for (int k = 4; k < kTileKeys; k += 8) {
+        m0 = max3(m0, s[k], s[k + 1]);
+        m1 = max3(m1, s[k + 2], s[k + 3]);
+        if (k + 4 < kTileKeys) {
+          m2 = max3(m2, s[k + 4], s[k + 5]);
+          m3 = max3(m3, s[k + 6], s[k + 7]);
+        }
+      }
+      const float next = fmaxf(max3(m0, m1, m2), fmaxf(m3, top));
+      const bool lags = (next - top) * scale > kSlack;  // also where top is still -inf
+      if (__any_sync(kFullMask, lags)) {
+        const float moved = lags ? next * scale : base;
+        const float keep = lags ? exp2_approx(top == -INFINITY ? -INFINITY : base - moved) : 1.0f;
+        if (j > 0) {
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            tmem_load32_async(o_at + 32 * q, o);
+            tmem_wait_load<32>(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+            tmem_store32(o_at + 32 * q, o);
+          }
+        }
+        sum *= keep;
+        base = moved;
+        if (lags) top = next;
+      }
+      const float2 factor = make_float2(scale, scale);
+      const float2 shift = make_float2(-base, -base);
+      float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t p[32];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const int at = 64 * q + 2 * k;
+          float2 x = __ffma2_rn(make_float2(s[at], s[at + 1]), factor, shift);
+          float2 y = __ffma2_rn(make_float2(s[at + 2], s[at + 3]), factor, shift);
+          x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          sum_a = __fadd2_rn(sum_a, x);
+          sum_b = __fadd2_rn(sum_b, y);
+          p[k] = Pack<T>::f32_to_word(x.x, x.y);
+          p[k + 1] = Pack<T>::f32_to_word(y.x, y.y);
+        }
+        tmem_store32(s_at + 32 * q, p);
+      }
+      sum_a = __fadd2_rn(sum_a, sum_b);
+      sum += sum_a.x + sum_a.y;
+      tmem_wait_store();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&c.bar.p_ready[i]);
+    }
+    if (ok && n[i] > 0) ok = wait_in(c, &c.bar.o_full[i], 0);
+    if constexpr (kPass == kPrompt) {
+      if (ok) ok = wait_in(c, &c.bar.guarded, 0);
+    }
+    ok = ok && !*reinterpret_cast<volatile int*>(&c.aborted);
+    tc_fence_after();
+    if (ok && n[i] > 0) {
+      if constexpr (kPass == kPrompt) {
+        if (*reinterpret_cast<volatile int*>(&c.unsafe)) {
+          for (int r = 0; r < kWarpSize; ++r) {
+            const int at = row - lane + r;
+            if (at < w.rows) plain_prompt_row<T, D>(a, w.token0, w.first_row + at, w.kv_head);
+          }
+        } else {
+          const float inv = 1.0f / sum;
+          T* out = static_cast<T*>(a.out) + (row < w.rows ? row_at<kPass, D>(a, w, row, a.out_stride) : 0);
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            tmem_load32_async(o_at + 32 * q, o);
+            tmem_wait_load<32>(o);
+            if (row < w.rows) {
+              uint32_t words[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                words[k] = Pack<T>::f32_to_word(__uint_as_float(o[2 * k]) * inv,
+                                                __uint_as_float(o[2 * k + 1]) * inv);
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                store16(out + 32 * q + 8 * k, make_uint4(words[4 * k], words[4 * k + 1],
+                                                         words[4 * k + 2], words[4 * k + 3]));
+              }
+            }
+          }
+        }
+      } else {
+        const int64_t r = w.first_row + row;
+        const int64_t request = r / a.group;
+        const int64_t at = (static_cast<int64_t>(w.split) * a.batch + request) * a.query_heads +
+                           static_cast<int64_t>(w.kv_head) * a.group + (r - request * a.group);
+        if (row < w.rows) {
+          a.prefix_state[at] = make_float2(top == -INFINITY ? -INFINITY : base, sum);
+        }
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          tmem_load32_async(o_at + 32 * q, o);
+          tmem_wait_load<32>(o);
+          if (row < w.rows) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              *reinterpret_cast<uint4*>(a.prefix_values + at * D + 32 * q + 4 * k) =
+                  make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    shrink_registers<kOtherRegisters>();
+    if (warp == kMmaWarp && lane == 0) {
+      constexpr uint32_t kScore = instruction<T>(kTileKeys, false);
+      constexpr uint32_t kValue = instruction<T>(D, true);
+      auto full = [&](int t) { return wait_in(c, &c.bar.full[t % kStages], (t / kStages) & 1); };
+      auto score = [&](int i, int j) {
+        const uint64_t q = smem_descriptor(smem + i * S::kQBytes);
+        const uint64_t k = smem_descriptor(stages + (2 * j % kStages) * S::kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          // 16 elements along d: 32 bytes inside a box, then the next box
+          const uint32_t step = (kk / 4) * (kBoxBytes >> 4) + 2 * (kk % 4);
+          mma_bf16(c.tmem + i * kTileKeys, q + step, k + step, kScore, kk != 0);
+        }
+        mma_commit(&c.bar.s_full[i]);
+      };
+      auto weigh = [&](int i, int j) {
+        const uint64_t v = value_descriptor(stages + ((2 * j + 1) % kStages) * S::kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < kTileKeys / 16; ++kk) {
+          mma_from_tmem(c.tmem + S::kOutColumn + i * D, c.tmem + i * kTileKeys + 8 * kk,
+                        v + kk * (2048 >> 4), kValue, (j | kk) != 0);
+        }
+        if (j == n[i] - 1) mma_commit(&c.bar.o_full[i]);
+      };
+      bool ok = wait_in(c, &c.bar.q_full, 0) && (tiles == 0 || full(0));
+      if (ok && tiles > 0) {
+        tc_fence_after();
+        for (int i = 0; i < 2; ++i) {
+          if (n[i] > 0) score(i, 0);
+        }
+        mma_commit(&c.bar.empty[0]);
+      }
+      for (int j = 0; ok && j < tiles; ++j) {
+        const bool more = j + 1 < tiles;
+        ok = full(2 * j + 1) && (!more || full(2 * j + 2));
+        if (!ok) break;
+        for (int i = 0; i < 2; ++i) {
+          if (j >= n[i]) continue;
+          if (!wait_in(c, &c.bar.p_ready[i], j & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          weigh(i, j);
+          if (j + 1 < n[i]) score(i, j + 1);
+        }
+        if (!ok) break;
+        mma_commit(&c.bar.empty[(2 * j + 1) % kStages]);
+        if (more) mma_commit(&c.bar.empty[(2 * j + 2) % kStages]);
+      }
+      mma_commit(&c.bar.done);
+    } else if (warp == kLoadWarp) {
+      for (int t = 0; t < 2 * tiles; ++t) {
+        const int stage = t % kStages;
+        bool ok = true;
+        if (lane == 0) {
+          ok = !*reinterpret_cast<volatile int*>(&c.aborted);
+          if (ok && t >= kStages) ok = wait_in(c, &c.bar.empty[stage], (t / kStages - 1) & 1);
+          if (ok) mbarrier_arrive_expect_tx(&c.bar.full[stage], S::kTileBytes);
+        }
+        if (!__shfl_sync(kFullMask, ok, 0)) break;
+        unsigned char* to = stages + stage * S::kTileBytes;
+        const CUtensorMap* map = t & 1 ? value_map : key_map;
+        const int key0 = (t / 2) * kTileKeys;
+        if constexpr (kPass == kPrompt) {
+          if (lane == 0) {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              tma_load_2d(to + h * kBoxBytes, map, w.kv_head * D + 64 * h,
+                          static_cast<int>(w.token0) + key0, &c.bar.full[stage]);
+            }
+          }
+        } else {
+          // one box to a block of the cache (or 128 slots of a larger one); a
+          // lane to a box. Blocks that do not exist, and what is behind the
+          // end, lie outside the map and arrive as zeros.
+          const int box = min(a.kv.block_size, kTileKeys);
+          for (int b = lane; b < kTileKeys / box; b += kWarpSize) {
+            const int64_t key = int64_t{w.key_first} + key0 + b * box;
+            int id = a.kv.num_blocks, slot = 0;
+            if (key < w.key_last) {
+              const int block = static_cast<int>(key / a.kv.block_size);
+              slot = static_cast<int>(key - static_cast<int64_t>(block) * a.kv.block_size);
+              id = a.prefix_blocks[block];
+              if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.kv.num_blocks)) id = a.kv.num_blocks;
+            }
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              tma_load_4d(to + h * kBoxBytes + b * box * 128, map, 64 * h, slot, w.kv_head, id,
+                          &c.bar.full[stage]);
+            }
+          }
+        }
+      }
+    } else if (kPass == kPrompt && warp > kLoadWarp) {
+      // V tiles that reach past the block's first row's last key
+      constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+      const int64_t first_limit = w.first_row / a.group;
+      bool bad = false;
+      for (int j = 0; j < tiles; ++j) {
+        const int stage = (2 * j + 1) % kStages;
+        if (!wait_in(c, &c.bar.full[stage], ((2 * j + 1) / kStages) & 1)) break;
+        if (int64_t{j + 1} * kTileKeys - 1 > first_limit) {
+          const uint4* v = reinterpret_cast<const uint4*>(stages + stage * S::kTileBytes);
+#pragma unroll 4
+          for (int t = (warp - kLoadWarp - 1) * kWarpSize + lane;
+               t < static_cast<int>(S::kTileBytes / 16); t += kGuardWarps * kWarpSize) {
+            const uint4 x = v[t];
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              bad |= (words[k] & kExponent) == kExponent || ((words[k] >> 16) & kExponent) == kExponent;
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&c.bar.empty[stage]);
+      }
+      if (bad) *reinterpret_cast<volatile int*>(&c.unsafe) = 1;
+      __threadfence_block();
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&c.bar.guarded);
+    }
+  }
+  __syncwarp();
+}
+
+// Set-up and release around attend(): barriers, tensor memory.
+template <int D>
+__device__ __forceinline__ void open_block(Control& c, bool guarded) {
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < TcShape<D>::kStages; ++s) {
+      mbarrier_init(&c.bar.full[s], 1);
+      mbarrier_init(&c.bar.empty[s], 1 + (guarded && (s & 1) ? kGuardWarps : 0));
+    }
+    mbarrier_init(&c.bar.q_full, kSoftmaxWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbarrier_init(&c.bar.s_full[i], 1);
+      mbarrier_init(&c.bar.p_ready[i], 4);
+      mbarrier_init(&c.bar.o_full[i], 1);
+    }
+    mbarrier_init(&c.bar.guarded, kGuardWarps);
+    mbarrier_init(&c.bar.done, 1);
+    c.aborted = 0;
+    c.unsafe = 0;
+    c.holes = 0;
+    fence_mbarrier_init();
+  }
+  if (threadIdx.x / kWarpSize == kMmaWarp) tmem_alloc(&c.tmem, TcShape<D>::kTmemColumns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+}
+
+template <int D>
+__device__ __forceinline__ void close_block(Control& c) {
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x / kWarpSize == kMmaWarp) {
+    // the issuer's last commit: no matrix instruction is still at work
+    if ((threadIdx.x & (kWarpSize - 1)) == 0) {
+      mbarrier_wait_bounded(&c.bar.done, 0);
+    }
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(c.tmem, TcShape<D>::kTmemColumns);
+  }
+  if (c.aborted && threadIdx.x == kLoadWarp * kWarpSize) {
+    // an expired wait: give loads that are still on their way a bounded time to land
+    for (int s = 0; s < TcShape<D>::kStages; ++s) {
+      for (uint32_t p = 0; p < 2; ++p) mbarrier_wait_limited(&c.bar.full[s], p, 1u << 16);
+    }
+  }
+}
+
+__device__ __forceinline__ unsigned char* aligned_tiles(unsigned char* p) {
+  return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t{1023});
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ CUtensorMap key_map,
+                     const __grid_constant__ CUtensorMap value_map,
+                     const __grid_constant__ PromptArgs a) {
+  extern __shared__ unsigned char dynamic_smem[];
+  __shared__ Control control;
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  const SequenceTile tile = find_tile<kThreads>(a.query_start, a.sequences, a.tokens, a.group,
+                                                2 * kTileRows, blockIdx.x / a.key_heads);
+  if (tile.tile < 0) return;
+  open_block<D>(control, true);
+  Work w{};
+  w.first_row = tile.tile * 2 * kTileRows;
+  w.rows = min(int64_t{2 * kTileRows}, tile.length * a.group - w.first_row);
+  w.token0 = tile.first_token;
+  w.kv_head = static_cast<int>(blockIdx.x % a.key_heads);
+  attend<T, D, kPrompt>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
+  close_block<D>(control);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_tc_kernel(const __grid_constant__ CUtensorMap key_map,
+                     const __grid_constant__ CUtensorMap value_map,
+                     const __grid_constant__ DecodeArgs a) {
+  extern __shared__ unsigned char dynamic_smem[];
+  __shared__ Control control;
+  open_block<D>(control, false);
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  Work w{};
+  w.first_row = static_cast<int64_t>(blockIdx.x) * 2 * kTileRows;
+  w.rows = min(int64_t{2 * kTileRows}, static_cast<int64_t>(a.batch) * a.group - w.first_row);
+  w.kv_head = blockIdx.y;
+  w.split = blockIdx.z;
+  const int64_t tiles = (a.prefix_tokens + kTileKeys - 1) / kTileKeys;
+  w.key_first = static_cast<int>(tiles * w.split / a.prefix_splits * kTileKeys);
+  w.key_last = static_cast<int>(min(tiles * (w.split + 1) / a.prefix_splits * kTileKeys,
+                                    int64_t{a.prefix_tokens}));
+  bool holes = false;
+  for (int b = w.key_first / a.kv.block_size + threadIdx.x;
+       b <= (w.key_last - 1) / a.kv.block_size; b += kThreads) {
+    holes |= static_cast<uint32_t>(a.prefix_blocks[b]) >= static_cast<uint32_t>(a.kv.num_blocks);
+  }
+  if (__syncthreads_or(holes) && threadIdx.x == 0) control.holes = 1;
+  __syncthreads();
+  attend<T, D, kPrefix>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
+  close_block<D>(control);
+}
+
+// ---- host ----------------------------------------------------------------------
+template <typename T>
+constexpr CUtensorMapDataType map_type() {
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// A map with boxes of 64 elements (128-byte swizzle) x `rows` of dimension 1.
+template <typename T>
+int encode_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
+               const cuuint64_t* byte_strides, int rows) {
+  int rc = SM120N_OK;
+  auto encode = tensor_map_encoder(&rc);
+  if (rc != SM120N_OK) return rc;
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, map_type<T>(), static_cast<cuuint32_t>(rank), const_cast<void*>(base),
+                            dims, byte_strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(SM120N_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  }
+  return SM120N_OK;
+}
+
+template <typename T, int D>
+int run_prompt(const PromptArgs& a, cudaStream_t stream) {
+  using S = TcShape<D>;
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.key_heads) * D,
+                                static_cast<cuuint64_t>(a.tokens)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(i ? a.value_stride : a.key_stride) * 2};
+    const int rc = encode_map<T>(&maps[i], i ? a.value : a.key, 2, dims, strides, kTileKeys);
+    if (rc != SM120N_OK) return rc;
+  }
+  auto kernel = prompt_tc_kernel<T, D>;
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
+  if (rc != SM120N_OK) return rc;
+  const int64_t tiles = (a.tokens * a.group + 2 * kTileRows - 1) / (2 * kTileRows) + a.sequences;
+  return launch(kernel, dim3(static_cast<unsigned>(tiles * a.key_heads)), dim3(kThreads), S::kSmem,
+                stream, maps[0], maps[1], a);
+}
+
+template <typename T, int D>
+int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
+  using S = TcShape<D>;
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(a.kv.block_size),
+                                static_cast<cuuint64_t>(a.key_heads),
+                                static_cast<cuuint64_t>(a.kv.num_blocks)};
+    // a dimension of one may have no stride of its own
+    auto bytes = [](int64_t stride) { return static_cast<cuuint64_t>(std::max<int64_t>(stride * 2, 16)); };
+    const cuuint64_t strides[3] = {bytes(a.kv.slot_stride), bytes(a.kv.head_stride),
+                                   bytes(a.kv.block_stride)};
+    const int rc = encode_map<T>(&maps[i], i ? a.kv.value : a.kv.key, 4, dims, strides,
+                                 std::min(a.kv.block_size, kTileKeys));
+    if (rc != SM120N_OK) return rc;
+  }
+  auto kernel = prefix_tc_kernel<T, D>;
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
+  if (rc != SM120N_OK) return rc;
+  const int64_t tiles = (static_cast<int64_t>(a.batch) * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
+  return launch(kernel,
+                dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.key_heads),
+                     static_cast<unsigned>(a.prefix_splits)),
+                dim3(kThreads), S::kSmem, stream, maps[0], maps[1], a);
+}
+
+}  // namespace
+
+int launch_prompt_tc(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream) {
+  if (head_dim == 64) {
+    return dtype == SM120N_F16 ? run_prompt<__half, 64>(a, stream)
+                               : run_prompt<__nv_bfloat16, 64>(a, stream);
+  }
+  return dtype == SM120N_F16 ? run_prompt<__half, 128>(a, stream)
+                             : run_prompt<__nv_bfloat16, 128>(a, stream);
+}
+
+int launch_prefix_tc(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream) {
+  if (head_dim == 64) {
+    return dtype == SM120N_F16 ? run_prefix<__half, 64>(a, stream)
+                               : run_prefix<__nv_bfloat16, 64>(a, stream);
+  }
+  return dtype == SM120N_F16 ? run_prefix<__half, 128>(a, stream)
+                             : run_prefix<__nv_bfloat16, 128>(a, stream);
+}
+
+}  // namespace sm120n
+
+using namespace sm120n;
+
+extern "C" int sm120s_get_device_faults(uint32_t* out_count) {
+  clear_error();
+  if (!out_count) return fail(SM120N_ERR_INVALID_ARGUMENT, "out_count must be non-null");
+  const cudaError_t err = cudaMemcpyFromSymbol(out_count, g_attention_expired_waits, sizeof *out_count);
+  return err == cudaSuccess ? SM120N_OK
+                            : fail(SM120N_ERR_CUDA, "reading the fault counter failed: %s",
+                                   cudaGetErrorString(err));
+}
+
+extern "C" int sm120s_reset_device_faults(void) {
+  clear_error();
+  const unsigned int zero = 0;
+  const cudaError_t err = cudaMemcpyToSymbol(g_attention_expired_waits, &zero, sizeof zero);
+  return err == cudaSuccess ? SM120N_OK
+                            : fail(SM120N_ERR_CUDA, "resetting the fault counter failed: %s",
+                                   cudaGetErrorString(err));
+}

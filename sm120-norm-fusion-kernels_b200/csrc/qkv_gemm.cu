@@ -41,8 +41,6 @@
 // its work (waiting, again bounded, for its own asynchronous operations) and
 // releases its tensor memory.
 #include <cooperative_groups.h>
-#include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <map>
@@ -50,6 +48,8 @@
 
 #include "head_utils.cuh"
 #include "runtime.h"
+#include "tensor_core.cuh"
+#include "tensor_map.h"
 
 namespace sm120n {
 
@@ -101,79 +101,6 @@ struct GemmArgs {
   float epsilon;
   int epilogue;  // 0: store the bf16 GEMM output only; 1: norm + RoPE + cache
 };
-
-// ---- PTX wrappers ----------------------------------------------------------
-__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y,
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(shared_address(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(shared_address(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   shared_address(slot)),
-               "r"(columns)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(columns)
-               : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
-                                         uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   shared_address(bar))
-               : "memory");
-}
-
-// 32 consecutive fp32 accumulator columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
-        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major, 128-byte-swizzled tile whose
-// rows are 128 bytes and whose 8-row groups are 1024 bytes apart (the layout
-// the TMA engine writes for a 64-element bf16 box with SWIZZLE_128B): start
-// address >> 4 in bits [0, 14), leading offset 1 (unused for this layout) in
-// [16, 30), stride offset 1024 >> 4 in [32, 46), descriptor version 1 at
-// bit 46, layout 2 (128-byte swizzle) in [61, 64).
-__device__ __forceinline__ uint64_t smem_descriptor(const void* tile) {
-  const uint64_t address = shared_address(tile);
-  return ((address & 0x3FFFFull) >> 4) | (uint64_t{1} << 16) | (uint64_t{1024 >> 4} << 32) |
-         (uint64_t{1} << 46) | (uint64_t{2} << 61);
-}
 
 __device__ __forceinline__ bool wait_or_record(uint64_t* bar, uint32_t parity) {
   if (mbarrier_wait_bounded(bar, parity)) return true;
@@ -1224,23 +1151,6 @@ __global__ void __launch_bounds__(kGemvThreads, 3) qkv_gemv_kernel(const __nv_bf
 }
 
 // ---- host ----------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder(int* rc) {
-  static std::once_flag once;
-  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-  static cudaError_t status = cudaSuccess;
-  std::call_once(once, [] {
-    cudaDriverEntryPointQueryResult query;
-    status = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", reinterpret_cast<void**>(&encode),
-                                     cudaEnableDefault, &query);
-    if (status == cudaSuccess && query != cudaDriverEntryPointSuccess) status = cudaErrorNotSupported;
-  });
-  *rc = status == cudaSuccess && encode != nullptr
-            ? SM120N_OK
-            : fail(SM120N_ERR_CUDA, "cuTensorMapEncodeTiled is not available: %s",
-                   cudaGetErrorString(status));
-  return encode;
-}
-
 // Row-major [rows, cols] bf16 matrix as a TMA map with a 64 x box_rows box,
 // 128-byte swizzle; rows past the end read as zeros.
 int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows) {

@@ -67,6 +67,8 @@ class DecodeArgs(_Sized):
 SIGNATURES: dict[str, tuple[list, object]] = {
     "sm120s_abi_version": ([], ctypes.c_int),
     "sm120s_last_error": ([], ctypes.c_char_p),
+    "sm120s_get_device_faults": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
+    "sm120s_reset_device_faults": ([], ctypes.c_int),
     "sm120s_plan_step": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                           _i64, _i64, _i64, _i64, _i64, _vp], ctypes.c_int),
     "sm120s_release_blocks": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp],
@@ -105,6 +107,16 @@ def _check(status: int) -> None:
 
 def abi_version() -> int:
     return load().sm120s_abi_version()
+
+
+def device_faults() -> int:
+    count = ctypes.c_uint32(0)
+    _check(load().sm120s_get_device_faults(ctypes.byref(count)))
+    return int(count.value)
+
+
+def reset_device_faults() -> None:
+    _check(load().sm120s_reset_device_faults())
 
 
 def plan_step(context_lens_ptr, query_lens_ptr, block_table_ptr, table_stride, free_blocks_ptr,
