@@ -210,7 +210,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
                                        const CUtensorMap* value_map, Control& c, unsigned char* smem) {
   using S = TcShape<D>;
   constexpr int kStages = S::kStages;
-  const int warp = threadIdx.x / kWarpSize;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / kWarpSize, 0);  // known to be uniform
   const int lane = threadIdx.x & (kWarpSize - 1);
   unsigned char* stages = smem + 2 * S::kQBytes;
 
@@ -412,9 +412,11 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
     }
   } else {
     shrink_registers<kOtherRegisters>();
-    if (warp == kMmaWarp && lane == 0) {
+    if (warp == kMmaWarp) {
+      // The whole warp keeps step; the instructions are one lane's.
       constexpr uint32_t kScore = instruction<T>(kTileKeys, false);
       constexpr uint32_t kValue = instruction<T>(D, true);
+      const uint32_t tmem = c.tmem;
       auto full = [&](int t) { return wait_in(c, &c.bar.full[t % kStages], (t / kStages) & 1); };
       auto score = [&](int i, int j) {
         const uint64_t q = smem_descriptor(smem + i * S::kQBytes);
@@ -423,7 +425,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         for (int kk = 0; kk < D / 16; ++kk) {
           // 16 elements along d: 32 bytes inside a box, then the next box
           const uint32_t step = (kk / 4) * (kBoxBytes >> 4) + 2 * (kk % 4);
-          mma_bf16(c.tmem + i * kTileKeys, q + step, k + step, kScore, kk != 0);
+          mma_bf16(tmem + i * kTileKeys, q + step, k + step, kScore, kk != 0);
         }
         mma_commit(&c.bar.s_full[i]);
       };
@@ -431,53 +433,51 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         const uint64_t v = value_descriptor(stages + ((2 * j + 1) % kStages) * S::kTileBytes);
 #pragma unroll
         for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-          mma_from_tmem(c.tmem + S::kOutColumn + i * D, c.tmem + i * kTileKeys + 8 * kk,
+          mma_from_tmem(tmem + S::kOutColumn + i * D, tmem + i * kTileKeys + 8 * kk,
                         v + kk * (2048 >> 4), kValue, (j | kk) != 0);
         }
         if (j == n[i] - 1) mma_commit(&c.bar.o_full[i]);
       };
-      bool ok = wait_in(c, &c.bar.q_full, 0) && (tiles == 0 || full(0));
-      if (ok && tiles > 0) {
+      bool ok = wait_in(c, &c.bar.q_full, 0) && full(0);
+      if (ok) {
         tc_fence_after();
-        for (int i = 0; i < 2; ++i) {
-          if (n[i] > 0) score(i, 0);
+        if (elect_lane()) {
+          score(0, 0);
+          if (n[1] > 0) score(1, 0);
+          mma_commit(&c.bar.empty[0]);
         }
-        mma_commit(&c.bar.empty[0]);
       }
       for (int j = 0; ok && j < tiles; ++j) {
         const bool more = j + 1 < tiles;
         ok = full(2 * j + 1) && (!more || full(2 * j + 2));
-        if (!ok) break;
+#pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (j >= n[i]) continue;
-          if (!wait_in(c, &c.bar.p_ready[i], j & 1)) {
-            ok = false;
-            break;
-          }
+          if (!ok || j >= n[i]) continue;
+          ok = wait_in(c, &c.bar.p_ready[i], j & 1);
+          if (!ok) continue;
           tc_fence_after();
-          weigh(i, j);
-          if (j + 1 < n[i]) score(i, j + 1);
+          if (elect_lane()) {
+            weigh(i, j);
+            if (j + 1 < n[i]) score(i, j + 1);
+          }
         }
-        if (!ok) break;
-        mma_commit(&c.bar.empty[(2 * j + 1) % kStages]);
-        if (more) mma_commit(&c.bar.empty[(2 * j + 2) % kStages]);
+        if (ok && elect_lane()) {
+          mma_commit(&c.bar.empty[(2 * j + 1) % kStages]);
+          if (more) mma_commit(&c.bar.empty[(2 * j + 2) % kStages]);
+        }
       }
-      mma_commit(&c.bar.done);
+      if (elect_lane()) mma_commit(&c.bar.done);
     } else if (warp == kLoadWarp) {
       for (int t = 0; t < 2 * tiles; ++t) {
         const int stage = t % kStages;
-        bool ok = true;
-        if (lane == 0) {
-          ok = !*reinterpret_cast<volatile int*>(&c.aborted);
-          if (ok && t >= kStages) ok = wait_in(c, &c.bar.empty[stage], (t / kStages - 1) & 1);
-          if (ok) mbarrier_arrive_expect_tx(&c.bar.full[stage], S::kTileBytes);
-        }
-        if (!__shfl_sync(kFullMask, ok, 0)) break;
+        if (*reinterpret_cast<volatile int*>(&c.aborted)) break;
+        if (t >= kStages && !wait_in(c, &c.bar.empty[stage], (t / kStages - 1) & 1)) break;
         unsigned char* to = stages + stage * S::kTileBytes;
         const CUtensorMap* map = t & 1 ? value_map : key_map;
         const int key0 = (t / 2) * kTileKeys;
         if constexpr (kPass == kPrompt) {
-          if (lane == 0) {
+          if (elect_lane()) {
+            mbarrier_arrive_expect_tx(&c.bar.full[stage], S::kTileBytes);
 #pragma unroll
             for (int h = 0; h < D / 64; ++h) {
               tma_load_2d(to + h * kBoxBytes, map, w.kv_head * D + 64 * h,
@@ -488,6 +488,8 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
           // one box to a block of the cache (or 128 slots of a larger one); a
           // lane to a box. Blocks that do not exist, and what is behind the
           // end, lie outside the map and arrive as zeros.
+          if (elect_lane()) mbarrier_arrive_expect_tx(&c.bar.full[stage], S::kTileBytes);
+          __syncwarp();
           const int box = min(a.kv.block_size, kTileKeys);
           for (int b = lane; b < kTileKeys / box; b += kWarpSize) {
             const int64_t key = int64_t{w.key_first} + key0 + b * box;

@@ -30,6 +30,21 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t columns) {
                : "memory");
 }
 
+// True in one lane of a converged warp. Tensor-core and TMA instructions of one
+// lane are issued under this predicate and not under a comparison of the lane:
+// their operands live in uniform registers, and only where the compiler knows
+// that one lane is active does it keep them there. 64 products of 128 x 128 x
+// 16 in a row: 67 cycles each under elect.sync, 159-252 under `lane == 0`.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t elected;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(elected));
+  return elected != 0;
+}
+
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
