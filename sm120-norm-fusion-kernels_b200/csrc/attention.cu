@@ -46,8 +46,8 @@ int check_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int
 // Whether the prefix runs on tensor memory: 256 rows and 128 keys to a tile
 // there, 64 and 64 otherwise.
 bool prefix_on_tensor_memory(const sm120s_decode_args& a) {
-  return a.head_dim <= 128 && a.cache_dtype == SM120N_CACHE_AUTO &&
-         block_fills_tiles(a.block_size) && a.num_blocks > 0;
+  return a.head_dim <= 128 && a.num_blocks > 0 &&
+         (a.cache_dtype == SM120N_CACHE_FP8_E4M3 || block_fills_tiles(a.block_size));
 }
 
 struct Plan {
@@ -269,7 +269,7 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
   const int head_dim = static_cast<int>(in.head_dim);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.prefix_splits > 0) {
-    rc = prefix_on_tensor_memory(in) ? launch_prefix_tc(a, in.dtype, head_dim, s)
+    rc = prefix_on_tensor_memory(in) ? launch_prefix_tc(a, in.dtype, in.cache_dtype, head_dim, s)
                                      : launch_prefix_mma(a, in.dtype, in.cache_dtype, head_dim, s);
     if (rc != SM120N_OK) return rc;
   }

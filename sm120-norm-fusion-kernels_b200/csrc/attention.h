@@ -77,10 +77,11 @@ int own_blocks_per_sm(int row_bytes);
 int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
 int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
                       cudaStream_t stream);
-// Head sizes 64 and 128, caches in dtype; the prefix form wants blocks that fill
-// a tile of 128 keys evenly, in whole groups of 8 (block_fills_tiles).
+// Head sizes 64 and 128. The prefix form on a cache in dtype (loaded by TMA)
+// wants blocks that fill a tile of 128 keys evenly, in whole groups of 8.
 int launch_prompt_tc(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
-int launch_prefix_tc(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream);
+int launch_prefix_tc(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
+                     cudaStream_t stream);
 inline bool block_fills_tiles(int64_t block_size) {
   return block_size % 128 == 0 || (block_size % 8 == 0 && 128 % block_size == 0);
 }

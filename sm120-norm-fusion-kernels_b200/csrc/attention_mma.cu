@@ -513,8 +513,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_mma_kernel(PromptArgs a) {
   SM120S_WORKER(F);
   wait_for_upstream_grid();
   release_downstream_grid();
-  const SequenceTile tile = find_tile<kThreads>(a.query_start, a.sequences, a.tokens, a.group,
-                                                F::kRows, blockIdx.x / a.key_heads);
+  const SequenceTile tile = find_tile<F::kRows>(a.query_start, a.sequences, a.tokens, a.group,
+                                                blockIdx.x / a.key_heads);
   if (tile.tile < 0) return;
   Worker<T, T, false, D, kPrompt, PromptArgs> w{a, dynamic_smem, live, offsets, row_factor};
   w.warp = threadIdx.x / kWarpSize;
@@ -528,7 +528,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_mma_kernel(PromptArgs a) {
   T* out = static_cast<T*>(a.out);
   if (w.run(p, a.scale_log2)) {
     for (int row = w.warp; row < p.rows; row += kWarps) {
-      plain_prompt_row<T, D>(a, p.token0, p.first_row + row, p.kv_head);
+      const int64_t token = (p.first_row + row) / a.group;
+      const int64_t head = int64_t{p.kv_head} * a.group + (p.first_row + row - token * a.group);
+      plain_prompt_row<T, D>(a, p.token0, token, head, p.kv_head);
     }
     return;
   }

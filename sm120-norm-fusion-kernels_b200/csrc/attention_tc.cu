@@ -8,18 +8,29 @@
 //   S_i = Q_i K^T      tcgen05.mma, both operands in shared memory -> TMEM
 //   P_i = 2^(scale S_i - m_i)   one thread per row; TMEM -> registers -> TMEM
 //   O_i += P_i V       tcgen05.mma, P from TMEM, V in shared memory -> TMEM
-// S_i and P_i share 128 columns of tensor memory, O_i has D of its own: at
-// D = 128 all 512 columns. While the 128 threads of one tile exponentiate,
-// the tensor cores work on the other tile. Both products of a tile pair take
-// 2048 cycles at D = 128, and so do the pair's 32768 exponentials on the
-// special-function units (16 a cycle): neither may wait for the other.
+// S_i takes 128 columns of tensor memory and O_i takes D. At D = 128 that is all
+// 512, so P_i lies in the first half of S_i and S_i of the next key tile follows
+// the product with P_i; while the 128 threads of one tile exponentiate, the
+// tensor cores work on the other tile. At D = 64 P_i has columns of its own, and
+// the next S_i is formed as soon as this one has been read. Both products of a
+// tile pair take 2048 cycles at D = 128, and so do the pair's 32768
+// exponentials on the special-function units (16 a cycle).
 //
 // Warps 0-3 and 4-7: softmax and epilogue of tile 0 and 1, a thread to a row, so
-// that no reduction crosses threads. Warp 8: issues every matrix instruction.
-// Warp 9: loads K and V tiles by TMA into kStages shared-memory stages. Warps
-// 10-11 (prompts): look for infinite or NaN values in the V tiles that some
-// rows must not see, where a product would multiply them by zero; a block
-// that meets one does its rows by plain arithmetic instead.
+// that no reduction crosses threads (two threads to a row, sharing the maximum
+// through shared memory, measured slower: 1898 us against 1782 for 16384
+// tokens). Warp 8: issues every matrix instruction. Warp 9: loads K and V tiles
+// by TMA into kStages shared-memory stages. Warps 10-11 (prompts): look for
+// infinite or NaN values in the V tiles that some rows must not see, where a
+// product would multiply them by zero; a block that meets one does its rows by
+// plain arithmetic instead. Q and O go through shared memory so that global
+// accesses are whole rows: a thread reading or writing its own row touches 32
+// lines in every instruction of its warp (4000 cycles for a block's rows).
+//
+// Prefixes in fp8 caches run as fp16: warps 9-11 load and convert the tiles
+// (exact), each row of q is scaled by a power of two into [1, 2) first (exact
+// but for elements 2^14 below the row's largest) and the power goes into the
+// row's score scale.
 //
 // The running maximum of a row follows the true one only when that has grown
 // by more than 2^8 (kSlack): p then stays below 256, exact enough in 16 bits
@@ -29,6 +40,8 @@
 //
 // Every wait on an mbarrier is bounded; one that runs out is counted
 // (sm120s_get_device_faults) and ends the block without results.
+#include <cuda_fp8.h>
+
 #include <algorithm>
 
 #include "attention.h"
@@ -61,6 +74,9 @@ struct TcShape {
   static constexpr uint32_t kQBytes = kTileRows * D * 2;
   static constexpr size_t kSmem = 2 * kQBytes + kStages * kTileBytes + 1024;
   static constexpr uint32_t kOutColumn = 256;  // of tile 0; tile 1 is D further
+  static constexpr bool kOwnP = D == 64;       // P beside S, 64 columns for each tile
+  static constexpr uint32_t kPColumn = kOwnP ? 256 + 2 * D : 0;
+  static constexpr uint32_t kPStep = kOwnP ? kTileKeys / 2 : kTileKeys;
   static constexpr uint32_t kTmemColumns = 512;
 };
 
@@ -157,18 +173,24 @@ __device__ __forceinline__ void shrink_registers() {
 constexpr int kSoftmaxRegisters = 208;
 constexpr int kOtherRegisters = 88;
 
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
-
-// What a block works on.
+// What a block works on. Row r is head (first_head + r) % group of the group and
+// token (or request) first_token + (first_head + r) / group.
 struct Work {
-  int64_t first_row;  // of the sequence, or of the batch
-  int64_t rows;       // up to 256
-  int64_t token0;     // kPrompt: the sequence's first token
-  int key_first;      // kPrefix: first key of its part of the prefix
+  int64_t first_token;  // within the sequence
+  int64_t token0;       // kPrompt: the sequence's first token
+  int first_head;
+  int rows;       // up to 256
+  int key_first;  // kPrefix: first key of its part of the prefix
   int key_last;
   int kv_head;
   int split;  // kPrefix
 };
+
+__device__ __forceinline__ void place_rows(Work& w, int64_t first_row, int64_t all_rows, int group) {
+  w.first_token = first_row / group;
+  w.first_head = static_cast<int>(first_row - w.first_token * group);
+  w.rows = static_cast<int>(min(int64_t{2 * kTileRows}, all_rows - first_row));
+}
 
 struct Barriers {
   uint64_t full[8];
@@ -177,6 +199,8 @@ struct Barriers {
   uint64_t s_full[2];
   uint64_t p_ready[2];
   uint64_t o_full[2];
+  uint64_t s_free[2];   // kOwnP: S has been read
+  uint64_t p_free[2];   // kOwnP: the product with P is complete
   uint64_t guarded;
   uint64_t done;
 };
@@ -196,16 +220,92 @@ __device__ __forceinline__ bool wait_in(Control& c, uint64_t* bar, uint32_t pari
   return false;
 }
 
-// Offset of a row of q or out, in elements.
-template <int kPass, int D, typename Args>
-__device__ __forceinline__ int64_t row_at(const Args& a, const Work& w, int64_t row, int64_t stride) {
-  const int64_t r = w.first_row + row;
-  const int64_t token = r / a.group;
-  const int64_t head = static_cast<int64_t>(w.kv_head) * a.group + (r - token * a.group);
-  return (w.token0 + token) * stride + head * D;
+// Token (or request) and head of a row, the head among all query heads.
+struct RowPlace {
+  int64_t token;  // within the sequence
+  int64_t head;
+};
+template <typename Args>
+__device__ __forceinline__ RowPlace row_place(const Args& a, const Work& w, int row) {
+  const uint32_t r = static_cast<uint32_t>(w.first_head + row);
+  const uint32_t step = r / static_cast<uint32_t>(a.group);
+  return RowPlace{w.first_token + step,
+                  static_cast<int64_t>(w.kv_head) * a.group + (r - step * a.group)};
 }
 
-template <typename T, int D, int kPass, typename Args>
+// Two e4m3 bytes as two fp16 values.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(b), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+// fp8: K and V tiles into the swizzled fp16 stages, by the three warps that TMA
+// leaves free. A thread has 16 bytes of a row at a time (32 bytes in the
+// stage), kDepth of them in flight.
+template <int D, typename Args>
+__device__ __forceinline__ void convert_tiles(const Args& a, const Work& w, Control& c,
+                                              unsigned char* stages, int tiles, int thread) {
+  using S = TcShape<D>;
+  constexpr int kConverters = 3 * kWarpSize;
+  constexpr int kRowChunks = D / 16;
+  constexpr int kAll = kTileKeys * kRowChunks;
+  constexpr int kDepth = 6;
+  const int64_t head = w.kv_head * a.kv.head_stride;
+  for (int t = 0; t < 2 * tiles; ++t) {
+    const int stage = t % S::kStages;
+    const uint8_t* source = static_cast<const uint8_t*>(t & 1 ? a.kv.value : a.kv.key) + head;
+    unsigned char* to = stages + stage * S::kTileBytes;
+    const int key0 = w.key_first + (t / 2) * kTileKeys;
+    bool free_stage = t < S::kStages;
+    for (int first = thread; first < kAll; first += kDepth * kConverters) {
+      uint4 v[kDepth];
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        const int at = first + d * kConverters;
+        const int key = key0 + at / kRowChunks;
+        v[d] = make_uint4(0, 0, 0, 0);
+        if (at < kAll && key < w.key_last) {
+          const uint32_t block = static_cast<uint32_t>(key) / static_cast<uint32_t>(a.kv.block_size);
+          const int id = a.prefix_blocks[block];
+          if (static_cast<uint32_t>(id) < static_cast<uint32_t>(a.kv.num_blocks)) {
+            v[d] = load16(source + id * a.kv.block_stride +
+                          static_cast<int64_t>(key - block * a.kv.block_size) * a.kv.slot_stride +
+                          (at % kRowChunks) * 16);
+          }
+        }
+      }
+      if (!free_stage) {
+        if (!wait_in(c, &c.bar.empty[stage], (t / S::kStages - 1) & 1)) return;
+        free_stage = true;
+      }
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        const int at = first + d * kConverters;
+        if (at >= kAll) break;
+        const int row = at / kRowChunks;
+        const int chunk = 2 * (at % kRowChunks);  // of 16 bytes in the stage
+        const uint32_t words[4] = {v[d].x, v[d].y, v[d].z, v[d].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          h[2 * e] = e4m3_pair(words[e] & 0xffffu);
+          h[2 * e + 1] = e4m3_pair(words[e] >> 16);
+        }
+        unsigned char* box = to + (chunk / 8) * kBoxBytes + row * 128;
+        *reinterpret_cast<uint4*>(box + ((chunk % 8) ^ (row & 7)) * 16) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(box + (((chunk + 1) % 8) ^ (row & 7)) * 16) =
+            make_uint4(h[4], h[5], h[6], h[7]);
+      }
+    }
+    fence_async_shared();
+    __syncwarp();
+    if ((threadIdx.x & (kWarpSize - 1)) == 0) mbarrier_arrive(&c.bar.full[stage]);
+  }
+}
+
+// TQ: type of q and out; T: operand type of the products.
+template <typename TQ, typename T, bool kFp8, int D, int kPass, typename Args>
 __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUtensorMap* key_map,
                                        const CUtensorMap* value_map, Control& c, unsigned char* smem) {
   using S = TcShape<D>;
@@ -218,11 +318,11 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
   int n[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int64_t rows = min(w.rows - i * kTileRows, int64_t{kTileRows});
+    const int rows = min(w.rows - i * kTileRows, kTileRows);
     if (rows <= 0) {
       n[i] = 0;
     } else if constexpr (kPass == kPrompt) {
-      n[i] = static_cast<int>((w.first_row + i * kTileRows + rows - 1) / a.group / kTileKeys + 1);
+      n[i] = static_cast<int>(row_place(a, w, i * kTileRows + rows - 1).token / kTileKeys + 1);
     } else {
       n[i] = (w.key_last - w.key_first + kTileKeys - 1) / kTileKeys;
     }
@@ -232,38 +332,73 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
   if (warp < kSoftmaxWarps) {
     grow_registers<kSoftmaxRegisters>();
     const int i = warp / 4;
-    const int row = i * kTileRows + (warp % 4) * kWarpSize + lane;
-    const T* query = static_cast<const T*>(a.query);
-    // Q of the warp's 32 rows into the swizzled operand layout
+    const int warp_row = (warp % 4) * kWarpSize;  // of the tile
+    const int row = i * kTileRows + warp_row + lane;
+    const RowPlace place = row_place(a, w, row);
+    const int live_rows = min(max(w.rows - (row - lane), 0), kWarpSize);  // of the warp
+    unsigned char* rows_smem = smem + i * S::kQBytes + warp_row * 128;  // of the warp, in each box
+    float scale = a.scale_log2;
+    // Q of the warp's rows into the swizzled operand layout, whole rows at a time
     {
       constexpr int kChunks = D / 8;
-#pragma unroll 8
-      for (int t = lane; t < kWarpSize * kChunks; t += kWarpSize) {
-        const int r = (warp % 4) * kWarpSize + t / kChunks;
-        const int chunk = t % kChunks;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (i * kTileRows + r < w.rows) {
-          v = load16(query + row_at<kPass, D>(a, w, i * kTileRows + r, a.query_stride) + chunk * 8);
+      constexpr int kRowsAtOnce = kWarpSize / kChunks;
+      constexpr int kBatch = 8;
+      const TQ* query = static_cast<const TQ*>(a.query) + (lane % kChunks) * 8;
+      const int64_t offset = (w.token0 + place.token) * a.query_stride + place.head * D;
+#pragma unroll 1
+      for (int r0 = 0; r0 < kWarpSize; r0 += kBatch * kRowsAtOnce) {
+        uint4 v[kBatch];
+#pragma unroll
+        for (int t = 0; t < kBatch; ++t) {
+          const int r = r0 + t * kRowsAtOnce + lane / kChunks;
+          const int64_t at = __shfl_sync(kFullMask, offset, r);
+          v[t] = r < live_rows ? load16(query + at) : make_uint4(0, 0, 0, 0);
         }
-        *reinterpret_cast<uint4*>(smem + i * S::kQBytes + (chunk / 8) * kBoxBytes + r * 128 +
-                                  ((chunk % 8) ^ (r & 7)) * 16) = v;
+#pragma unroll
+        for (int t = 0; t < kBatch; ++t) {
+          const int r = r0 + t * kRowsAtOnce + lane / kChunks;
+          if constexpr (kFp8) {
+            float f[8];
+            Pack<TQ>::to_f32(v[t], f);
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]));
+#pragma unroll
+            for (int d = 1; d < kChunks; d *= 2) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, d));
+            // 2^-e and 2^e with e the exponent of the row's largest, kept normal
+            const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 2), 252);
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] *= down;
+            v[t] = Pack<T>::from_f32(f);
+            const float up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+            for (int k = 0; k < kRowsAtOnce; ++k) {
+              const float mine = __shfl_sync(kFullMask, up, k * kChunks);
+              if (lane == r0 + t * kRowsAtOnce + k) scale *= mine;
+            }
+          }
+          const int chunk = lane % kChunks;
+          *reinterpret_cast<uint4*>(rows_smem + (chunk / 8) * kBoxBytes + r * 128 +
+                                    ((chunk % 8) ^ (r & 7)) * 16) = v[t];
+        }
       }
+      if constexpr (kFp8) scale *= *a.k_scale;
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&c.bar.q_full);
     }
-    const uint32_t lane_base = c.tmem + (static_cast<uint32_t>((warp % 4) * kWarpSize) << 16);
+    const uint32_t lane_base = c.tmem + (static_cast<uint32_t>(warp_row) << 16);
     const uint32_t s_at = lane_base + i * kTileKeys;
+    const uint32_t p_at = lane_base + S::kPColumn + i * S::kPStep;
     const uint32_t o_at = lane_base + S::kOutColumn + i * D;
-    const float scale = a.scale_log2;
-    float top = -INFINITY;   // true maximum of the raw scores
-    float base = 0.0f;       // scale * the maximum in use
+    float top = -INFINITY;  // raw maximum that `base` follows
+    float base = 0.0f;      // scale * the maximum in use
     float sum = 0.0f;
     // last key of the row, counted from the first key tile's first
-    const int64_t limit = kPass == kPrompt ? (w.first_row + row) / a.group
-                                           : int64_t{w.key_last} - w.key_first - 1;
+    const int64_t limit = kPass == kPrompt ? place.token : int64_t{w.key_last} - w.key_first - 1;
     const int64_t first_limit =  // smallest of the tile: tiles behind it need no mask
-        kPass == kPrompt ? (w.first_row + i * kTileRows) / a.group : limit;
+        kPass == kPrompt ? row_place(a, w, i * kTileRows).token : limit;
     bool ok = true;
     for (int j = 0; j < n[i]; ++j) {
       if (!wait_in(c, &c.bar.s_full[i], j & 1)) {
@@ -275,10 +410,15 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
 #pragma unroll
       for (int q = 0; q < kTileKeys / 32; ++q) tmem_load32_async(s_at + 32 * q, raw + 32 * q);
       tmem_wait_load<kTileKeys>(raw);
+      if constexpr (S::kOwnP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&c.bar.s_free[i]);
+      }
       float* s = reinterpret_cast<float*>(raw);
       const int64_t key0 = int64_t{j} * kTileKeys;
       if (key0 + kTileKeys - 1 > first_limit) {
-        const int last = static_cast<int>(min(limit - key0, int64_t{kTileKeys}));
+        const int last = static_cast<int>(max(min(limit - key0, int64_t{kTileKeys}), int64_t{-1}));
 #pragma unroll
         for (int k = 0; k < kTileKeys; ++k) {
           if (k > last) s[k] = -INFINITY;
@@ -296,15 +436,21 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       }
       float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-      for (int k = 4; k < kTileKeys; k += 8) {
-        m0 = max3(m0, s[k], s[k + 1]);
-        m1 = max3(m1, s[k + 2], s[k + 3]);
-        if (k + 4 < kTileKeys) {
-          m2 = max3(m2, s[k + 4], s[k + 5]);
-          m3 = max3(m3, s[k + 6], s[k + 7]);
-        }
+      for (int k = 4; k < kTileKeys; k += 4) {
+        m0 = fmaxf(m0, s[k]);
+        m1 = fmaxf(m1, s[k + 1]);
+        m2 = fmaxf(m2, s[k + 2]);
+        m3 = fmaxf(m3, s[k + 3]);
       }
-      const float next = fmaxf(max3(m0, m1, m2), fmaxf(m3, top));
+      const float next = fmaxf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), top);
+      if constexpr (S::kOwnP) {
+        // P and O are free for this tile once the last product is complete
+        if (j > 0 && !wait_in(c, &c.bar.p_free[i], (j - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
       const bool lags = (next - top) * scale > kSlack;  // also where top is still -inf
       if (__any_sync(kFullMask, lags)) {
         const float moved = lags ? next * scale : base;
@@ -342,7 +488,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
           p[k] = Pack<T>::f32_to_word(x.x, x.y);
           p[k + 1] = Pack<T>::f32_to_word(y.x, y.y);
         }
-        tmem_store32(s_at + 32 * q, p);
+        tmem_store32(p_at + 32 * q, p);
       }
       sum_a = __fadd2_rn(sum_a, sum_b);
       sum += sum_a.x + sum_a.y;
@@ -356,57 +502,75 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       if (ok) ok = wait_in(c, &c.bar.guarded, 0);
     }
     ok = ok && !*reinterpret_cast<volatile int*>(&c.aborted);
+    ok = __all_sync(kFullMask, ok);
     tc_fence_after();
-    if (ok && n[i] > 0) {
-      if constexpr (kPass == kPrompt) {
-        if (*reinterpret_cast<volatile int*>(&c.unsafe)) {
-          for (int r = 0; r < kWarpSize; ++r) {
-            const int at = row - lane + r;
-            if (at < w.rows) plain_prompt_row<T, D>(a, w.token0, w.first_row + at, w.kv_head);
-          }
-        } else {
-          const float inv = 1.0f / sum;
-          T* out = static_cast<T*>(a.out) + (row < w.rows ? row_at<kPass, D>(a, w, row, a.out_stride) : 0);
-#pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t o[32];
-            tmem_load32_async(o_at + 32 * q, o);
-            tmem_wait_load<32>(o);
-            if (row < w.rows) {
-              uint32_t words[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                words[k] = Pack<T>::f32_to_word(__uint_as_float(o[2 * k]) * inv,
-                                                __uint_as_float(o[2 * k + 1]) * inv);
-              }
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                store16(out + 32 * q + 8 * k, make_uint4(words[4 * k], words[4 * k + 1],
-                                                         words[4 * k + 2], words[4 * k + 3]));
-              }
-            }
+    if (ok && live_rows > 0) {
+      if (kPass == kPrompt && *reinterpret_cast<volatile int*>(&c.unsafe)) {
+        if constexpr (kPass == kPrompt) {
+          for (int r = 0; r < live_rows; ++r) {
+            const RowPlace to = row_place(a, w, row - lane + r);
+            plain_prompt_row<T, D>(a, w.token0, to.token, to.head, w.kv_head);
           }
         }
       } else {
-        const int64_t r = w.first_row + row;
-        const int64_t request = r / a.group;
-        const int64_t at = (static_cast<int64_t>(w.split) * a.batch + request) * a.query_heads +
-                           static_cast<int64_t>(w.kv_head) * a.group + (r - request * a.group);
-        if (row < w.rows) {
-          a.prefix_state[at] = make_float2(top == -INFINITY ? -INFINITY : base, sum);
+        // O through the warp's rows of the Q tile (its products are complete),
+        // kColumns at a time: 64 of fp32 partials, 128 bytes a row and box
+        constexpr int kElem = kPass == kPrompt ? 2 : 4;
+        constexpr int kColumns = kPass == kPrompt ? D : D / 2;
+        constexpr int kChunks = kColumns * kElem / 16;
+        constexpr int kRowsAtOnce = kWarpSize / kChunks;
+        const float inv = kPass == kPrompt ? 1.0f / sum : 1.0f;
+        unsigned char* out;
+        int64_t offset;  // bytes, of this lane's row
+        if constexpr (kPass == kPrompt) {
+          out = static_cast<unsigned char*>(a.out);
+          offset = ((w.token0 + place.token) * a.out_stride + place.head * D) * kElem;
+        } else {
+          const int64_t at = (static_cast<int64_t>(w.split) * a.batch + place.token) * a.query_heads +
+                             place.head;
+          if (lane < live_rows) {
+            a.prefix_state[at] = make_float2(top == -INFINITY ? -INFINITY : base, sum);
+          }
+          out = reinterpret_cast<unsigned char*>(a.prefix_values);
+          offset = at * D * kElem;
         }
 #pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          tmem_load32_async(o_at + 32 * q, o);
-          tmem_wait_load<32>(o);
-          if (row < w.rows) {
+        for (int c0 = 0; c0 < D; c0 += kColumns) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              *reinterpret_cast<uint4*>(a.prefix_values + at * D + 32 * q + 4 * k) =
-                  make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          for (int q = 0; q < kColumns / 32; ++q) {
+            uint32_t o[32];
+            tmem_load32_async(o_at + c0 + 32 * q, o);
+            tmem_wait_load<32>(o);
+            float* f = reinterpret_cast<float*>(o);
+            constexpr int kPerChunk = 16 / kElem;
+#pragma unroll
+            for (int k = 0; k < 32 / kPerChunk; ++k) {
+              const int chunk = q * (32 / kPerChunk) + k;
+              uint4 v;
+              if constexpr (kPass == kPrompt) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[8 * k + e] *= inv;
+                v = Pack<TQ>::from_f32(f + 8 * k);
+              } else {
+                v = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              }
+              *reinterpret_cast<uint4*>(rows_smem + (chunk / 8) * kBoxBytes + lane * 128 +
+                                        ((chunk % 8) ^ (lane & 7)) * 16) = v;
             }
           }
+          __syncwarp();
+#pragma unroll 4
+          for (int r0 = 0; r0 < kWarpSize; r0 += kRowsAtOnce) {
+            const int r = r0 + lane / kChunks;
+            const int chunk = lane % kChunks;
+            const int64_t at = __shfl_sync(kFullMask, offset, r);
+            if (r < live_rows) {
+              store16(out + at + c0 * kElem + chunk * 16,
+                      load16_shared(rows_smem + (chunk / 8) * kBoxBytes + r * 128 +
+                                    ((chunk % 8) ^ (r & 7)) * 16));
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -433,9 +597,11 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         const uint64_t v = value_descriptor(stages + ((2 * j + 1) % kStages) * S::kTileBytes);
 #pragma unroll
         for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-          mma_from_tmem(tmem + S::kOutColumn + i * D, tmem + i * kTileKeys + 8 * kk,
+          mma_from_tmem(tmem + S::kOutColumn + i * D,
+                        tmem + S::kPColumn + i * S::kPStep + 8 * kk,
                         v + kk * (2048 >> 4), kValue, (j | kk) != 0);
         }
+        if (S::kOwnP && j + 1 < n[i]) mma_commit(&c.bar.p_free[i]);
         if (j == n[i] - 1) mma_commit(&c.bar.o_full[i]);
       };
       bool ok = wait_in(c, &c.bar.q_full, 0) && full(0);
@@ -449,16 +615,34 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       }
       for (int j = 0; ok && j < tiles; ++j) {
         const bool more = j + 1 < tiles;
-        ok = full(2 * j + 1) && (!more || full(2 * j + 2));
+        if constexpr (S::kOwnP) {
+          ok = !more || full(2 * j + 2);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!ok || j >= n[i]) continue;
-          ok = wait_in(c, &c.bar.p_ready[i], j & 1);
-          if (!ok) continue;
-          tc_fence_after();
-          if (elect_lane()) {
-            weigh(i, j);
-            if (j + 1 < n[i]) score(i, j + 1);
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || j + 1 >= n[i]) continue;
+            ok = wait_in(c, &c.bar.s_free[i], j & 1);
+            tc_fence_after();
+            if (ok && elect_lane()) score(i, j + 1);
+          }
+          ok = ok && full(2 * j + 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || j >= n[i]) continue;
+            ok = wait_in(c, &c.bar.p_ready[i], j & 1);
+            tc_fence_after();
+            if (ok && elect_lane()) weigh(i, j);
+          }
+        } else {
+          ok = full(2 * j + 1) && (!more || full(2 * j + 2));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || j >= n[i]) continue;
+            ok = wait_in(c, &c.bar.p_ready[i], j & 1);
+            tc_fence_after();
+            if (ok && elect_lane()) {
+              weigh(i, j);
+              if (j + 1 < n[i]) score(i, j + 1);
+            }
           }
         }
         if (ok && elect_lane()) {
@@ -467,6 +651,10 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         }
       }
       if (elect_lane()) mma_commit(&c.bar.done);
+    } else if (kFp8) {
+      if constexpr (kFp8) {
+        convert_tiles<D>(a, w, c, stages, tiles, (warp - kLoadWarp) * kWarpSize + lane);
+      }
     } else if (warp == kLoadWarp) {
       for (int t = 0; t < 2 * tiles; ++t) {
         const int stage = t % kStages;
@@ -511,7 +699,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
     } else if (kPass == kPrompt && warp > kLoadWarp) {
       // V tiles that reach past the block's first row's last key
       constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-      const int64_t first_limit = w.first_row / a.group;
+      const int64_t first_limit = w.first_token;
       bool bad = false;
       for (int j = 0; j < tiles; ++j) {
         const int stage = (2 * j + 1) % kStages;
@@ -543,16 +731,18 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
 
 // Set-up and release around attend(): barriers, tensor memory.
 template <int D>
-__device__ __forceinline__ void open_block(Control& c, bool guarded) {
+__device__ __forceinline__ void open_block(Control& c, bool guarded, bool converted) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < TcShape<D>::kStages; ++s) {
-      mbarrier_init(&c.bar.full[s], 1);
+      mbarrier_init(&c.bar.full[s], converted ? 3 : 1);
       mbarrier_init(&c.bar.empty[s], 1 + (guarded && (s & 1) ? kGuardWarps : 0));
     }
     mbarrier_init(&c.bar.q_full, kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) {
       mbarrier_init(&c.bar.s_full[i], 1);
       mbarrier_init(&c.bar.p_ready[i], 4);
+      mbarrier_init(&c.bar.s_free[i], 4);
+      mbarrier_init(&c.bar.p_free[i], 1);
       mbarrier_init(&c.bar.o_full[i], 1);
     }
     mbarrier_init(&c.bar.guarded, kGuardWarps);
@@ -602,32 +792,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Control control;
   wait_for_upstream_grid();
   release_downstream_grid();
-  const SequenceTile tile = find_tile<kThreads>(a.query_start, a.sequences, a.tokens, a.group,
-                                                2 * kTileRows, blockIdx.x / a.key_heads);
+  const SequenceTile tile = find_tile<2 * kTileRows>(a.query_start, a.sequences, a.tokens, a.group,
+                                                     blockIdx.x / a.key_heads);
   if (tile.tile < 0) return;
-  open_block<D>(control, true);
+  open_block<D>(control, true, false);
   Work w{};
-  w.first_row = tile.tile * 2 * kTileRows;
-  w.rows = min(int64_t{2 * kTileRows}, tile.length * a.group - w.first_row);
+  place_rows(w, tile.tile * 2 * kTileRows, tile.length * a.group, a.group);
   w.token0 = tile.first_token;
   w.kv_head = static_cast<int>(blockIdx.x % a.key_heads);
-  attend<T, D, kPrompt>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
+  attend<T, T, false, D, kPrompt>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
   close_block<D>(control);
 }
 
-template <typename T, int D>
+template <typename TQ, typename T, bool kFp8, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap key_map,
                      const __grid_constant__ CUtensorMap value_map,
                      const __grid_constant__ DecodeArgs a) {
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ Control control;
-  open_block<D>(control, false);
+  open_block<D>(control, false, kFp8);
   wait_for_upstream_grid();
   release_downstream_grid();
   Work w{};
-  w.first_row = static_cast<int64_t>(blockIdx.x) * 2 * kTileRows;
-  w.rows = min(int64_t{2 * kTileRows}, static_cast<int64_t>(a.batch) * a.group - w.first_row);
+  place_rows(w, static_cast<int64_t>(blockIdx.x) * 2 * kTileRows,
+             static_cast<int64_t>(a.batch) * a.group, a.group);
   w.kv_head = blockIdx.y;
   w.split = blockIdx.z;
   const int64_t tiles = (a.prefix_tokens + kTileKeys - 1) / kTileKeys;
@@ -641,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (__syncthreads_or(holes) && threadIdx.x == 0) control.holes = 1;
   __syncthreads();
-  attend<T, D, kPrefix>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
+  attend<TQ, T, kFp8, D, kPrefix>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
   close_block<D>(control);
 }
 
@@ -690,11 +879,11 @@ int run_prompt(const PromptArgs& a, cudaStream_t stream) {
                 stream, maps[0], maps[1], a);
 }
 
-template <typename T, int D>
+template <typename TQ, typename T, bool kFp8, int D>
 int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
   using S = TcShape<D>;
-  CUtensorMap maps[2];
-  for (int i = 0; i < 2; ++i) {
+  CUtensorMap maps[2] = {};
+  for (int i = 0; !kFp8 && i < 2; ++i) {
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(a.kv.block_size),
                                 static_cast<cuuint64_t>(a.key_heads),
                                 static_cast<cuuint64_t>(a.kv.num_blocks)};
@@ -706,7 +895,7 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
                                  std::min(a.kv.block_size, kTileKeys));
     if (rc != SM120N_OK) return rc;
   }
-  auto kernel = prefix_tc_kernel<T, D>;
+  auto kernel = prefix_tc_kernel<TQ, T, kFp8, D>;
   const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
   if (rc != SM120N_OK) return rc;
   const int64_t tiles = (static_cast<int64_t>(a.batch) * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
@@ -714,6 +903,16 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
                 dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.key_heads),
                      static_cast<unsigned>(a.prefix_splits)),
                 dim3(kThreads), S::kSmem, stream, maps[0], maps[1], a);
+}
+
+template <int D>
+int run_prefix_typed(const DecodeArgs& a, int dtype, bool fp8, cudaStream_t stream) {
+  if (dtype == SM120N_F16) {
+    return fp8 ? run_prefix<__half, __half, true, D>(a, stream)
+               : run_prefix<__half, __half, false, D>(a, stream);
+  }
+  return fp8 ? run_prefix<__nv_bfloat16, __half, true, D>(a, stream)
+             : run_prefix<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream);
 }
 
 }  // namespace
@@ -727,13 +926,11 @@ int launch_prompt_tc(const PromptArgs& a, int dtype, int head_dim, cudaStream_t 
                              : run_prompt<__nv_bfloat16, 128>(a, stream);
 }
 
-int launch_prefix_tc(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream) {
-  if (head_dim == 64) {
-    return dtype == SM120N_F16 ? run_prefix<__half, 64>(a, stream)
-                               : run_prefix<__nv_bfloat16, 64>(a, stream);
-  }
-  return dtype == SM120N_F16 ? run_prefix<__half, 128>(a, stream)
-                             : run_prefix<__nv_bfloat16, 128>(a, stream);
+int launch_prefix_tc(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
+                     cudaStream_t stream) {
+  const bool fp8 = cache_dtype == SM120N_CACHE_FP8_E4M3;
+  return head_dim == 64 ? run_prefix_typed<64>(a, dtype, fp8, stream)
+                        : run_prefix_typed<128>(a, dtype, fp8, stream);
 }
 
 }  // namespace sm120n

@@ -14,15 +14,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 // One row of a prompt by plain arithmetic, one warp, keys one by one: for the
 // rows of a block that has an infinite or NaN value among the keys that some
-// of its rows must not see (a matrix product would multiply it by zero). `row`
-// counts the (token, head of the group) rows of the sequence at `token0`.
+// of its rows must not see (a matrix product would multiply it by zero).
+// `token` counts from the sequence's first, `token0`; `head` from the first of all.
 template <typename T, int D>
-__device__ __noinline__ void plain_prompt_row(const PromptArgs& a, int64_t token0, int64_t row,
-                                              int kv_head) {
+__device__ __noinline__ void plain_prompt_row(const PromptArgs& a, int64_t token0, int64_t token,
+                                              int64_t head, int kv_head) {
   constexpr int kPer = D / kWarpSize;
   const int lane = threadIdx.x & (kWarpSize - 1);
-  const int64_t token = row / a.group;
-  const int64_t head = static_cast<int64_t>(kv_head) * a.group + (row - token * a.group);
   const T* q = static_cast<const T*>(a.query) + (token0 + token) * a.query_stride + head * D;
   float acc[kPer] = {};
   float top = -INFINITY, sum = 0.0f;
@@ -54,61 +52,66 @@ __device__ __noinline__ void plain_prompt_row(const PromptArgs& a, int64_t token
   for (int i = 0; i < kPer; ++i) out[lane + i * kWarpSize] = static_cast<T>(acc[i] / sum);
 }
 
-// The sequence and tile of its rows that block `index` of the tile list works
-// on: tiles of `rows` (token, head) rows, sequence after sequence. Whole block.
+// The sequence and tile of its rows that entry `index` of the tile list stands
+// for: tiles of kRows (token, head) rows, sequence after sequence, the last
+// rows of a sequence (they have the most keys) first. Every warp finds it on
+// its own, 128 sequences at a step: no barrier, and one round of loads where
+// there are few.
 struct SequenceTile {
   int64_t first_token;
   int64_t length;
   int64_t tile;  // -1: the list is shorter
-  int64_t tiles;
 };
 
 __device__ __forceinline__ int64_t clamp_start(int32_t v, int64_t tokens) {
   return min(max(static_cast<int64_t>(v), int64_t{0}), tokens);
 }
 
-template <int kBlockThreads>
+template <int kRows>
 __device__ __forceinline__ SequenceTile find_tile(const int32_t* query_start, int sequences,
-                                                  int64_t tokens, int group, int rows,
-                                                  int64_t index) {
-  __shared__ int64_t totals[kBlockThreads / kWarpSize];
-  __shared__ SequenceTile found;
+                                                  int64_t tokens, int group, int64_t index) {
+  constexpr int kPer = 4;
   const int lane = threadIdx.x & (kWarpSize - 1);
-  const int warp = threadIdx.x / kWarpSize;
-  if (threadIdx.x == 0) found.tile = -1;
   int64_t before = 0;
-  for (int base = 0; base < sequences; base += kBlockThreads) {
-    const int i = base + threadIdx.x;
-    int64_t first = 0, length = 0;
-    if (i < sequences) {
-      first = clamp_start(query_start[i], tokens);
-      length = max(clamp_start(query_start[i + 1], tokens) - first, int64_t{0});
+  for (int base = 0; base < sequences; base += kPer * kWarpSize) {
+    int64_t start[kPer + 1];
+#pragma unroll
+    for (int k = 0; k <= kPer; ++k) {
+      start[k] = clamp_start(query_start[min(base + lane * kPer + k, sequences)], tokens);
     }
-    const int64_t mine = (length * group + rows - 1) / rows;
+    int64_t tiles[kPer], mine = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      tiles[k] = (max(start[k + 1] - start[k], int64_t{0}) * group + kRows - 1) / kRows;
+      mine += tiles[k];
+    }
     int64_t upto = mine;
 #pragma unroll
     for (int d = 1; d < kWarpSize; d *= 2) {
       const int64_t x = __shfl_up_sync(kFullMask, upto, d);
       if (lane >= d) upto += x;
     }
-    __syncthreads();
-    if (lane == kWarpSize - 1) totals[warp] = upto;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < kBlockThreads / kWarpSize; ++w) {
-      if (w < warp) upto += totals[w];
-      all += totals[w];
+    const int64_t first = before + upto - mine;
+    const unsigned holder = __ballot_sync(kFullMask, index >= first && index < first + mine);
+    if (holder) {
+      SequenceTile found{0, 0, 0};
+      int64_t at = first;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        if (index >= at && index < at + tiles[k]) {
+          found = SequenceTile{start[k], start[k + 1] - start[k], at + tiles[k] - 1 - index};
+        }
+        at += tiles[k];
+      }
+      const int source = __ffs(holder) - 1;
+      found.first_token = __shfl_sync(kFullMask, found.first_token, source);
+      found.length = __shfl_sync(kFullMask, found.length, source);
+      found.tile = __shfl_sync(kFullMask, found.tile, source);
+      return found;
     }
-    upto += before;
-    if (index < upto && index >= upto - mine) {
-      // the last rows of a sequence have the most keys: first
-      found = SequenceTile{first, length, upto - 1 - index, mine};
-    }
-    before += all;
-    if (index < before) break;
+    before += __shfl_sync(kFullMask, upto, kWarpSize - 1);
   }
-  __syncthreads();
-  return found;
+  return SequenceTile{0, 0, -1};
 }
 
 }  // namespace sm120n
