@@ -19,15 +19,18 @@
 // Warps 0-3 and 4-7: softmax and epilogue of tile 0 and 1, a thread to a row, so
 // that no reduction crosses threads (two threads to a row, sharing the maximum
 // through shared memory, measured slower: 1898 us against 1782 for 16384
-// tokens). Warp 8: issues every matrix instruction. Warp 9: loads K and V tiles
-// by TMA into kStages shared-memory stages. Warps 10-11 (prompts): look for
-// infinite or NaN values in the V tiles that some rows must not see, where a
-// product would multiply them by zero; a block that meets one does its rows by
-// plain arithmetic instead. Q and O go through shared memory so that global
+// tokens). Warp 8: issues the matrix instructions; at D = 64 only tile 0's, and
+// warp 9 tile 1's, since there the waits for one tile would hold up the other
+// (4096 tokens: 110 us with two issuers, 116 with one; at D = 128, where the
+// tiles take turns, 158 with two and four more warps, 146 with one). The next
+// warp loads K and V tiles by TMA into kStages shared-memory stages. The rest of
+// the 12 warps (prompts) look for infinite or NaN values in the V tiles that
+// some rows must not see, where a product would multiply them by zero; a block
+// that meets one does its rows by plain arithmetic instead. Q and O go through shared memory so that global
 // accesses are whole rows: a thread reading or writing its own row touches 32
 // lines in every instruction of its warp (4000 cycles for a block's rows).
 //
-// Prefixes in fp8 caches run as fp16: warps 9-11 load and convert the tiles
+// Prefixes in fp8 caches run as fp16: all but the issuers load and convert the tiles
 // (exact), each row of q is scaled by a power of two into [1, 2) first (exact
 // but for elements 2^14 below the row's largest) and the power goes into the
 // row's score scale.
@@ -59,8 +62,6 @@ constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 8;
-constexpr int kLoadWarp = 9;
-constexpr int kGuardWarps = 2;  // 10, 11
 constexpr int kThreads = 12 * kWarpSize;
 constexpr uint32_t kBoxBytes = kTileKeys * 128;  // 64 elements of 128 rows
 constexpr float kSlack = 8.0f;                   // log2 of how far a maximum may lag
@@ -78,6 +79,10 @@ struct TcShape {
   static constexpr uint32_t kPColumn = kOwnP ? 256 + 2 * D : 0;
   static constexpr uint32_t kPStep = kOwnP ? kTileKeys / 2 : kTileKeys;
   static constexpr uint32_t kTmemColumns = 512;
+  static constexpr int kIssuers = D == 64 ? 2 : 1;
+  static constexpr int kLoadWarp = kMmaWarp + kIssuers;
+  static constexpr int kConvertWarps = kThreads / kWarpSize - kLoadWarp;
+  static constexpr int kGuardWarps = kConvertWarps - 1;
 };
 
 // Instruction descriptor of tcgen05.mma.kind::f16: fp32 accumulator (bit 4), the
@@ -239,14 +244,14 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
   return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
 
-// fp8: K and V tiles into the swizzled fp16 stages, by the three warps that TMA
-// leaves free. A thread has 16 bytes of a row at a time (32 bytes in the
+// fp8: K and V tiles into the swizzled fp16 stages, by the warps that load
+// or look on otherwise. A thread has 16 bytes of a row at a time (32 bytes in the
 // stage), kDepth of them in flight.
 template <int D, typename Args>
 __device__ __forceinline__ void convert_tiles(const Args& a, const Work& w, Control& c,
                                               unsigned char* stages, int tiles, int thread) {
   using S = TcShape<D>;
-  constexpr int kConverters = 3 * kWarpSize;
+  constexpr int kConverters = S::kConvertWarps * kWarpSize;
   constexpr int kRowChunks = D / 16;
   constexpr int kAll = kTileKeys * kRowChunks;
   constexpr int kDepth = 6;
@@ -576,15 +581,18 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
     }
   } else {
     shrink_registers<kOtherRegisters>();
-    if (warp == kMmaWarp) {
+    if (warp < S::kLoadWarp) {
       // The whole warp keeps step; the instructions are one lane's.
       constexpr uint32_t kScore = instruction<T>(kTileKeys, false);
       constexpr uint32_t kValue = instruction<T>(D, true);
+      const int issuer = warp - kMmaWarp;
       const uint32_t tmem = c.tmem;
+      const uint64_t first_key = smem_descriptor(stages);
+      const uint64_t first_value = value_descriptor(stages);
       auto full = [&](int t) { return wait_in(c, &c.bar.full[t % kStages], (t / kStages) & 1); };
-      auto score = [&](int i, int j) {
+      auto score = [&](int i, int t) {  // with the key tile of stage use t
         const uint64_t q = smem_descriptor(smem + i * S::kQBytes);
-        const uint64_t k = smem_descriptor(stages + (2 * j % kStages) * S::kTileBytes);
+        const uint64_t k = first_key + (t % kStages) * (S::kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           // 16 elements along d: 32 bytes inside a box, then the next box
@@ -593,69 +601,65 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         }
         mma_commit(&c.bar.s_full[i]);
       };
-      auto weigh = [&](int i, int j) {
-        const uint64_t v = value_descriptor(stages + ((2 * j + 1) % kStages) * S::kTileBytes);
+      auto weigh = [&](int i, int t) {  // with the value tile of stage use t
+        const uint64_t v = first_value + (t % kStages) * (S::kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-          mma_from_tmem(tmem + S::kOutColumn + i * D,
-                        tmem + S::kPColumn + i * S::kPStep + 8 * kk,
-                        v + kk * (2048 >> 4), kValue, (j | kk) != 0);
+          mma_from_tmem(tmem + S::kOutColumn + i * D, tmem + S::kPColumn + i * S::kPStep + 8 * kk,
+                        v + kk * (2048 >> 4), kValue, t > 1 || kk != 0);
         }
-        if (S::kOwnP && j + 1 < n[i]) mma_commit(&c.bar.p_free[i]);
-        if (j == n[i] - 1) mma_commit(&c.bar.o_full[i]);
+        if (t / 2 == n[i] - 1) {
+          mma_commit(&c.bar.o_full[i]);
+        } else if (S::kOwnP) {
+          mma_commit(&c.bar.p_free[i]);
+        }
       };
+      auto mine = [&](int i) { return S::kIssuers == 1 || i == issuer; };
+      // A stage is free once every issuer has committed behind its products with it.
       bool ok = wait_in(c, &c.bar.q_full, 0) && full(0);
-      if (ok) {
-        tc_fence_after();
-        if (elect_lane()) {
-          score(0, 0);
-          if (n[1] > 0) score(1, 0);
-          mma_commit(&c.bar.empty[0]);
+      tc_fence_after();
+      if (ok && elect_lane()) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (mine(i) && n[i] > 0) score(i, 0);
         }
+        mma_commit(&c.bar.empty[0]);
       }
       for (int j = 0; ok && j < tiles; ++j) {
         const bool more = j + 1 < tiles;
-        if constexpr (S::kOwnP) {
-          ok = !more || full(2 * j + 2);
+        if (S::kOwnP && more) {
+          ok = full(2 * j + 2);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (!ok || j + 1 >= n[i]) continue;
+            if (!ok || !mine(i) || j + 1 >= n[i]) continue;
             ok = wait_in(c, &c.bar.s_free[i], j & 1);
             tc_fence_after();
-            if (ok && elect_lane()) score(i, j + 1);
+            if (ok && elect_lane()) score(i, 2 * j + 2);
           }
-          ok = ok && full(2 * j + 1);
+          if (ok && elect_lane()) mma_commit(&c.bar.empty[(2 * j + 2) % kStages]);
+        }
+        ok = ok && full(2 * j + 1) && (S::kOwnP || !more || full(2 * j + 2));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!ok || j >= n[i]) continue;
-            ok = wait_in(c, &c.bar.p_ready[i], j & 1);
-            tc_fence_after();
-            if (ok && elect_lane()) weigh(i, j);
-          }
-        } else {
-          ok = full(2 * j + 1) && (!more || full(2 * j + 2));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!ok || j >= n[i]) continue;
-            ok = wait_in(c, &c.bar.p_ready[i], j & 1);
-            tc_fence_after();
-            if (ok && elect_lane()) {
-              weigh(i, j);
-              if (j + 1 < n[i]) score(i, j + 1);
-            }
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || !mine(i) || j >= n[i]) continue;
+          ok = wait_in(c, &c.bar.p_ready[i], j & 1);
+          tc_fence_after();
+          if (ok && elect_lane()) {
+            weigh(i, 2 * j + 1);
+            if (!S::kOwnP && j + 1 < n[i]) score(i, 2 * j + 2);
           }
         }
         if (ok && elect_lane()) {
           mma_commit(&c.bar.empty[(2 * j + 1) % kStages]);
-          if (more) mma_commit(&c.bar.empty[(2 * j + 2) % kStages]);
+          if (!S::kOwnP && more) mma_commit(&c.bar.empty[(2 * j + 2) % kStages]);
         }
       }
       if (elect_lane()) mma_commit(&c.bar.done);
     } else if (kFp8) {
       if constexpr (kFp8) {
-        convert_tiles<D>(a, w, c, stages, tiles, (warp - kLoadWarp) * kWarpSize + lane);
+        convert_tiles<D>(a, w, c, stages, tiles, (warp - S::kLoadWarp) * kWarpSize + lane);
       }
-    } else if (warp == kLoadWarp) {
+    } else if (warp == S::kLoadWarp) {
       for (int t = 0; t < 2 * tiles; ++t) {
         const int stage = t % kStages;
         if (*reinterpret_cast<volatile int*>(&c.aborted)) break;
@@ -696,7 +700,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
           }
         }
       }
-    } else if (kPass == kPrompt && warp > kLoadWarp) {
+    } else if (kPass == kPrompt) {
       // V tiles that reach past the block's first row's last key
       constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
       const int64_t first_limit = w.first_token;
@@ -707,8 +711,8 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         if (int64_t{j + 1} * kTileKeys - 1 > first_limit) {
           const uint4* v = reinterpret_cast<const uint4*>(stages + stage * S::kTileBytes);
 #pragma unroll 4
-          for (int t = (warp - kLoadWarp - 1) * kWarpSize + lane;
-               t < static_cast<int>(S::kTileBytes / 16); t += kGuardWarps * kWarpSize) {
+          for (int t = (warp - S::kLoadWarp - 1) * kWarpSize + lane;
+               t < static_cast<int>(S::kTileBytes / 16); t += S::kGuardWarps * kWarpSize) {
             const uint4 x = v[t];
             const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -732,10 +736,11 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
 // Set-up and release around attend(): barriers, tensor memory.
 template <int D>
 __device__ __forceinline__ void open_block(Control& c, bool guarded, bool converted) {
+  using S = TcShape<D>;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < TcShape<D>::kStages; ++s) {
-      mbarrier_init(&c.bar.full[s], converted ? 3 : 1);
-      mbarrier_init(&c.bar.empty[s], 1 + (guarded && (s & 1) ? kGuardWarps : 0));
+    for (int s = 0; s < S::kStages; ++s) {
+      mbarrier_init(&c.bar.full[s], converted ? S::kConvertWarps : 1);
+      mbarrier_init(&c.bar.empty[s], S::kIssuers + (guarded && (s & 1) ? S::kGuardWarps : 0));
     }
     mbarrier_init(&c.bar.q_full, kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) {
@@ -745,8 +750,8 @@ __device__ __forceinline__ void open_block(Control& c, bool guarded, bool conver
       mbarrier_init(&c.bar.p_free[i], 1);
       mbarrier_init(&c.bar.o_full[i], 1);
     }
-    mbarrier_init(&c.bar.guarded, kGuardWarps);
-    mbarrier_init(&c.bar.done, 1);
+    mbarrier_init(&c.bar.guarded, S::kGuardWarps);
+    mbarrier_init(&c.bar.done, S::kIssuers);
     c.aborted = 0;
     c.unsafe = 0;
     c.holes = 0;
@@ -771,7 +776,7 @@ __device__ __forceinline__ void close_block(Control& c) {
     tc_fence_after();
     tmem_dealloc(c.tmem, TcShape<D>::kTmemColumns);
   }
-  if (c.aborted && threadIdx.x == kLoadWarp * kWarpSize) {
+  if (c.aborted && threadIdx.x == TcShape<D>::kLoadWarp * kWarpSize) {
     // an expired wait: give loads that are still on their way a bounded time to land
     for (int s = 0; s < TcShape<D>::kStages; ++s) {
       for (uint32_t p = 0; p < 2; ++p) mbarrier_wait_limited(&c.bar.full[s], p, 1u << 16);
