@@ -347,20 +347,21 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
     {
       constexpr int kChunks = D / 8;
       constexpr int kRowsAtOnce = kWarpSize / kChunks;
-      constexpr int kBatch = 8;
+      constexpr int kBatch = 16;  // all loads of a 128-wide head in flight
       const TQ* query = static_cast<const TQ*>(a.query) + (lane % kChunks) * 8;
       const int64_t offset = (w.token0 + place.token) * a.query_stride + place.head * D;
+      constexpr int kLoads = kWarpSize / kRowsAtOnce < kBatch ? kWarpSize / kRowsAtOnce : kBatch;
 #pragma unroll 1
-      for (int r0 = 0; r0 < kWarpSize; r0 += kBatch * kRowsAtOnce) {
-        uint4 v[kBatch];
+      for (int r0 = 0; r0 < kWarpSize; r0 += kLoads * kRowsAtOnce) {
+        uint4 v[kLoads];
 #pragma unroll
-        for (int t = 0; t < kBatch; ++t) {
+        for (int t = 0; t < kLoads; ++t) {
           const int r = r0 + t * kRowsAtOnce + lane / kChunks;
           const int64_t at = __shfl_sync(kFullMask, offset, r);
           v[t] = r < live_rows ? load16(query + at) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int t = 0; t < kBatch; ++t) {
+        for (int t = 0; t < kLoads; ++t) {
           const int r = r0 + t * kRowsAtOnce + lane / kChunks;
           if constexpr (kFp8) {
             float f[8];
@@ -422,11 +423,20 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       }
       float* s = reinterpret_cast<float*>(raw);
       const int64_t key0 = int64_t{j} * kTileKeys;
+      // Tiles that some row must not see whole: `last` is the row's last key of
+      // the tile. It does not fall from lane to lane, so lane 0 tells which runs
+      // of 32 keys need no mask.
       if (key0 + kTileKeys - 1 > first_limit) {
         const int last = static_cast<int>(max(min(limit - key0, int64_t{kTileKeys}), int64_t{-1}));
+        const int all_see = __shfl_sync(kFullMask, last, 0) + 1;
 #pragma unroll
-        for (int k = 0; k < kTileKeys; ++k) {
-          if (k > last) s[k] = -INFINITY;
+        for (int q = 0; q < kTileKeys / 32; ++q) {
+          if (32 * q + 32 > all_see) {
+#pragma unroll
+            for (int k = 32 * q; k < 32 * q + 32; ++k) {
+              if (k > last) s[k] = -INFINITY;
+            }
+          }
         }
       }
       if constexpr (kPass == kPrefix) {
