@@ -60,29 +60,37 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-constexpr int kSoftmaxWarps = 8;
-constexpr int kMmaWarp = 8;
-constexpr int kThreads = 12 * kWarpSize;
 constexpr uint32_t kBoxBytes = kTileKeys * 128;  // 64 elements of 128 rows
 constexpr float kSlack = 8.0f;                   // log2 of how far a maximum may lag
 
 enum Pass : int { kPrompt, kPrefix };
 
-template <int D>
+// A block of one or two row tiles. Two share K and V and fill the SM. One
+// leaves room for a second block: half the rows to a block and twice as many
+// blocks, which spread more evenly over the SMs.
+template <int D, int kTiles>
 struct TcShape {
-  static constexpr int kStages = D == 64 ? 8 : 4;  // K and V tiles alternate: even
+  static constexpr int kStages =  // K and V tiles alternate: even
+      kTiles == 2 ? (D == 64 ? 8 : 4) : (D == 64 ? 4 : 2);
   static constexpr uint32_t kTileBytes = kTileKeys * D * 2;
   static constexpr uint32_t kQBytes = kTileRows * D * 2;
-  static constexpr size_t kSmem = 2 * kQBytes + kStages * kTileBytes + 1024;
-  static constexpr uint32_t kOutColumn = 256;  // of tile 0; tile 1 is D further
-  static constexpr bool kOwnP = D == 64;       // P beside S, 64 columns for each tile
-  static constexpr uint32_t kPColumn = kOwnP ? 256 + 2 * D : 0;
+  static constexpr size_t kSmem = kTiles * kQBytes + kStages * kTileBytes + 1024;
+  static constexpr uint32_t kOutColumn = kTiles * kTileKeys;  // of tile 0; tile 1 is D further
+  static constexpr bool kOwnP = D == 64;  // P beside S, 64 columns for each tile
+  static constexpr uint32_t kPColumn = kOwnP ? kOutColumn + kTiles * D : 0;
   static constexpr uint32_t kPStep = kOwnP ? kTileKeys / 2 : kTileKeys;
-  static constexpr uint32_t kTmemColumns = 512;
-  static constexpr int kIssuers = D == 64 ? 2 : 1;
-  static constexpr int kLoadWarp = kMmaWarp + kIssuers;
-  static constexpr int kConvertWarps = kThreads / kWarpSize - kLoadWarp;
+  static constexpr uint32_t kTmemColumns = kTiles * 256;
+  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kIssuers = D == 64 ? kTiles : 1;
+  static constexpr int kLoadWarp = kSoftmaxWarps + kIssuers;
+  static constexpr int kWarps = kSoftmaxWarps + 4;
+  static constexpr int kThreads = kWarps * kWarpSize;
+  static constexpr int kConvertWarps = kWarps - kLoadWarp;
   static constexpr int kGuardWarps = kConvertWarps - 1;
+  // Registers at launch: 168 for 384 threads, 128 for each of two blocks of
+  // 256; 2 x 208 + 88 = 3 x 168 and 208 + 48 = 2 x 128.
+  static constexpr int kSoftmaxRegisters = 208;
+  static constexpr int kOtherRegisters = kTiles == 2 ? 88 : 48;
 };
 
 // Instruction descriptor of tcgen05.mma.kind::f16: fp32 accumulator (bit 4), the
@@ -174,27 +182,24 @@ template <int kRegisters>
 __device__ __forceinline__ void shrink_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
 }
-// 384 threads launch with 168 registers each: 2 x 208 + 88 = 3 x 168.
-constexpr int kSoftmaxRegisters = 208;
-constexpr int kOtherRegisters = 88;
-
 // What a block works on. Row r is head (first_head + r) % group of the group and
 // token (or request) first_token + (first_head + r) / group.
 struct Work {
   int64_t first_token;  // within the sequence
   int64_t token0;       // kPrompt: the sequence's first token
   int first_head;
-  int rows;       // up to 256
+  int rows;       // up to 128 for each row tile
   int key_first;  // kPrefix: first key of its part of the prefix
   int key_last;
   int kv_head;
   int split;  // kPrefix
 };
 
+template <int kTiles>
 __device__ __forceinline__ void place_rows(Work& w, int64_t first_row, int64_t all_rows, int group) {
   w.first_token = first_row / group;
   w.first_head = static_cast<int>(first_row - w.first_token * group);
-  w.rows = static_cast<int>(min(int64_t{2 * kTileRows}, all_rows - first_row));
+  w.rows = static_cast<int>(min(int64_t{kTiles * kTileRows}, all_rows - first_row));
 }
 
 struct Barriers {
@@ -247,10 +252,9 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
 // fp8: K and V tiles into the swizzled fp16 stages, by the warps that load
 // or look on otherwise. A thread has 16 bytes of a row at a time (32 bytes in the
 // stage), kDepth of them in flight.
-template <int D, typename Args>
+template <typename S, int D, typename Args>
 __device__ __forceinline__ void convert_tiles(const Args& a, const Work& w, Control& c,
                                               unsigned char* stages, int tiles, int thread) {
-  using S = TcShape<D>;
   constexpr int kConverters = S::kConvertWarps * kWarpSize;
   constexpr int kRowChunks = D / 16;
   constexpr int kAll = kTileKeys * kRowChunks;
@@ -310,19 +314,19 @@ __device__ __forceinline__ void convert_tiles(const Args& a, const Work& w, Cont
 }
 
 // TQ: type of q and out; T: operand type of the products.
-template <typename TQ, typename T, bool kFp8, int D, int kPass, typename Args>
+template <typename TQ, typename T, bool kFp8, int D, int kTiles, int kPass, typename Args>
 __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUtensorMap* key_map,
                                        const CUtensorMap* value_map, Control& c, unsigned char* smem) {
-  using S = TcShape<D>;
+  using S = TcShape<D, kTiles>;
   constexpr int kStages = S::kStages;
   const int warp = __shfl_sync(kFullMask, threadIdx.x / kWarpSize, 0);  // known to be uniform
   const int lane = threadIdx.x & (kWarpSize - 1);
-  unsigned char* stages = smem + 2 * S::kQBytes;
+  unsigned char* stages = smem + kTiles * S::kQBytes;
 
   // key tiles of each row tile
-  int n[2];
+  int n[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < kTiles; ++i) {
     const int rows = min(w.rows - i * kTileRows, kTileRows);
     if (rows <= 0) {
       n[i] = 0;
@@ -334,8 +338,8 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
   }
   const int tiles = max(n[0], n[1]);
 
-  if (warp < kSoftmaxWarps) {
-    grow_registers<kSoftmaxRegisters>();
+  if (warp < S::kSoftmaxWarps) {
+    grow_registers<S::kSoftmaxRegisters>();
     const int i = warp / 4;
     const int warp_row = (warp % 4) * kWarpSize;  // of the tile
     const int row = i * kTileRows + warp_row + lane;
@@ -590,12 +594,12 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       }
     }
   } else {
-    shrink_registers<kOtherRegisters>();
+    shrink_registers<S::kOtherRegisters>();
     if (warp < S::kLoadWarp) {
       // The whole warp keeps step; the instructions are one lane's.
       constexpr uint32_t kScore = instruction<T>(kTileKeys, false);
       constexpr uint32_t kValue = instruction<T>(D, true);
-      const int issuer = warp - kMmaWarp;
+      const int issuer = warp - S::kSoftmaxWarps;
       const uint32_t tmem = c.tmem;
       const uint64_t first_key = smem_descriptor(stages);
       const uint64_t first_value = value_descriptor(stages);
@@ -630,7 +634,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       tc_fence_after();
       if (ok && elect_lane()) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kTiles; ++i) {
           if (mine(i) && n[i] > 0) score(i, 0);
         }
         mma_commit(&c.bar.empty[0]);
@@ -640,7 +644,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         if (S::kOwnP && more) {
           ok = full(2 * j + 2);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kTiles; ++i) {
             if (!ok || !mine(i) || j + 1 >= n[i]) continue;
             ok = wait_in(c, &c.bar.s_free[i], j & 1);
             tc_fence_after();
@@ -650,7 +654,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         }
         ok = ok && full(2 * j + 1) && (S::kOwnP || !more || full(2 * j + 2));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kTiles; ++i) {
           if (!ok || !mine(i) || j >= n[i]) continue;
           ok = wait_in(c, &c.bar.p_ready[i], j & 1);
           tc_fence_after();
@@ -667,7 +671,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       if (elect_lane()) mma_commit(&c.bar.done);
     } else if (kFp8) {
       if constexpr (kFp8) {
-        convert_tiles<D>(a, w, c, stages, tiles, (warp - S::kLoadWarp) * kWarpSize + lane);
+        convert_tiles<S, D>(a, w, c, stages, tiles, (warp - S::kLoadWarp) * kWarpSize + lane);
       }
     } else if (warp == S::kLoadWarp) {
       for (int t = 0; t < 2 * tiles; ++t) {
@@ -744,15 +748,14 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
 }
 
 // Set-up and release around attend(): barriers, tensor memory.
-template <int D>
+template <typename S>
 __device__ __forceinline__ void open_block(Control& c, bool guarded, bool converted) {
-  using S = TcShape<D>;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbarrier_init(&c.bar.full[s], converted ? S::kConvertWarps : 1);
       mbarrier_init(&c.bar.empty[s], S::kIssuers + (guarded && (s & 1) ? S::kGuardWarps : 0));
     }
-    mbarrier_init(&c.bar.q_full, kSoftmaxWarps);
+    mbarrier_init(&c.bar.q_full, S::kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) {
       mbarrier_init(&c.bar.s_full[i], 1);
       mbarrier_init(&c.bar.p_ready[i], 4);
@@ -767,28 +770,28 @@ __device__ __forceinline__ void open_block(Control& c, bool guarded, bool conver
     c.holes = 0;
     fence_mbarrier_init();
   }
-  if (threadIdx.x / kWarpSize == kMmaWarp) tmem_alloc(&c.tmem, TcShape<D>::kTmemColumns);
+  if (threadIdx.x / kWarpSize == S::kSoftmaxWarps) tmem_alloc(&c.tmem, S::kTmemColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
 }
 
-template <int D>
+template <typename S>
 __device__ __forceinline__ void close_block(Control& c) {
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x / kWarpSize == kMmaWarp) {
+  if (threadIdx.x / kWarpSize == S::kSoftmaxWarps) {
     // the issuer's last commit: no matrix instruction is still at work
     if ((threadIdx.x & (kWarpSize - 1)) == 0) {
       mbarrier_wait_bounded(&c.bar.done, 0);
     }
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(c.tmem, TcShape<D>::kTmemColumns);
+    tmem_dealloc(c.tmem, S::kTmemColumns);
   }
-  if (c.aborted && threadIdx.x == TcShape<D>::kLoadWarp * kWarpSize) {
+  if (c.aborted && threadIdx.x == S::kLoadWarp * kWarpSize) {
     // an expired wait: give loads that are still on their way a bounded time to land
-    for (int s = 0; s < TcShape<D>::kStages; ++s) {
+    for (int s = 0; s < S::kStages; ++s) {
       for (uint32_t p = 0; p < 2; ++p) mbarrier_wait_limited(&c.bar.full[s], p, 1u << 16);
     }
   }
@@ -798,40 +801,43 @@ __device__ __forceinline__ unsigned char* aligned_tiles(unsigned char* p) {
   return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t{1023});
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int D, int kTiles>
+__global__ void __launch_bounds__(TcShape<D, kTiles>::kThreads, 3 - kTiles)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap key_map,
                      const __grid_constant__ CUtensorMap value_map,
                      const __grid_constant__ PromptArgs a) {
+  using S = TcShape<D, kTiles>;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ Control control;
   wait_for_upstream_grid();
   release_downstream_grid();
-  const SequenceTile tile = find_tile<2 * kTileRows>(a.query_start, a.sequences, a.tokens, a.group,
-                                                     blockIdx.x / a.key_heads);
+  const SequenceTile tile = find_tile<kTiles * kTileRows>(a.query_start, a.sequences, a.tokens,
+                                                          a.group, blockIdx.x / a.key_heads);
   if (tile.tile < 0) return;
-  open_block<D>(control, true, false);
+  open_block<S>(control, true, false);
   Work w{};
-  place_rows(w, tile.tile * 2 * kTileRows, tile.length * a.group, a.group);
+  place_rows<kTiles>(w, tile.tile * kTiles * kTileRows, tile.length * a.group, a.group);
   w.token0 = tile.first_token;
   w.kv_head = static_cast<int>(blockIdx.x % a.key_heads);
-  attend<T, T, false, D, kPrompt>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
-  close_block<D>(control);
+  attend<T, T, false, D, kTiles, kPrompt>(a, w, &key_map, &value_map, control,
+                                          aligned_tiles(dynamic_smem));
+  close_block<S>(control);
 }
 
 template <typename TQ, typename T, bool kFp8, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(TcShape<D, 2>::kThreads, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap key_map,
                      const __grid_constant__ CUtensorMap value_map,
                      const __grid_constant__ DecodeArgs a) {
+  using S = TcShape<D, 2>;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ Control control;
-  open_block<D>(control, false, kFp8);
+  open_block<S>(control, false, kFp8);
   wait_for_upstream_grid();
   release_downstream_grid();
   Work w{};
-  place_rows(w, static_cast<int64_t>(blockIdx.x) * 2 * kTileRows,
-             static_cast<int64_t>(a.batch) * a.group, a.group);
+  place_rows<2>(w, static_cast<int64_t>(blockIdx.x) * 2 * kTileRows,
+                static_cast<int64_t>(a.batch) * a.group, a.group);
   w.kv_head = blockIdx.y;
   w.split = blockIdx.z;
   const int64_t tiles = (a.prefix_tokens + kTileKeys - 1) / kTileKeys;
@@ -840,16 +846,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     int64_t{a.prefix_tokens}));
   bool holes = false;
   for (int b = w.key_first / a.kv.block_size + threadIdx.x;
-       b <= (w.key_last - 1) / a.kv.block_size; b += kThreads) {
+       b <= (w.key_last - 1) / a.kv.block_size; b += S::kThreads) {
     holes |= static_cast<uint32_t>(a.prefix_blocks[b]) >= static_cast<uint32_t>(a.kv.num_blocks);
   }
   if (__syncthreads_or(holes) && threadIdx.x == 0) control.holes = 1;
   __syncthreads();
-  attend<TQ, T, kFp8, D, kPrefix>(a, w, &key_map, &value_map, control, aligned_tiles(dynamic_smem));
-  close_block<D>(control);
+  attend<TQ, T, kFp8, D, 2, kPrefix>(a, w, &key_map, &value_map, control,
+                                     aligned_tiles(dynamic_smem));
+  close_block<S>(control);
 }
 
 // ---- host ----------------------------------------------------------------------
+// Prompts run in single-tile blocks up to this many two-tile blocks per SM.
+// Measured (32/8 heads, D = 128 unless stated; single-tile against two-tile
+// blocks): 64 tokens 7.7 us against 9.8, seven prompts of 66-190 tokens 12.2
+// against 16.9, 1024 tokens 19.4 against 22.6, 4096 tokens 133 against 141, 19
+// prompts of up to 1500 tokens 172 against 177 and at D = 64 132 against 149;
+// 16384 tokens (13.8 blocks per SM) 2044 against 2008 in a long run: there
+// loading K and V once per block and not twice counts, and the ends do not.
+constexpr int kSingleTileWaves = 12;
+
 template <typename T>
 constexpr CUtensorMapDataType map_type() {
   return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
@@ -875,9 +891,20 @@ int encode_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* d
   return SM120N_OK;
 }
 
+template <typename T, int D, int kTiles>
+int run_prompt(const PromptArgs& a, const CUtensorMap* maps, cudaStream_t stream) {
+  using S = TcShape<D, kTiles>;
+  auto kernel = prompt_tc_kernel<T, D, kTiles>;
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
+  if (rc != SM120N_OK) return rc;
+  constexpr int64_t kRows = kTiles * kTileRows;
+  const int64_t tiles = (a.tokens * a.group + kRows - 1) / kRows + a.sequences;
+  return launch(kernel, dim3(static_cast<unsigned>(tiles * a.key_heads)), dim3(S::kThreads),
+                S::kSmem, stream, maps[0], maps[1], a);
+}
+
 template <typename T, int D>
-int run_prompt(const PromptArgs& a, cudaStream_t stream) {
-  using S = TcShape<D>;
+int run_prompt_tiles(const PromptArgs& a, cudaStream_t stream) {
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.key_heads) * D,
@@ -886,17 +913,17 @@ int run_prompt(const PromptArgs& a, cudaStream_t stream) {
     const int rc = encode_map<T>(&maps[i], i ? a.value : a.key, 2, dims, strides, kTileKeys);
     if (rc != SM120N_OK) return rc;
   }
-  auto kernel = prompt_tc_kernel<T, D>;
-  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
+  DeviceInfo dev;
+  const int rc = current_device_info(&dev);
   if (rc != SM120N_OK) return rc;
-  const int64_t tiles = (a.tokens * a.group + 2 * kTileRows - 1) / (2 * kTileRows) + a.sequences;
-  return launch(kernel, dim3(static_cast<unsigned>(tiles * a.key_heads)), dim3(kThreads), S::kSmem,
-                stream, maps[0], maps[1], a);
+  const int64_t pairs = (a.tokens * a.group + 2 * kTileRows - 1) / (2 * kTileRows) * a.key_heads;
+  return pairs <= kSingleTileWaves * dev.sm_count ? run_prompt<T, D, 1>(a, maps, stream)
+                                                  : run_prompt<T, D, 2>(a, maps, stream);
 }
 
 template <typename TQ, typename T, bool kFp8, int D>
 int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
-  using S = TcShape<D>;
+  using S = TcShape<D, 2>;
   CUtensorMap maps[2] = {};
   for (int i = 0; !kFp8 && i < 2; ++i) {
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(a.kv.block_size),
@@ -917,7 +944,7 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
   return launch(kernel,
                 dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.key_heads),
                      static_cast<unsigned>(a.prefix_splits)),
-                dim3(kThreads), S::kSmem, stream, maps[0], maps[1], a);
+                dim3(S::kThreads), S::kSmem, stream, maps[0], maps[1], a);
 }
 
 template <int D>
@@ -934,11 +961,11 @@ int run_prefix_typed(const DecodeArgs& a, int dtype, bool fp8, cudaStream_t stre
 
 int launch_prompt_tc(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream) {
   if (head_dim == 64) {
-    return dtype == SM120N_F16 ? run_prompt<__half, 64>(a, stream)
-                               : run_prompt<__nv_bfloat16, 64>(a, stream);
+    return dtype == SM120N_F16 ? run_prompt_tiles<__half, 64>(a, stream)
+                               : run_prompt_tiles<__nv_bfloat16, 64>(a, stream);
   }
-  return dtype == SM120N_F16 ? run_prompt<__half, 128>(a, stream)
-                             : run_prompt<__nv_bfloat16, 128>(a, stream);
+  return dtype == SM120N_F16 ? run_prompt_tiles<__half, 128>(a, stream)
+                             : run_prompt_tiles<__nv_bfloat16, 128>(a, stream);
 }
 
 int launch_prefix_tc(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
