@@ -37,7 +37,8 @@ SHARED_SOURCES = ["device_caches.cu", "cache_args.cu", "tensor_map.cu"]  # in bo
 NORM_SOURCES = ["runtime.cu", "row_norm.cu", "head_norm_rope.cu", "head_cache.cu", "norm_quant.cu",
                 "norm_fp4.cu", "qkv_gemm.cu", *SHARED_SOURCES]
 SERVING_SOURCES = ["serving_runtime.cu", "step_plan.cu", "head_mrope.cu", "attention.cu",
-                   "attention_mma.cu", "attention_tc.cu", *SHARED_SOURCES]
+                   "attention_mma.cu", "attention_tc.cu",
+                   "attention_decode.cu", *SHARED_SOURCES]
 BINDING_SOURCES = ["torch_binding.cpp", "serving_binding.cpp"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",

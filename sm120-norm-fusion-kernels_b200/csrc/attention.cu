@@ -47,7 +47,7 @@ int check_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int
 // there, 64 and 64 otherwise.
 bool prefix_on_tensor_memory(const sm120s_decode_args& a) {
   return a.head_dim <= 128 && a.num_blocks > 0 &&
-         (a.cache_dtype == SM120N_CACHE_FP8_E4M3 || block_fills_tiles(a.block_size));
+         (a.cache_dtype == SM120N_CACHE_FP8_E4M3 || block_fills_tiles(a.block_size, 128));
 }
 
 struct Plan {
@@ -101,9 +101,8 @@ int plan_decode(const sm120s_decode_args& a, Plan* plan) {
   plan->row_tiles = static_cast<int>((group + 15) / 16);
   const int64_t triples = a.batch * a.key_heads * plan->row_tiles;
   const int64_t most_tiles = (a.table_width * a.block_size + 63) / 64;
-  const int elem = a.cache_dtype == SM120N_CACHE_FP8_E4M3 ? 1 : 2;
   plan->own_grid = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(own_blocks_per_sm(static_cast<int>(a.head_dim) * elem) * dev.sm_count,
+      1, std::min<int64_t>(own_blocks_per_sm(static_cast<int>(a.head_dim)) * dev.sm_count,
                            triples * most_tiles)));
   plan->prefix_splits = 0;
   if (a.prefix_blocks_count > 0) {
@@ -273,7 +272,7 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
                                      : launch_prefix_mma(a, in.dtype, in.cache_dtype, head_dim, s);
     if (rc != SM120N_OK) return rc;
   }
-  rc = launch_own_mma(a, in.dtype, in.cache_dtype, head_dim, s);
+  rc = launch_own(a, in.dtype, in.cache_dtype, head_dim, s);
   if (rc != SM120N_OK) return rc;
   return launch_merge(a, in.dtype, head_dim, s);
 }

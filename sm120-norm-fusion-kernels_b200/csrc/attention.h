@@ -70,8 +70,8 @@ struct DecodeArgs {
   float* prefix_values;  // the same rows x head_dim
 };
 
-// Blocks per SM of the pass over own tokens for cache rows of this many bytes.
-int own_blocks_per_sm(int row_bytes);
+// Blocks per SM of the pass over own tokens.
+int own_blocks_per_sm(int head_dim);
 
 // One launch each; element types as sm120n_dtype, caches as sm120n_cache_dtype.
 int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
@@ -82,11 +82,16 @@ int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_
 int launch_prompt_tc(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
 int launch_prefix_tc(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
                      cudaStream_t stream);
-inline bool block_fills_tiles(int64_t block_size) {
-  return block_size % 128 == 0 || (block_size % 8 == 0 && 128 % block_size == 0);
+// Whether TMA boxes of cache blocks, in whole groups of the swizzle's 8 rows,
+// make up tiles of `keys` keys.
+inline bool block_fills_tiles(int64_t block_size, int keys) {
+  return block_size % keys == 0 || (block_size % 8 == 0 && keys % block_size == 0);
 }
-int launch_own_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
-                   cudaStream_t stream);
+int launch_own(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim, cudaStream_t stream);
 int launch_merge(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream);
+
+// Expired-wait counter of the pass over own tokens.
+int read_decode_faults(unsigned int* value);
+int reset_decode_faults();
 
 }  // namespace sm120n

@@ -1,0 +1,778 @@
+// attention_decode.cu -- a decode step's pass over each request's own cached
+// tokens, and the kernel that joins the parts of a row.
+//
+// Bound by memory: every cached key and value is read once, for all query heads
+// of its key head (up to 16 rows of one m16n8k16 tile). The key tiles of all
+// (request, key head, row tile) triples stand in one list, cut into
+// min(own_grid, tiles) equal runs, none empty: a block's run may end one triple
+// and begin others, and every triple it touches gets one partial result, at
+// index triple + block, which no other (triple, block) of the list shares. So
+// the load is even whatever the lengths are, and nothing depends on the order
+// in which blocks run.
+//
+// A block is four warps that compute and one that loads. The loader walks the
+// run tile by tile across the ends of triples, K and V into a ring of stages,
+// with the first tile of a triple also its query rows. Cache blocks that fill a
+// tile of 64 keys evenly come by TMA, one box for each block and 128 bytes of a
+// row; others row by row with cp.async, for which one warp is too slow to keep
+// HBM busy (1600 cycles to issue a tile of 32 KB; 4.4 TB/s). The four warps
+// share the rows and split the 64 keys of a tile; each keeps its own maximum,
+// sum and values until the triple ends. Keys behind the end, or in a block that
+// does not exist, are masked and their values zeroed, so nothing stored there
+// can reach a result.
+//
+// A stage holds K and V as boxes of 64 rows x 128 bytes with the TMA engine's
+// swizzle: 16-byte chunk c of row r at c ^ (r & 7), free of bank conflicts for
+// the matrix loads. fp8 tiles are read 16 bytes (K) and 4 bytes (V) at a time
+// instead; there column c of a group of eight scores stands for key c ^ 4 (c &
+// 1), which keeps rows that are read at once apart in both. (Rows of 64 bytes:
+// chunk c at c ^ ((r >> 1) & 3).)
+//
+// fp8 caches: e4m3 to fp16 is exact and one instruction for two values, so
+// these run the fp16 instruction, with each row of q scaled by a power of two
+// into [1, 2) first (exact but for elements 2^14 below the row's largest) and
+// the power folded into the row's score scale.
+#include <algorithm>
+
+#include "attention.h"
+#include "attention_utils.cuh"
+#include "tensor_core.cuh"
+#include "tensor_map.h"
+#include "warp_mma.cuh"
+
+namespace sm120n {
+
+__device__ unsigned int g_decode_expired_waits = 0;
+
+namespace {
+
+constexpr int kTileKeys = 64;
+constexpr int kWarps = 4;  // that compute
+constexpr int kThreads = (kWarps + 1) * kWarpSize;
+constexpr int kWarpKeys = kTileKeys / kWarps;
+constexpr int kMergeColumns = 32;
+
+template <bool kFp8, int D>
+struct OwnForm {
+  static constexpr int kRowBytes = D * (kFp8 ? 1 : 2);
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kBoxRow = kRowBytes < 128 ? kRowBytes : 128;  // bytes of a row in a box
+  static constexpr int kBoxes = kRowBytes / kBoxRow;
+  static constexpr int kBoxBytes = kTileKeys * kBoxRow;
+  // Byte offset of 16-byte chunk c of row r within a tile.
+  __device__ __forceinline__ static int chunk(int r, int c) {
+    if constexpr (kBoxRow == 64) return r * 64 + (c ^ ((r >> 1) & 3)) * 16;
+    return (c >> 3) * kBoxBytes + r * 128 + ((c & 7) ^ (r & 7)) * 16;
+  }
+  static constexpr int kTileBytes = kTileKeys * kRowBytes;
+  // About 100 KB of tiles to a block and two blocks to an SM, or 200 KB and one
+  // with heads of 256, whose values and queries fill a thread's registers: well
+  // past the 50 KB in flight that latency times bandwidth asks.
+  static constexpr int kStages = D == 256 ? (kFp8 ? 5 : 3) : kRowBytes == 256 ? 3 : 5;
+  static constexpr int kBlocksPerSm = D == 256 ? 1 : 2;
+  static constexpr size_t stage_bytes(int q_rows) { return 2 * kTileBytes + q_rows * D * 2; }
+  static constexpr size_t smem(int q_rows) {
+    return 1024 + kStages * stage_bytes(q_rows) + static_cast<size_t>(kWarps) * q_rows * kMergeColumns * 4;
+  }
+};
+
+__device__ __forceinline__ int own_tokens(const DecodeArgs& a, int request, int* first_key) {
+  const int64_t cap = static_cast<int64_t>(a.table_width) * a.kv.block_size;
+  const int64_t n = min(static_cast<int64_t>(max(a.seq_lens[request], 0)), cap);
+  const bool shares = n >= a.prefix_tokens;
+  *first_key = shares ? a.prefix_tokens : 0;
+  return static_cast<int>(n) - *first_key;
+}
+
+// A run's walk over the list, the same for the loader and the other warps.
+struct Walk {
+  int64_t at, end;  // tiles of the list
+  int64_t request_start;
+  int request;
+  // the triple at hand
+  int tiles;  // of this request
+  int kv_head, first_head;
+  int triple;
+  int first_key, keys;
+  int tile0, tile1;
+
+  __device__ __forceinline__ bool next(const DecodeArgs& a) {
+    if (at >= end) return false;
+    for (;;) {
+      keys = own_tokens(a, request, &first_key);
+      tiles = (keys + kTileKeys - 1) / kTileKeys;
+      const int64_t all = static_cast<int64_t>(tiles) * a.key_heads * a.row_tiles;
+      if (at < request_start + all) break;
+      request_start += all;
+      ++request;
+    }
+    triple = static_cast<int>((at - request_start) / tiles);
+    kv_head = triple / a.row_tiles;
+    first_head = (triple - kv_head * a.row_tiles) * 16;
+    const int64_t start = request_start + static_cast<int64_t>(triple) * tiles;
+    tile0 = static_cast<int>(at - start);
+    tile1 = static_cast<int>(min(end - start, static_cast<int64_t>(tiles)));
+    at = start + tile1;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void bar_compute() {  // the four computing warps
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+}
+
+__device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+// One arrival of this thread once its copies so far have landed.
+__device__ __forceinline__ void mbarrier_arrive_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(bar))
+               : "memory");
+}
+
+// Key of column c of a group of eight scores.
+template <bool kFp8>
+__device__ __forceinline__ int key_of(int c) {
+  return kFp8 ? c ^ ((c & 1) << 2) : c;
+}
+
+template <typename TQ, typename T, bool kFp8, int D, bool kTma>
+__global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
+    own_kernel(const __grid_constant__ CUtensorMap key_map,
+               const __grid_constant__ CUtensorMap value_map, const __grid_constant__ DecodeArgs a) {
+  using F = OwnForm<kFp8, D>;
+  constexpr int kStages = F::kStages;
+  extern __shared__ unsigned char dynamic_smem[];
+  // the swizzle repeats every 1024 bytes
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(dynamic_smem) + 1023) & ~uintptr_t{1023});
+  __shared__ __align__(8) uint64_t full[kStages];
+  __shared__ __align__(8) uint64_t empty[kStages];
+  __shared__ uint32_t live[kStages][2];  // which keys of a tile exist, one bit each
+  __shared__ float2 states[kWarps][16];
+  __shared__ int32_t warp_totals[kThreads / kWarpSize];
+  __shared__ int64_t found_start;
+  __shared__ int found_request;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / kWarpSize, 0);
+  const int lane = threadIdx.x & (kWarpSize - 1);
+  const int q_rows = a.group <= 8 ? 8 : 16;
+  const uint32_t stage_bytes = static_cast<uint32_t>(F::stage_bytes(q_rows));
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbarrier_init(&full[s], kWarpSize + 1);  // copies of every lane, and the masks
+      mbarrier_init(&empty[s], kWarps);
+    }
+    fence_mbarrier_init();
+  }
+  // Behind a prefix pass this one reads nothing that pass writes: it starts
+  // beside it, and waits for it only before it ends, so that its own end tells
+  // the joining kernel of both. Whatever came before the prefix pass is
+  // complete: that waited for it before it let this kernel start.
+  const bool beside_prefix = a.prefix_splits > 0;
+  if (!beside_prefix) wait_for_upstream_grid();
+  release_downstream_grid();
+
+  const int triples = a.key_heads * a.row_tiles;  // of one request
+  // Sums of the requests' tiles, kThreads requests at a step; f(request, tiles before, tiles).
+  auto over_requests = [&](auto f) {
+    int64_t before = 0;
+    for (int base = 0; base < a.batch; base += kThreads) {
+      const int i = base + threadIdx.x;
+      int first;
+      const int mine = i < a.batch ? (own_tokens(a, i, &first) + kTileKeys - 1) / kTileKeys : 0;
+      int64_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < kWarpSize; d *= 2) {
+        const int64_t x = __shfl_up_sync(kFullMask, upto, d);
+        if (lane >= d) upto += x;
+      }
+      __syncthreads();
+      if (lane == kWarpSize - 1) warp_totals[warp] = static_cast<int32_t>(upto);
+      __syncthreads();
+      int64_t all = 0;
+#pragma unroll
+      for (int k = 0; k < kThreads / kWarpSize; ++k) {
+        if (k < warp) upto += warp_totals[k];
+        all += warp_totals[k];
+      }
+      if (i < a.batch) f(i, before + upto - mine, mine);
+      before += all;
+    }
+    return before;
+  };
+  const int64_t total = over_requests([&](int i, int64_t start, int) {
+                          if (blockIdx.x == 0) a.tile_start[i] = static_cast<int32_t>(start);
+                        }) * triples;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = static_cast<int32_t>(total / triples);
+  const int64_t runs = min(total, int64_t{a.own_grid});
+  if (blockIdx.x >= runs) {
+    if (beside_prefix) wait_for_upstream_grid();
+    return;
+  }
+  Walk walk;
+  walk.at = total * blockIdx.x / runs;
+  walk.end = total * (blockIdx.x + 1) / runs;
+  over_requests([&](int i, int64_t start, int n) {
+    if (walk.at >= start * triples && walk.at < (start + n) * triples) {
+      found_request = i;
+      found_start = start * triples;
+    }
+  });
+  __syncthreads();
+  walk.request = found_request;
+  walk.request_start = found_start;
+
+  if (warp == kWarps) {
+    // ---- the loader
+    int use = 0;
+    bool ok = true;
+    while (ok && walk.next(a)) {
+      const int32_t* table = a.table + static_cast<int64_t>(walk.request) * a.table_stride;
+      const int64_t head = walk.kv_head * a.kv.head_stride * (kFp8 ? 1 : 2);
+      const unsigned char* key = static_cast<const unsigned char*>(a.kv.key) + head;
+      const unsigned char* value = static_cast<const unsigned char*>(a.kv.value) + head;
+      for (int t = walk.tile0; t < walk.tile1; ++t, ++use) {
+        const int stage = use % kStages;
+        uint32_t bits[2];    // which keys exist
+        int64_t offset[2];   // !kTma: byte offsets of rows `lane` and `lane + 32` within the head
+        const int box = min(a.kv.block_size, kTileKeys);  // kTma: rows; a lane has a box
+        int id = a.kv.num_blocks, slot = 0;               // outside the map: arrives as zeros
+        if constexpr (kTma) {
+          const int within = t * kTileKeys + lane * box;
+          int there = 0;
+          if (lane * box < kTileKeys && within < walk.keys) {
+            const uint32_t j = static_cast<uint32_t>(walk.first_key + within);
+            const uint32_t block = j / static_cast<uint32_t>(a.kv.block_size);
+            const int found = table[block];
+            if (static_cast<uint32_t>(found) < static_cast<uint32_t>(a.kv.num_blocks)) {
+              id = found;
+              slot = static_cast<int>(j - block * a.kv.block_size);
+              there = min(box, walk.keys - within);
+            }
+          }
+          const int mine = lane * box < kTileKeys ? lane * box : kTileKeys;  // first row of the box
+          uint32_t low = 0, high = 0;
+          if (there > 0) {
+            const uint64_t run = (there == 64 ? ~uint64_t{0} : (uint64_t{1} << there) - 1) << mine;
+            low = static_cast<uint32_t>(run);
+            high = static_cast<uint32_t>(run >> 32);
+          }
+          bits[0] = __reduce_or_sync(kFullMask, low);
+          bits[1] = __reduce_or_sync(kFullMask, high);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int within = t * kTileKeys + h * kWarpSize + lane;
+            offset[h] = -1;
+            if (within < walk.keys) {
+              const uint32_t j = static_cast<uint32_t>(walk.first_key + within);
+              const uint32_t block = j / static_cast<uint32_t>(a.kv.block_size);
+              const int found = table[block];
+              if (static_cast<uint32_t>(found) < static_cast<uint32_t>(a.kv.num_blocks)) {
+                offset[h] = (found * a.kv.block_stride +
+                             static_cast<int64_t>(j - block * a.kv.block_size) * a.kv.slot_stride) *
+                            (kFp8 ? 1 : 2);
+              }
+            }
+            bits[h] = __ballot_sync(kFullMask, offset[h] >= 0);
+          }
+        }
+        if (use >= kStages && !mbarrier_wait_bounded(&empty[stage], (use / kStages - 1) & 1)) {
+          if (lane == 0) atomicAdd(&g_decode_expired_waits, 1u);
+          ok = false;
+          break;
+        }
+        unsigned char* tile = smem + stage * stage_bytes;
+        const uint32_t to = shared_address(tile);
+        if (lane == 0) {
+          live[stage][0] = bits[0];
+          live[stage][1] = bits[1];
+          if constexpr (kTma) {
+            mbarrier_arrive_expect_tx(&full[stage], 2 * F::kTileBytes);
+          } else {
+            mbarrier_arrive(&full[stage]);
+          }
+        }
+        __syncwarp();
+        if constexpr (kTma) {
+          for (int b = 0; b < kTileKeys / box; ++b) {
+            const int block = __shfl_sync(kFullMask, id, b);
+            const int first_slot = __shfl_sync(kFullMask, slot, b);
+            if (elect_lane()) {
+#pragma unroll
+              for (int h = 0; h < F::kBoxes; ++h) {
+                unsigned char* part = tile + h * F::kBoxBytes + b * box * F::kBoxRow;
+                const int x = h * F::kBoxRow / (kFp8 ? 1 : 2);
+                tma_load_4d(part, &key_map, x, first_slot, walk.kv_head, block, &full[stage]);
+                tma_load_4d(part + F::kTileBytes, &value_map, x, first_slot, walk.kv_head, block,
+                            &full[stage]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll 8
+            for (int i = lane; i < kWarpSize * F::kChunks; i += kWarpSize) {
+              const int r = i / F::kChunks;
+              const int c = i % F::kChunks;
+              const int64_t from = __shfl_sync(kFullMask, offset[h], r);
+              const int64_t at = max(from, int64_t{0}) + c * 16;
+              const uint32_t place = to + F::chunk(h * kWarpSize + r, c);
+              copy16(place, key + at, from >= 0);
+              copy16(place + F::kTileBytes, value + at, from >= 0);
+            }
+          }
+        }
+        if (t == walk.tile0) {
+          const TQ* query = static_cast<const TQ*>(a.query) +
+                            static_cast<int64_t>(walk.request) * a.query_stride +
+                            (static_cast<int64_t>(walk.kv_head) * a.group + walk.first_head) * D;
+          const int rows = min(16, a.group - walk.first_head);
+          for (int i = lane; i < q_rows * (D / 8); i += kWarpSize) {
+            const int row = i / (D / 8), c = i % (D / 8);
+            copy16(to + 2 * F::kTileBytes + (row * (D / 8) + (c ^ (row & 7))) * 16,
+                   query + (row < rows ? row * D + c * 8 : 0), row < rows);
+          }
+        }
+        mbarrier_arrive_copies(&full[stage]);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (beside_prefix) wait_for_upstream_grid();
+    return;
+  }
+
+  // ---- the computing warps
+  const float head_scale = kFp8 ? a.scale_log2 * *a.k_scale : a.scale_log2;
+  float* merge = reinterpret_cast<float*>(smem + kStages * stage_bytes);  // [kWarps][q_rows][kMergeColumns]
+  const int g = lane >> 2, tq = lane & 3;
+  const int key0 = warp * kWarpKeys;
+  int use = 0;
+  bool ok = true;  // false after a wait ran out: keep step with the other warps, write nothing
+  while (walk.next(a)) {
+    const int rows = min(16, a.group - walk.first_head);
+    uint32_t q[D / 16][4];
+    float f0 = head_scale, f1 = head_scale;
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    for (int t = walk.tile0; t < walk.tile1; ++t, ++use) {
+      const int stage = use % kStages;
+      if (ok && !mbarrier_wait_bounded(&full[stage], (use / kStages) & 1)) {
+        if (lane == 0) atomicAdd(&g_decode_expired_waits, 1u);
+        ok = false;
+      }
+      if (!ok) continue;
+      unsigned char* tile = smem + stage * stage_bytes;
+      const uint32_t k = shared_address(tile);
+      const uint32_t v = k + F::kTileBytes;
+      if (t == walk.tile0) {
+        const unsigned char* q_tile = tile + 2 * F::kTileBytes;
+        if constexpr (!kFp8) {
+          const int r = (lane & 15) & (q_rows - 1);  // rows that do not exist repeat others
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            ldmatrix4(q[kk], shared_address(q_tile) + (r * (D / 8) + ((2 * kk + (lane >> 4)) ^ (r & 7))) * 16);
+          }
+        } else {
+          // in the order of the summed index that scores() below uses, scaled
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int r = (g + 8 * half) & (q_rows - 1);
+            uint4 raw[D / 32];
+            float most = 0.0f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              const int chunk = (c / 2) * 8 + 2 * tq + c % 2;
+              raw[c] = *reinterpret_cast<const uint4*>(q_tile + (r * (D / 8) + (chunk ^ (r & 7))) * 16);
+              float x[8];
+              Pack<TQ>::to_f32(raw[c], x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+            }
+            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+            // 2^-e and 2^e with e the exponent of the row's largest, kept normal
+            const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 2), 252);
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+            (half ? f1 : f0) *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              float x[8];
+              Pack<TQ>::to_f32(raw[c], x);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] *= down;
+              const uint4 y = Pack<T>::from_f32(x);
+              // run c / 2 of 64 elements: steps 2 (c % 2) and the next
+              const int kk = (c / 2) * 4 + 2 * (c % 2);
+              q[kk][half] = y.x;
+              q[kk][2 + half] = y.y;
+              q[kk + 1][half] = y.z;
+              q[kk + 1][2 + half] = y.w;
+            }
+          }
+        }
+      }
+      // scores of 16 rows x 16 keys
+      float s[2][4] = {};
+      if constexpr (!kFp8) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t b[4];
+          const int r = key0 + (lane & 7) + ((lane >> 4) << 3);
+          ldmatrix4(b, k + F::chunk(r, 2 * kk + ((lane >> 3) & 1)));
+          Mma<T>::mma(s[0], q[kk], b[0], b[1]);
+          Mma<T>::mma(s[1], q[kk], b[2], b[3]);
+        }
+      } else {
+        // The order of the summed index is free: in each run of 64 elements,
+        // step i of four takes elements 16t + 4i .. + 3 of lane t, so that a
+        // lane's bytes for four steps are one 16-byte load.
+#pragma unroll
+        for (int run = 0; run < D / 64; ++run) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                tile + F::chunk(key0 + n * 8 + key_of<true>(g), run * 4 + tq));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              Mma<T>::mma(s[n], q[run * 4 + i], e4m3_pair(w[i] & 0xffffu), e4m3_pair(w[i] >> 16));
+            }
+          }
+        }
+      }
+      const uint32_t there = (live[stage][warp / 2] >> (16 * (warp & 1))) & 0xffffu;  // of its keys
+      if (kTma && there != 0xffffu) {
+        // whole blocks came, with whatever lies behind the end: no weight, and no value
+        for (int i = lane; i < kWarpKeys * F::kChunks; i += kWarpSize) {
+          const int r = i / F::kChunks;
+          if (!((there >> r) & 1u)) {
+            *reinterpret_cast<uint4*>(tile + F::kTileBytes + F::chunk(key0 + r, i % F::kChunks)) =
+                make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_shared();  // before TMA fills the stage again
+        __syncwarp();
+      }
+      float top0 = m0, top1 = m1;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const bool real = (there >> (n * 8 + key_of<kFp8>(2 * tq + c))) & 1u;
+          s[n][c] = real ? s[n][c] * f0 : -INFINITY;
+          s[n][2 + c] = real ? s[n][2 + c] * f1 : -INFINITY;
+          top0 = fmaxf(top0, s[n][c]);
+          top1 = fmaxf(top1, s[n][2 + c]);
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d *= 2) {
+        top0 = fmaxf(top0, __shfl_xor_sync(kFullMask, top0, d));
+        top1 = fmaxf(top1, __shfl_xor_sync(kFullMask, top1, d));
+      }
+      // a row that has seen nothing yet keeps everything at zero
+      const float base0 = top0 == -INFINITY ? 0.0f : top0;
+      const float base1 = top1 == -INFINITY ? 0.0f : top1;
+      if (__any_sync(kFullMask, top0 > m0 || top1 > m1)) {
+        const float keep0 = exp2_approx(m0 - base0);
+        const float keep1 = exp2_approx(m1 - base1);
+        l0 *= keep0;
+        l1 *= keep1;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][0] *= keep0;
+          o[n][1] *= keep0;
+          o[n][2] *= keep1;
+          o[n][3] *= keep1;
+        }
+        m0 = top0;
+        m1 = top1;
+      }
+      uint32_t p[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float x0 = exp2_approx(s[n][0] - base0), y0 = exp2_approx(s[n][1] - base0);
+        const float x1 = exp2_approx(s[n][2] - base1), y1 = exp2_approx(s[n][3] - base1);
+        l0 += x0 + y0;
+        l1 += x1 + y1;
+        p[2 * n] = Pack<T>::f32_to_word(x0, y0);
+        p[2 * n + 1] = Pack<T>::f32_to_word(x1, y1);
+      }
+      if constexpr (!kFp8) {
+        const int r = key0 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < D / 8; n += 2) {
+          uint32_t b[4];
+          ldmatrix4_trans(b, v + F::chunk(r, n + (lane >> 4)));
+          Mma<T>::mma(o[n], p, b[0], b[1]);
+          Mma<T>::mma(o[n + 1], p, b[2], b[3]);
+        }
+      } else {
+        // The order of the columns is free: of a run of 32, lane group g
+        // holds 4g .. 4g + 3, the i-th of them in product i of four.
+#pragma unroll
+        for (int run = 0; run < D / 32; ++run) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = key0 + key_of<true>(2 * tq + (j & 1)) + (j >> 1) * 8;
+            w[j] = *reinterpret_cast<const uint32_t*>(
+                tile + F::kTileBytes + F::chunk(r, run * 2 + (g >> 2)) + (g & 3) * 4);
+          }
+          const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5140), hi0 = __byte_perm(w[0], w[1], 0x7362);
+          const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5140), hi1 = __byte_perm(w[2], w[3], 0x7362);
+          Mma<T>::mma(o[run * 4], p, e4m3_pair(lo0 & 0xffffu), e4m3_pair(lo1 & 0xffffu));
+          Mma<T>::mma(o[run * 4 + 1], p, e4m3_pair(lo0 >> 16), e4m3_pair(lo1 >> 16));
+          Mma<T>::mma(o[run * 4 + 2], p, e4m3_pair(hi0 & 0xffffu), e4m3_pair(hi1 & 0xffffu));
+          Mma<T>::mma(o[run * 4 + 3], p, e4m3_pair(hi0 >> 16), e4m3_pair(hi1 >> 16));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&empty[stage]);
+    }
+
+    // The four warps' states of the same rows become one partial result, a
+    // few columns at a time.
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+      l0 += __shfl_xor_sync(kFullMask, l0, d);
+      l1 += __shfl_xor_sync(kFullMask, l1, d);
+    }
+    if (tq == 0) {
+      states[warp][g] = make_float2(m0, l0);
+      states[warp][g + 8] = make_float2(m1, l1);
+    }
+    bar_compute();
+    float weight[2];  // of this warp's values of rows g and g + 8 in the joint result
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, states[w][g + 8 * half].x);
+      weight[half] = exp2_approx((half ? m1 : m0) - (top == -INFINITY ? 0.0f : top));
+    }
+    const int64_t slot = (static_cast<int64_t>(walk.request) * triples + walk.triple + blockIdx.x) * 16;
+    if (ok && threadIdx.x < rows) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, states[w][threadIdx.x].x);
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 st = states[w][threadIdx.x];
+        sum += st.y * exp2_approx(st.x - (top == -INFINITY ? 0.0f : top));
+      }
+      a.own_state[slot + threadIdx.x] = make_float2(top, sum);
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < D / kMergeColumns; ++c0) {
+#pragma unroll
+      for (int i = 0; i < kMergeColumns / 8; ++i) {
+        const int n = c0 * (kMergeColumns / 8) + i;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int row = g + 8 * half;
+          if (row >= rows) continue;
+          float* to = merge + (warp * q_rows + row) * kMergeColumns;
+          // columns of o[n]: neighbours, or (fp8) four apart in the run of 32
+          const int col = kFp8 ? 8 * tq + i : i * 8 + 2 * tq;
+          to[col] = o[n][2 * half] * weight[half];
+          to[col + (kFp8 ? 4 : 1)] = o[n][2 * half + 1] * weight[half];
+        }
+      }
+      bar_compute();
+      for (int i = threadIdx.x; i < rows * (kMergeColumns / 4); i += kWarps * kWarpSize) {
+        const int row = i / (kMergeColumns / 4), c = i % (kMergeColumns / 4);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(merge + (w * q_rows + row) * kMergeColumns + 4 * c);
+          sum.x += x.x;
+          sum.y += x.y;
+          sum.z += x.z;
+          sum.w += x.w;
+        }
+        if (ok) {
+          *reinterpret_cast<float4*>(a.own_values + (slot + row) * D + c0 * kMergeColumns + 4 * c) = sum;
+        }
+      }
+      bar_compute();
+    }
+  }
+  if (beside_prefix) wait_for_upstream_grid();
+}
+
+// ---- the parts of a row joined ---------------------------------------------------
+// One warp to a (request, query head): the parts of the prefix, then the runs
+// that touched the row's triple, always in this order. A lane reads the state
+// of one part, so that all of them arrive in one latency; then the values.
+template <typename TQ, int D>
+__global__ void __launch_bounds__(kWarps* kWarpSize) merge_kernel(DecodeArgs a) {
+  constexpr int kPer = D / kWarpSize;
+  const int lane = threadIdx.x & (kWarpSize - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / kWarpSize;
+  wait_for_upstream_grid();
+  release_downstream_grid();
+  if (row >= static_cast<int64_t>(a.batch) * a.query_heads) return;
+  const int request = static_cast<int>(row / a.query_heads);
+  const int head = static_cast<int>(row - static_cast<int64_t>(request) * a.query_heads);
+  const int kv_head = head / a.group;
+  const int in_group = head - kv_head * a.group;
+  int first_key;
+  const int keys = own_tokens(a, request, &first_key);
+  const int from_prefix = first_key > 0 ? a.prefix_splits : 0;  // does the request share the prefix?
+  int own_runs = 0;
+  int64_t own_row = 0;  // of the first run that touched the triple; the others follow 16 rows apart
+  if (keys > 0) {
+    const int triples = a.key_heads * a.row_tiles;
+    const int triple = kv_head * a.row_tiles + in_group / 16;
+    const int64_t total = static_cast<int64_t>(a.tile_start[a.batch]) * triples;
+    const int64_t n = a.tile_start[request + 1] - a.tile_start[request];
+    const int64_t t0 = static_cast<int64_t>(a.tile_start[request]) * triples + triple * n;
+    const int64_t runs = min(total, int64_t{a.own_grid});
+    // the runs that hold the triple's first and last tile
+    const int64_t from = ((t0 + 1) * runs - 1) / total;
+    own_runs = static_cast<int>(((t0 + n) * runs - 1) / total - from) + 1;
+    own_row = (static_cast<int64_t>(request) * triples + triple + from) * 16 + in_group % 16;
+  }
+  const int parts = from_prefix + own_runs;
+  float top = -INFINITY, sum = 0.0f;
+  float acc[kPer] = {};
+  for (int first = 0; first < parts; first += kWarpSize) {
+    const int part = first + lane;
+    float2 state = make_float2(-INFINITY, 0.0f);
+    const float* values = nullptr;
+    if (part < from_prefix) {
+      const int64_t at = static_cast<int64_t>(part) * a.batch * a.query_heads + row;
+      state = a.prefix_state[at];
+      values = a.prefix_values + at * D;
+    } else if (part < parts) {
+      const int64_t at = own_row + static_cast<int64_t>(part - from_prefix) * 16;
+      state = a.own_state[at];
+      values = a.own_values + at * D;
+    }
+    // nothing seen; a sum that is not zero has seen a NaN and passes it on
+    const bool seen = !(state.x == -INFINITY && state.y == 0.0f);
+    float next = state.x;
+#pragma unroll
+    for (int d = kWarpSize / 2; d > 0; d /= 2) next = fmaxf(next, __shfl_xor_sync(kFullMask, next, d));
+    next = fmaxf(next, top);
+    const float base = next == -INFINITY ? 0.0f : next;
+    const float keep = exp2_approx(top - base);
+    const float factor = seen ? exp2_approx(state.x - base) : 0.0f;
+    float part_sum = seen ? state.y * factor : 0.0f;
+#pragma unroll
+    for (int d = kWarpSize / 2; d > 0; d /= 2) part_sum += __shfl_xor_sync(kFullMask, part_sum, d);
+    top = next;
+    sum = sum * keep + part_sum;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] *= keep;
+    const unsigned those = __ballot_sync(kFullMask, seen);
+    const int count = min(parts - first, kWarpSize);
+#pragma unroll 4
+    for (int k = 0; k < count; ++k) {
+      const float f = __shfl_sync(kFullMask, factor, k);
+      const float* from = reinterpret_cast<const float*>(
+          __shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(values), k));
+      if ((those >> k) & 1u) {
+        float x[kPer];
+        if constexpr (kPer % 4 == 0) {
+#pragma unroll
+          for (int i = 0; i < kPer; i += 4) {
+            *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(from + lane * kPer + i);
+          }
+        } else {
+          *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from + lane * kPer);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] += x[i] * f;
+      }
+    }
+  }
+  const float v_scale = a.v_scale ? *a.v_scale : 1.0f;
+  const float inv = sum == 0.0f ? 0.0f : v_scale / sum;
+  TQ* out = static_cast<TQ*>(a.out) + request * a.out_stride + static_cast<int64_t>(head) * D + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer; i += 2) {
+    *reinterpret_cast<uint32_t*>(out + i) = Pack<TQ>::f32_to_word(acc[i] * inv, acc[i + 1] * inv);
+  }
+}
+
+template <typename TQ, typename T, bool kFp8, int D, bool kTma>
+int run_own(const DecodeArgs& a, cudaStream_t stream) {
+  using F = OwnForm<kFp8, D>;
+  CUtensorMap maps[2] = {};
+  for (int i = 0; kTma && i < 2; ++i) {
+    const int rc = encode_cache_map(&maps[i], i ? a.kv.value : a.kv.key, a.kv, D, a.key_heads,
+                                    kFp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tensor_map_type<T>(),
+                                    kFp8 ? 1 : 2, F::kBoxRow, kTileKeys);
+    if (rc != SM120N_OK) return rc;
+  }
+  auto kernel = own_kernel<TQ, T, kFp8, D, kTma>;
+  const size_t smem = F::smem(a.group <= 8 ? 8 : 16);
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), F::smem(16));
+  if (rc != SM120N_OK) return rc;
+  return launch(kernel, dim3(static_cast<unsigned>(a.own_grid)), dim3(kThreads), smem, stream,
+                maps[0], maps[1], a);
+}
+
+template <typename TQ, typename T, bool kFp8, int D>
+int run_own(const DecodeArgs& a, cudaStream_t stream) {
+  return block_fills_tiles(a.kv.block_size, kTileKeys) && a.kv.num_blocks > 0
+             ? run_own<TQ, T, kFp8, D, true>(a, stream)
+             : run_own<TQ, T, kFp8, D, false>(a, stream);
+}
+
+}  // namespace
+
+int own_blocks_per_sm(int head_dim) { return head_dim == 256 ? 1 : 2; }
+
+#define SM120S_BY_HEAD_DIM(CALL)      \
+  switch (head_dim) {                 \
+    case 64: return CALL(64);         \
+    case 128: return CALL(128);       \
+    default: return CALL(256);        \
+  }
+
+int launch_own(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim, cudaStream_t stream) {
+  const bool fp8 = cache_dtype == SM120N_CACHE_FP8_E4M3;
+#define CALL(D)                                                                       \
+  dtype == SM120N_F16 ? (fp8 ? run_own<__half, __half, true, D>(a, stream)            \
+                             : run_own<__half, __half, false, D>(a, stream))          \
+                      : (fp8 ? run_own<__nv_bfloat16, __half, true, D>(a, stream)     \
+                             : run_own<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream))
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+int launch_merge(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.query_heads;
+  const dim3 grid(static_cast<unsigned>((rows + kWarps - 1) / kWarps));
+  const dim3 block(kWarps * kWarpSize);
+#define CALL(D)                                                                         \
+  dtype == SM120N_F16 ? launch(merge_kernel<__half, D>, grid, block, 0, stream, a)      \
+                      : launch(merge_kernel<__nv_bfloat16, D>, grid, block, 0, stream, a)
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+int read_decode_faults(unsigned int* value) {
+  const cudaError_t err = cudaMemcpyFromSymbol(value, g_decode_expired_waits, sizeof *value);
+  return err == cudaSuccess ? SM120N_OK
+                            : fail(SM120N_ERR_CUDA, "reading the fault counter failed: %s",
+                                   cudaGetErrorString(err));
+}
+
+int reset_decode_faults() {
+  const unsigned int zero = 0;
+  const cudaError_t err = cudaMemcpyToSymbol(g_decode_expired_waits, &zero, sizeof zero);
+  return err == cudaSuccess ? SM120N_OK
+                            : fail(SM120N_ERR_CUDA, "resetting the fault counter failed: %s",
+                                   cudaGetErrorString(err));
+}
+
+}  // namespace sm120n

@@ -1,6 +1,6 @@
-// attention_mma.cu -- attention on warp-level matrix instructions: the pass of
-// a decode step over each request's own cached tokens, and prompts and shared
-// prefixes with the head size that has no tensor-memory form.
+// attention_mma.cu -- attention on warp-level matrix instructions, for what has
+// no tensor-memory form: prompts and shared prefixes with heads of 256, and
+// prefixes in blocks that do not fill a tile of 128 keys evenly.
 //
 //   o_i = sum_j softmax_j(scale * q_i . k_j) v_j
 // with the running maximum m and sum l of a row's exponentials: a tile of keys
@@ -9,9 +9,7 @@
 // p is rounded to the 16-bit operand type of the second product only.
 //
 // The query heads of one key head are rows of one tile, so K and V are read
-// once for all of them. A warp owns 16 rows. Where there are few rows (one
-// token per request) the four warps of a block share the rows and split the
-// 64 keys of a tile; otherwise each has rows of its own. K and V tiles go
+// once for all of them. A warp owns 16 rows. K and V tiles of 64 keys go
 // from global to shared memory by cp.async, kStages tiles deep, 16-byte
 // chunks swizzled so that every matrix load is free of bank conflicts. Keys
 // behind the end of the sequence, or in a block that does not exist, are
@@ -21,12 +19,11 @@
 // these run the fp16 instruction, with each row of q scaled by a power of two
 // into [1, 2) first (exact but for elements 2^14 below the row's largest) and
 // the power folded into the row's score scale.
-#include <cuda_fp8.h>
-
 #include <algorithm>
 
 #include "attention.h"
 #include "attention_utils.cuh"
+#include "warp_mma.cuh"
 
 namespace sm120n {
 namespace {
@@ -35,89 +32,20 @@ constexpr int kTileKeys = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * kWarpSize;
 
-enum Pass : int { kPrompt, kPrefix, kOwn };
+enum Pass : int { kPrompt, kPrefix };
 
-template <typename T>
-struct Mma;
-template <>
-struct Mma<__nv_bfloat16> {
-  __device__ __forceinline__ static void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <>
-struct Mma<__half> {
-  __device__ __forceinline__ static void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-
-__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t address) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(address)
-               : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, uint32_t address) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(address)
-               : "memory");
-}
-
-// 16 bytes from global to shared memory, zeros where `real` is false.
-__device__ __forceinline__ void copy16(uint32_t smem, const void* gmem, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem),
-               "r"(real ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
-// Two e4m3 bytes (low half of `b`) as two fp16 values.
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(b), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-}
-
-// Geometry of a pass: kRowWarps warps with rows of their own, the others
-// (kOwn) split the keys of a tile.
 template <typename T, bool kFp8, int D, int kPass>
 struct Form {
   static constexpr int kElem = kFp8 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
   static constexpr int kChunks = kRowBytes / 16;
-  static constexpr int kRows = kPass == kOwn ? 16 : 16 * kWarps;
-  static constexpr int kWarpKeys = kPass == kOwn ? kTileKeys / kWarps : kTileKeys;
+  static constexpr int kRows = 16 * kWarps;
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
   static constexpr int kQBytes = kRows * D * 2;
-  // Three tiles of K and V in flight, two for 512-byte rows: with two or
-  // three blocks to an SM that is 100 KB and more, past the 50 KB that
-  // latency times bandwidth asks of an SM.
+  // tiles of K and V in flight
   static constexpr int kStages = kRowBytes > 256 ? 2 : 3;
   static constexpr size_t kSmem = kQBytes + kStages * 2 * kTileBytes;
 };
-
-// Where 16-byte chunk c of a row lies. 16-bit tiles: the 8 rows of a matrix
-// hit 8 different chunks. fp8 tiles: two neighbouring rows read 64 bytes each
-// (K) and rows 0, 2, 4, 6 read 32 bytes each (V) at once.
-template <int kChunks, bool kFp8>
-__device__ __forceinline__ int chunk_at(int row, int c) {
-  if constexpr (!kFp8) return row * kChunks + (c ^ (row & 7));
-  if constexpr (kChunks == 4) return row * kChunks + (c ^ (((row >> 1) & 1) << 1));
-  return row * kChunks + (c ^ ((((row ^ (row >> 1)) & 1) << 2) | (((row >> 2) & 1) << 1)));
-}
 
 // A block's piece of work: rows of one key head against keys [key_first, key_last).
 struct Piece {
@@ -127,22 +55,16 @@ struct Piece {
   int key_last;
   int kv_head;
   int64_t token0;  // kPrompt: the sequence's first token
-  int request;     // kOwn
 };
 
 // Row `row` of a piece: its token and query head, as an offset into q or out.
 template <int kPass, typename Args>
 __device__ __forceinline__ int64_t row_offset(const Args& a, const Piece& p, int64_t row, int64_t stride,
                                               int d) {
-  if constexpr (kPass == kOwn) {
-    return static_cast<int64_t>(p.request) * stride +
-           (static_cast<int64_t>(p.kv_head) * a.group + p.first_row + row) * d;
-  } else {
-    const int64_t r = p.first_row + row;
-    const int64_t token = r / a.group;
-    const int64_t head = static_cast<int64_t>(p.kv_head) * a.group + (r - token * a.group);
-    return (p.token0 + token) * stride + head * d;
-  }
+  const int64_t r = p.first_row + row;
+  const int64_t token = r / a.group;
+  const int64_t head = static_cast<int64_t>(p.kv_head) * a.group + (r - token * a.group);
+  return (p.token0 + token) * stride + head * d;
 }
 
 template <typename TQ, typename T, bool kFp8, int D, int kPass, typename Args>
@@ -170,9 +92,7 @@ struct Worker {
       return p.token0 + j;
     } else {
       const int block = static_cast<int>(j / a.kv.block_size);
-      const int id = kPass == kPrefix
-                         ? a.prefix_blocks[block]
-                         : a.table[static_cast<int64_t>(p.request) * a.table_stride + block];
+      const int id = a.prefix_blocks[block];
       if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.kv.num_blocks)) return -1;
       return id * a.kv.block_stride + (j - static_cast<int64_t>(block) * a.kv.block_size) * a.kv.slot_stride;
     }
@@ -256,11 +176,10 @@ struct Worker {
     }
   }
 
-  // Scores of this warp's 16 rows x kWarpKeys keys of the tile in `stage`.
+  // Scores of this warp's 16 rows with the keys of the tile in `stage`.
   __device__ __forceinline__ void scores(int stage, float (*s)[4]) {
-    constexpr int kNt = F::kWarpKeys / 8;
-    const int key0 = kPass == kOwn ? warp * F::kWarpKeys : 0;
-    const int row0 = kPass == kOwn ? 0 : warp * 16;
+    constexpr int kNt = kTileKeys / 8;
+    const int row0 = warp * 16;
     const uint32_t q = shared_address(smem);
     const uint32_t k = shared_address(k_tile(stage));
 #pragma unroll
@@ -274,7 +193,7 @@ struct Worker {
 #pragma unroll
         for (int n = 0; n < kNt; n += 2) {
           uint32_t b[4];
-          const int r = key0 + n * 8 + (lane & 7) + ((lane >> 4) << 3);
+          const int r = n * 8 + (lane & 7) + ((lane >> 4) << 3);
           ldmatrix4(b, k + chunk_at<F::kChunks, false>(r, 2 * kk + ((lane >> 3) & 1)) * 16);
           Mma<T>::mma(s[n], qa, b[0], b[1]);
           Mma<T>::mma(s[n + 1], qa, b[2], b[3]);
@@ -303,7 +222,7 @@ struct Worker {
         }
 #pragma unroll
         for (int n = 0; n < kNt; ++n) {
-          const int r = key0 + n * 8 + g;
+          const int r = n * 8 + g;
           const uint4 v = *reinterpret_cast<const uint4*>(
               k_tile(stage) + chunk_at<F::kChunks, true>(r, run * 4 + t) * 16);
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -316,15 +235,14 @@ struct Worker {
     }
   }
 
-  // o += p v over this warp's keys; p as operand registers, 16 keys each.
+  // o += p v; p as operand registers, 16 keys each.
   __device__ __forceinline__ void weigh(int stage, const uint32_t (*p)[4]) {
-    const int key0 = kPass == kOwn ? warp * F::kWarpKeys : 0;
     unsigned char* tile = k_tile(stage) + F::kTileBytes;
     const uint32_t v = shared_address(tile);
 #pragma unroll
-    for (int kk = 0; kk < F::kWarpKeys / 16; ++kk) {
+    for (int kk = 0; kk < kTileKeys / 16; ++kk) {
       if constexpr (!kFp8) {
-        const int r = key0 + kk * 16 + (lane & 15);
+        const int r = kk * 16 + (lane & 15);
 #pragma unroll
         for (int n = 0; n < D / 8; n += 2) {
           uint32_t b[4];
@@ -341,7 +259,7 @@ struct Worker {
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int r = key0 + kk * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
+            const int r = kk * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
             w[j] = *reinterpret_cast<const uint32_t*>(
                 tile + chunk_at<F::kChunks, true>(r, run * 2 + (g >> 2)) * 16 + (g & 3) * 4);
           }
@@ -386,7 +304,7 @@ struct Worker {
   // Runs over the piece's keys. kPrompt: true when a value that some rows
   // must not see was infinite or NaN.
   __device__ __forceinline__ bool run(const Piece& p, float scale_log2) {
-    constexpr int kNt = F::kWarpKeys / 8;
+    constexpr int kNt = kTileKeys / 8;
     constexpr int kRing = F::kStages + 1;
     const int tiles = (p.key_last - p.key_first + kTileKeys - 1) / kTileKeys;
     bool unsafe = false;
@@ -406,7 +324,7 @@ struct Worker {
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.0f;
-    const int row0 = (kPass == kOwn ? 0 : warp * 16) + (lane >> 2);
+    const int row0 = warp * 16 + (lane >> 2);
     int64_t limit[2] = {0, 0};  // kPrompt: last key of the row
     if constexpr (kPass == kPrompt) {
       limit[0] = (p.first_row + row0) / a.group;
@@ -435,13 +353,12 @@ struct Worker {
       }
       const uint32_t live0 = live[slot * 2], live1 = live[slot * 2 + 1];
       const bool whole = (live0 & live1) == kFullMask;
-      const int warp_key = kPass == kOwn ? warp * F::kWarpKeys : 0;
       float top0 = m[0], top1 = m[1];
 #pragma unroll
       for (int n = 0; n < kNt; ++n) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int key = warp_key + n * 8 + 2 * (lane & 3) + c;
+          const int key = n * 8 + 2 * (lane & 3) + c;
           s[n][c] *= f0;
           s[n][2 + c] *= f1;
           const bool there = whole || (((key < 32 ? live0 : live1) >> (key & 31)) & 1u);
@@ -587,214 +504,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(DecodeArgs a) {
   }
 }
 
-// ---- each request's own tokens ------------------------------------------------------
-// The key tiles of all (request, key head, row tile) triples stand in one
-// list, cut into min(own_grid, tiles) equal runs, none empty: a block's run may
-// end one triple and begin others, and every triple it touches gets one
-// partial result, at index triple + block, which no other (triple, block) of
-// the list shares.
-__device__ __forceinline__ int own_tokens(const DecodeArgs& a, int request, int* first_block) {
-  const int64_t cap = static_cast<int64_t>(a.table_width) * a.kv.block_size;
-  const int64_t n = min(static_cast<int64_t>(max(a.seq_lens[request], 0)), cap);
-  const bool shares = n >= a.prefix_tokens;
-  *first_block = shares ? a.prefix_tokens : 0;
-  return static_cast<int>(n) - *first_block;
-}
-
-template <typename TQ, typename T, bool kFp8, int D>
-__global__ void __launch_bounds__(kThreads, 1) own_mma_kernel(DecodeArgs a) {
-  using F = Form<T, kFp8, D, kOwn>;
-  SM120S_WORKER(F);
-  __shared__ int32_t warp_totals[kWarps];
-  __shared__ int64_t found_start;
-  __shared__ int found_request;
-  wait_for_upstream_grid();
-  release_downstream_grid();
-  Worker<TQ, T, kFp8, D, kOwn, DecodeArgs> w{a, dynamic_smem, live, offsets, row_factor};
-  w.warp = threadIdx.x / kWarpSize;
-  w.lane = threadIdx.x & (kWarpSize - 1);
-  const int triples = a.key_heads * a.row_tiles;  // of one request
-  const float scale = kFp8 ? a.scale_log2 * *a.k_scale : a.scale_log2;
-
-  auto tiles_of = [&](int request) {
-    int first;
-    return (own_tokens(a, request, &first) + kTileKeys - 1) / kTileKeys;
-  };
-  // sums of the requests' tiles, chunk by chunk; f(request, tiles before, tiles)
-  auto over_requests = [&](auto f) {
-    int64_t before = 0;
-    for (int base = 0; base < a.batch; base += kThreads) {
-      const int i = base + threadIdx.x;
-      const int mine = i < a.batch ? tiles_of(i) : 0;
-      int upto = mine;
-#pragma unroll
-      for (int d = 1; d < kWarpSize; d *= 2) {
-        const int x = __shfl_up_sync(kFullMask, upto, d);
-        if (w.lane >= d) upto += x;
-      }
-      __syncthreads();
-      if (w.lane == kWarpSize - 1) warp_totals[w.warp] = upto;
-      __syncthreads();
-      int64_t all = 0;
-      for (int k = 0; k < kWarps; ++k) {
-        if (k < w.warp) upto += warp_totals[k];
-        all += warp_totals[k];
-      }
-      if (i < a.batch) f(i, before + upto - mine, mine);
-      before += all;
-    }
-    return before;
-  };
-  const int64_t total = over_requests([&](int i, int64_t start, int) {
-                          if (blockIdx.x == 0) a.tile_start[i] = static_cast<int32_t>(start);
-                        }) * triples;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = static_cast<int32_t>(total / triples);
-  const int64_t runs = min(total, int64_t{a.own_grid});
-  if (blockIdx.x >= runs) return;
-  int64_t at = total * blockIdx.x / runs;
-  const int64_t end = total * (blockIdx.x + 1) / runs;
-  over_requests([&](int i, int64_t start, int n) {
-    if (at >= start * triples && at < (start + n) * triples) {
-      found_request = i;
-      found_start = start * triples;
-    }
-  });
-  __syncthreads();
-  int request = found_request;
-  int64_t request_start = found_start;
-  while (at < end) {
-    int first_key;
-    const int keys = own_tokens(a, request, &first_key);
-    const int n = (keys + kTileKeys - 1) / kTileKeys;
-    if (n == 0) {
-      ++request;
-      continue;
-    }
-    const int triple = static_cast<int>((at - request_start) / n);
-    const int64_t triple_start = request_start + static_cast<int64_t>(triple) * n;
-    const int tile0 = static_cast<int>(at - triple_start);
-    const int tile1 = static_cast<int>(min(end - triple_start, int64_t{n}));
-    Piece p{};
-    p.request = request;
-    p.kv_head = triple / a.row_tiles;
-    p.first_row = static_cast<int64_t>(triple % a.row_tiles) * 16;
-    p.rows = min(16, a.group - static_cast<int>(p.first_row));
-    p.key_first = first_key + tile0 * kTileKeys;
-    p.key_last = first_key + min(tile1 * kTileKeys, keys);
-    w.run(p, scale);
-
-    // The four warps' states of the same rows become one; their values pass
-    // through the K / V stages, which the run has left.
-    __shared__ float2 states[kWarps][16];
-    float* values = reinterpret_cast<float*>(dynamic_smem + F::kQBytes);  // [kWarps][16][D]
-    static_assert(static_cast<size_t>(kWarps) * 16 * D * 4 <= F::kStages * 2 * F::kTileBytes,
-                  "the warps' partial values fit the stages");
-    __syncthreads();
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int row = (w.lane >> 2) + 8 * half;
-      if ((w.lane & 3) == 0) states[w.warp][row] = make_float2(w.m[half], w.l[half]);
-      if (row < p.rows) {
-        float* to = values + (w.warp * 16 + row) * D;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          to[w.column(i, 0)] = w.o[i][2 * half];
-          to[w.column(i, 1)] = w.o[i][2 * half + 1];
-        }
-      }
-    }
-    __syncthreads();
-    const int64_t slot = (static_cast<int64_t>(request) * triples + triple + blockIdx.x) * 16;
-    for (int i = threadIdx.x; i < p.rows * (D / 4); i += kThreads) {
-      const int row = i / (D / 4), c = i % (D / 4);
-      float top = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, states[k][row].x);
-      const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const float2 st = states[k][row];
-        const float f = exp2_approx(st.x - base);
-        sum += st.y * f;
-        const float4 x = *reinterpret_cast<const float4*>(values + (k * 16 + row) * D + 4 * c);
-        v.x += x.x * f;
-        v.y += x.y * f;
-        v.z += x.z * f;
-        v.w += x.w * f;
-      }
-      *reinterpret_cast<float4*>(a.own_values + (slot + row) * D + 4 * c) = v;
-      if (c == 0) a.own_state[slot + row] = make_float2(top, sum);
-    }
-    at = triple_start + tile1;
-    if (at >= request_start + static_cast<int64_t>(n) * triples) {
-      request_start += static_cast<int64_t>(n) * triples;
-      ++request;
-    }
-  }
-}
-
-// ---- the parts of a row joined ---------------------------------------------------
-// One warp to a (request, query head): the parts of the prefix, then the runs
-// that touched the row's triple, always in this order.
-template <typename TQ, int D>
-__global__ void __launch_bounds__(kThreads) merge_kernel(DecodeArgs a) {
-  constexpr int kPer = D / kWarpSize;
-  const int lane = threadIdx.x & (kWarpSize - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / kWarpSize;
-  wait_for_upstream_grid();
-  release_downstream_grid();
-  if (row >= static_cast<int64_t>(a.batch) * a.query_heads) return;
-  const int request = static_cast<int>(row / a.query_heads);
-  const int head = static_cast<int>(row - static_cast<int64_t>(request) * a.query_heads);
-  const int kv_head = head / a.group;
-  const int in_group = head - kv_head * a.group;
-  float top = -INFINITY, sum = 0.0f;
-  float acc[kPer] = {};
-  auto add = [&](float2 state, const float* values) {
-    // nothing seen; a sum that is not zero has seen a NaN and passes it on
-    if (state.x == -INFINITY && state.y == 0.0f) return;
-    const float next = fmaxf(top, state.x);
-    const float keep = exp2_approx(top - next);
-    const float f = exp2_approx(state.x - next);
-    top = next;
-    sum = sum * keep + state.y * f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * keep + values[lane * kPer + i] * f;
-  };
-  int first_key;
-  const int keys = own_tokens(a, request, &first_key);
-  if (first_key > 0) {  // the request shares the prefix
-    for (int s = 0; s < a.prefix_splits; ++s) {
-      const int64_t at = static_cast<int64_t>(s) * a.batch * a.query_heads + row;
-      add(a.prefix_state[at], a.prefix_values + at * D);
-    }
-  }
-  if (keys > 0) {
-    const int triples = a.key_heads * a.row_tiles;
-    const int triple = kv_head * a.row_tiles + in_group / 16;
-    const int64_t total = static_cast<int64_t>(a.tile_start[a.batch]) * triples;
-    const int64_t n = a.tile_start[request + 1] - a.tile_start[request];
-    const int64_t t0 = static_cast<int64_t>(a.tile_start[request]) * triples + triple * n;
-    // the runs that hold the triple's first and last tile
-    const int64_t runs = min(total, int64_t{a.own_grid});
-    const int64_t from = ((t0 + 1) * runs - 1) / total;
-    const int64_t to = ((t0 + n) * runs - 1) / total;
-    for (int64_t run = from; run <= to; ++run) {
-      const int64_t at = (static_cast<int64_t>(request) * triples + triple + run) * 16 + in_group % 16;
-      add(a.own_state[at], a.own_values + at * D);
-    }
-  }
-  const float v_scale = a.v_scale ? *a.v_scale : 1.0f;
-  const float inv = sum == 0.0f ? 0.0f : v_scale / sum;
-  TQ* out = static_cast<TQ*>(a.out) + request * a.out_stride + static_cast<int64_t>(head) * D + lane * kPer;
-#pragma unroll
-  for (int i = 0; i < kPer; i += 2) {
-    *reinterpret_cast<uint32_t*>(out + i) = Pack<TQ>::f32_to_word(acc[i] * inv, acc[i + 1] * inv);
-  }
-}
-
 template <typename T, int D>
 int run_prompt(const PromptArgs& a, cudaStream_t stream) {
   using F = Form<T, false, D, kPrompt>;
@@ -819,22 +528,7 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
                 dim3(kThreads), F::kSmem, stream, a);
 }
 
-template <typename TQ, typename T, bool kFp8, int D>
-int run_own(const DecodeArgs& a, cudaStream_t stream) {
-  using F = Form<T, kFp8, D, kOwn>;
-  auto kernel = own_mma_kernel<TQ, T, kFp8, D>;
-  int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), F::kSmem);
-  if (rc != SM120N_OK) return rc;
-  return launch(kernel, dim3(static_cast<unsigned>(a.own_grid)), dim3(kThreads), F::kSmem, stream, a);
-}
-
 }  // namespace
-
-// As many as shared memory holds (100 KB a block for 256-byte rows), at most four.
-int own_blocks_per_sm(int row_bytes) {
-  const int stages = row_bytes > 256 ? 2 : 3;
-  return std::min(4, 220 * 1024 / (stages * 2 * kTileKeys * row_bytes + 12 * 1024));
-}
 
 #define SM120S_BY_HEAD_DIM(CALL)      \
   switch (head_dim) {                 \
@@ -858,28 +552,6 @@ int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_
                              : run_prefix<__half, __half, false, D>(a, stream))          \
                       : (fp8 ? run_prefix<__nv_bfloat16, __half, true, D>(a, stream)     \
                              : run_prefix<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream))
-  SM120S_BY_HEAD_DIM(CALL)
-#undef CALL
-}
-
-int launch_own_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
-                   cudaStream_t stream) {
-  const bool fp8 = cache_dtype == SM120N_CACHE_FP8_E4M3;
-#define CALL(D)                                                                       \
-  dtype == SM120N_F16 ? (fp8 ? run_own<__half, __half, true, D>(a, stream)            \
-                             : run_own<__half, __half, false, D>(a, stream))          \
-                      : (fp8 ? run_own<__nv_bfloat16, __half, true, D>(a, stream)     \
-                             : run_own<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream))
-  SM120S_BY_HEAD_DIM(CALL)
-#undef CALL
-}
-
-int launch_merge(const DecodeArgs& a, int dtype, int head_dim, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.query_heads;
-  const dim3 grid(static_cast<unsigned>((rows + kWarps - 1) / kWarps));
-#define CALL(D)                                                                                \
-  dtype == SM120N_F16 ? launch(merge_kernel<__half, D>, grid, dim3(kThreads), 0, stream, a)    \
-                      : launch(merge_kernel<__nv_bfloat16, D>, grid, dim3(kThreads), 0, stream, a)
   SM120S_BY_HEAD_DIM(CALL)
 #undef CALL
 }

@@ -165,15 +165,6 @@ __device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
 }
 
-__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y,
-                                            int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(shared_address(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(shared_address(bar))
-      : "memory");
-}
-
 template <int kRegisters>
 __device__ __forceinline__ void grow_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
@@ -866,31 +857,6 @@ __global__ void __launch_bounds__(TcShape<D, 2>::kThreads, 1)
 // loading K and V once per block and not twice counts, and the ends do not.
 constexpr int kSingleTileWaves = 12;
 
-template <typename T>
-constexpr CUtensorMapDataType map_type() {
-  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-}
-
-// A map with boxes of 64 elements (128-byte swizzle) x `rows` of dimension 1.
-template <typename T>
-int encode_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-               const cuuint64_t* byte_strides, int rows) {
-  int rc = SM120N_OK;
-  auto encode = tensor_map_encoder(&rc);
-  if (rc != SM120N_OK) return rc;
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
-  const cuuint32_t steps[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, map_type<T>(), static_cast<cuuint32_t>(rank), const_cast<void*>(base),
-                            dims, byte_strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    return fail(SM120N_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
-  }
-  return SM120N_OK;
-}
-
 template <typename T, int D, int kTiles>
 int run_prompt(const PromptArgs& a, const CUtensorMap* maps, cudaStream_t stream) {
   using S = TcShape<D, kTiles>;
@@ -910,7 +876,9 @@ int run_prompt_tiles(const PromptArgs& a, cudaStream_t stream) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.key_heads) * D,
                                 static_cast<cuuint64_t>(a.tokens)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(i ? a.value_stride : a.key_stride) * 2};
-    const int rc = encode_map<T>(&maps[i], i ? a.value : a.key, 2, dims, strides, kTileKeys);
+    const cuuint32_t box[2] = {64, kTileKeys};
+    const int rc = encode_tensor_map(&maps[i], i ? a.value : a.key, tensor_map_type<T>(), 2, dims,
+                                     strides, box, 128);
     if (rc != SM120N_OK) return rc;
   }
   DeviceInfo dev;
@@ -926,15 +894,8 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
   using S = TcShape<D, 2>;
   CUtensorMap maps[2] = {};
   for (int i = 0; !kFp8 && i < 2; ++i) {
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(a.kv.block_size),
-                                static_cast<cuuint64_t>(a.key_heads),
-                                static_cast<cuuint64_t>(a.kv.num_blocks)};
-    // a dimension of one may have no stride of its own
-    auto bytes = [](int64_t stride) { return static_cast<cuuint64_t>(std::max<int64_t>(stride * 2, 16)); };
-    const cuuint64_t strides[3] = {bytes(a.kv.slot_stride), bytes(a.kv.head_stride),
-                                   bytes(a.kv.block_stride)};
-    const int rc = encode_map<T>(&maps[i], i ? a.kv.value : a.kv.key, 4, dims, strides,
-                                 std::min(a.kv.block_size, kTileKeys));
+    const int rc = encode_cache_map(&maps[i], i ? a.kv.value : a.kv.key, a.kv, D, a.key_heads,
+                                    tensor_map_type<T>(), 2, 128, kTileKeys);
     if (rc != SM120N_OK) return rc;
   }
   auto kernel = prefix_tc_kernel<TQ, T, kFp8, D>;
@@ -982,17 +943,22 @@ using namespace sm120n;
 extern "C" int sm120s_get_device_faults(uint32_t* out_count) {
   clear_error();
   if (!out_count) return fail(SM120N_ERR_INVALID_ARGUMENT, "out_count must be non-null");
-  const cudaError_t err = cudaMemcpyFromSymbol(out_count, g_attention_expired_waits, sizeof *out_count);
-  return err == cudaSuccess ? SM120N_OK
-                            : fail(SM120N_ERR_CUDA, "reading the fault counter failed: %s",
-                                   cudaGetErrorString(err));
+  unsigned int mine = 0, decode = 0;
+  const cudaError_t err = cudaMemcpyFromSymbol(&mine, g_attention_expired_waits, sizeof mine);
+  if (err != cudaSuccess) {
+    return fail(SM120N_ERR_CUDA, "reading the fault counter failed: %s", cudaGetErrorString(err));
+  }
+  const int rc = read_decode_faults(&decode);
+  if (rc == SM120N_OK) *out_count = mine + decode;
+  return rc;
 }
 
 extern "C" int sm120s_reset_device_faults(void) {
   clear_error();
   const unsigned int zero = 0;
   const cudaError_t err = cudaMemcpyToSymbol(g_attention_expired_waits, &zero, sizeof zero);
-  return err == cudaSuccess ? SM120N_OK
-                            : fail(SM120N_ERR_CUDA, "resetting the fault counter failed: %s",
-                                   cudaGetErrorString(err));
+  if (err != cudaSuccess) {
+    return fail(SM120N_ERR_CUDA, "resetting the fault counter failed: %s", cudaGetErrorString(err));
+  }
+  return reset_decode_faults();
 }

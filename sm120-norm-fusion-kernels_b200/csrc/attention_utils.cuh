@@ -1,8 +1,11 @@
 // attention_utils.cuh -- device code that the attention kernels share.
 #pragma once
 
+#include <algorithm>
+
 #include "attention.h"
 #include "device_utils.cuh"
+#include "tensor_map.h"
 
 namespace sm120n {
 
@@ -112,6 +115,48 @@ __device__ __forceinline__ SequenceTile find_tile(const int32_t* query_start, in
     before += __shfl_sync(kFullMask, upto, kWarpSize - 1);
   }
   return SequenceTile{0, 0, -1};
+}
+
+// ---- host: tensor maps ------------------------------------------------------------
+template <typename T>
+constexpr CUtensorMapDataType tensor_map_type() {
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// A map whose boxes have rows of `row_bytes` (64 or 128: the swizzle's span).
+inline int encode_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int rank,
+                             const cuuint64_t* dims, const cuuint64_t* byte_strides,
+                             const cuuint32_t* box, int row_bytes) {
+  int rc = SM120N_OK;
+  auto encode = tensor_map_encoder(&rc);
+  if (rc != SM120N_OK) return rc;
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims,
+                            byte_strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(SM120N_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  }
+  return SM120N_OK;
+}
+
+// A paged cache as [blocks, heads, slots, head_dim], boxes of one block's slots
+// (at most tile_keys) x row_bytes.
+inline int encode_cache_map(CUtensorMap* map, const void* base, const KvSource& kv, int head_dim,
+                            int heads, CUtensorMapDataType type, int elem, int row_bytes,
+                            int tile_keys) {
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(kv.block_size),
+                              static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(kv.num_blocks)};
+  // a dimension of one may have no stride of its own
+  auto bytes = [elem](int64_t stride) {
+    return static_cast<cuuint64_t>(std::max<int64_t>(stride * elem, 16));
+  };
+  const cuuint64_t strides[3] = {bytes(kv.slot_stride), bytes(kv.head_stride), bytes(kv.block_stride)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(row_bytes / elem),
+                             static_cast<cuuint32_t>(std::min(kv.block_size, tile_keys)), 1, 1};
+  return encode_tensor_map(map, base, type, 4, dims, strides, box, row_bytes);
 }
 
 }  // namespace sm120n
