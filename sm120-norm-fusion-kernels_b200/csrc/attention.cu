@@ -46,8 +46,7 @@ int check_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int
 // Whether the prefix runs on tensor memory: 256 rows and 128 keys to a tile
 // there, 64 and 64 otherwise.
 bool prefix_on_tensor_memory(const sm120s_decode_args& a) {
-  return a.head_dim <= 128 && a.num_blocks > 0 &&
-         (a.cache_dtype == SM120N_CACHE_FP8_E4M3 || block_fills_tiles(a.block_size, 128));
+  return a.head_dim <= 128 && a.num_blocks > 0 && block_fills_tiles(a.block_size, 128);
 }
 
 struct Plan {

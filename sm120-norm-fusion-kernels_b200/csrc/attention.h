@@ -77,8 +77,7 @@ int own_blocks_per_sm(int head_dim);
 int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
 int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
                       cudaStream_t stream);
-// Head sizes 64 and 128. The prefix form on a cache in dtype (loaded by TMA)
-// wants blocks that fill a tile of 128 keys evenly, in whole groups of 8.
+// Head sizes 64 and 128; the prefix form wants blocks that fill a tile of 128 keys.
 int launch_prompt_tc(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
 int launch_prefix_tc(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
                      cudaStream_t stream);

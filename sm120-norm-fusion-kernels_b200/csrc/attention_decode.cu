@@ -165,9 +165,10 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
     fence_mbarrier_init();
   }
   // Behind a prefix pass this one reads nothing that pass writes: it starts
-  // beside it, and waits for it only before it ends, so that its own end tells
-  // the joining kernel of both. Whatever came before the prefix pass is
-  // complete: that waited for it before it let this kernel start.
+  // beside it, and its first block waits for it before it ends, so that this
+  // grid's end tells the joining kernel of both. (One block: the others make
+  // room for those that have not started.) Whatever came before the prefix pass
+  // is complete: that waited for it before it let this kernel start.
   const bool beside_prefix = a.prefix_splits > 0;
   if (!beside_prefix) wait_for_upstream_grid();
   release_downstream_grid();
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = static_cast<int32_t>(total / triples);
   const int64_t runs = min(total, int64_t{a.own_grid});
   if (blockIdx.x >= runs) {
-    if (beside_prefix) wait_for_upstream_grid();
+    if (beside_prefix && blockIdx.x == 0) wait_for_upstream_grid();
     return;
   }
   Walk walk;
@@ -339,7 +340,6 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (beside_prefix) wait_for_upstream_grid();
     return;
   }
 
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
       bar_compute();
     }
   }
-  if (beside_prefix) wait_for_upstream_grid();
+  if (beside_prefix && blockIdx.x == 0) wait_for_upstream_grid();
 }
 
 // ---- the parts of a row joined ---------------------------------------------------
@@ -709,7 +709,7 @@ int run_own(const DecodeArgs& a, cudaStream_t stream) {
   for (int i = 0; kTma && i < 2; ++i) {
     const int rc = encode_cache_map(&maps[i], i ? a.kv.value : a.kv.key, a.kv, D, a.key_heads,
                                     kFp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tensor_map_type<T>(),
-                                    kFp8 ? 1 : 2, F::kBoxRow, kTileKeys);
+                                    kFp8 ? 1 : 2, F::kBoxRow, kTileKeys, true);
     if (rc != SM120N_OK) return rc;
   }
   auto kernel = own_kernel<TQ, T, kFp8, D, kTma>;

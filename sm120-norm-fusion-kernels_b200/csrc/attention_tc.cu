@@ -30,8 +30,8 @@
 // accesses are whole rows: a thread reading or writing its own row touches 32
 // lines in every instruction of its warp (4000 cycles for a block's rows).
 //
-// Prefixes in fp8 caches run as fp16: all but the issuers load and convert the tiles
-// (exact), each row of q is scaled by a power of two into [1, 2) first (exact
+// Prefixes in fp8 caches run as fp16: TMA brings raw tiles to a ring of their
+// own, and the warps that look on otherwise convert them into the stages (exact), each row of q is scaled by a power of two into [1, 2) first (exact
 // but for elements 2^14 below the row's largest) and the power goes into the
 // row's score scale.
 //
@@ -74,7 +74,11 @@ struct TcShape {
       kTiles == 2 ? (D == 64 ? 8 : 4) : (D == 64 ? 4 : 2);
   static constexpr uint32_t kTileBytes = kTileKeys * D * 2;
   static constexpr uint32_t kQBytes = kTileRows * D * 2;
-  static constexpr size_t kSmem = kTiles * kQBytes + kStages * kTileBytes + 1024;
+  static constexpr int kRawTiles = D == 64 ? 4 : 2;  // fp8 tiles on their way to be converted
+  static constexpr uint32_t kRawBytes = kTileKeys * D;
+  static constexpr size_t smem(bool fp8) {
+    return kTiles * kQBytes + kStages * kTileBytes + (fp8 ? kRawTiles * kRawBytes : 0) + 1024;
+  }
   static constexpr uint32_t kOutColumn = kTiles * kTileKeys;  // of tile 0; tile 1 is D further
   static constexpr bool kOwnP = D == 64;  // P beside S, 64 columns for each tile
   static constexpr uint32_t kPColumn = kOwnP ? kOutColumn + kTiles * D : 0;
@@ -85,8 +89,7 @@ struct TcShape {
   static constexpr int kLoadWarp = kSoftmaxWarps + kIssuers;
   static constexpr int kWarps = kSoftmaxWarps + 4;
   static constexpr int kThreads = kWarps * kWarpSize;
-  static constexpr int kConvertWarps = kWarps - kLoadWarp;
-  static constexpr int kGuardWarps = kConvertWarps - 1;
+  static constexpr int kGuardWarps = kWarps - kLoadWarp - 1;  // look on, or convert
   // Registers at launch: 168 for 384 threads, 128 for each of two blocks of
   // 256; 2 x 208 + 88 = 3 x 168 and 208 + 48 = 2 x 128.
   static constexpr int kSoftmaxRegisters = 208;
@@ -196,6 +199,8 @@ __device__ __forceinline__ void place_rows(Work& w, int64_t first_row, int64_t a
 struct Barriers {
   uint64_t full[8];
   uint64_t empty[8];
+  uint64_t raw_full[4];
+  uint64_t raw_empty[4];
   uint64_t q_full;
   uint64_t s_full[2];
   uint64_t p_ready[2];
@@ -240,67 +245,44 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
   return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
 
-// fp8: K and V tiles into the swizzled fp16 stages, by the warps that load
-// or look on otherwise. A thread has 16 bytes of a row at a time (32 bytes in the
-// stage), kDepth of them in flight.
-template <typename S, int D, typename Args>
-__device__ __forceinline__ void convert_tiles(const Args& a, const Work& w, Control& c,
-                                              unsigned char* stages, int tiles, int thread) {
-  constexpr int kConverters = S::kConvertWarps * kWarpSize;
+// fp8: raw tiles, which TMA has brought, into the swizzled fp16 stages. A thread
+// has 16 bytes of a row at a time, 32 in the stage.
+template <typename S, int D>
+__device__ __forceinline__ void convert_tiles(Control& c, unsigned char* stages,
+                                              const unsigned char* raw_tiles, int tiles, int thread) {
   constexpr int kRowChunks = D / 16;
   constexpr int kAll = kTileKeys * kRowChunks;
-  constexpr int kDepth = 6;
-  const int64_t head = w.kv_head * a.kv.head_stride;
   for (int t = 0; t < 2 * tiles; ++t) {
     const int stage = t % S::kStages;
-    const uint8_t* source = static_cast<const uint8_t*>(t & 1 ? a.kv.value : a.kv.key) + head;
+    const int slot = t % S::kRawTiles;
+    if (!wait_in(c, &c.bar.raw_full[slot], (t / S::kRawTiles) & 1)) return;
+    if (t >= S::kStages && !wait_in(c, &c.bar.empty[stage], (t / S::kStages - 1) & 1)) return;
+    const unsigned char* raw = raw_tiles + slot * S::kRawBytes;
     unsigned char* to = stages + stage * S::kTileBytes;
-    const int key0 = w.key_first + (t / 2) * kTileKeys;
-    bool free_stage = t < S::kStages;
-    for (int first = thread; first < kAll; first += kDepth * kConverters) {
-      uint4 v[kDepth];
+#pragma unroll 4
+    for (int at = thread; at < kAll; at += S::kGuardWarps * kWarpSize) {
+      const uint4 v = load16_shared(raw + at * 16);
+      const int row = at / kRowChunks;
+      const int chunk = 2 * (at % kRowChunks);  // of 16 bytes in the stage
+      const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+      uint32_t h[8];
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int at = first + d * kConverters;
-        const int key = key0 + at / kRowChunks;
-        v[d] = make_uint4(0, 0, 0, 0);
-        if (at < kAll && key < w.key_last) {
-          const uint32_t block = static_cast<uint32_t>(key) / static_cast<uint32_t>(a.kv.block_size);
-          const int id = a.prefix_blocks[block];
-          if (static_cast<uint32_t>(id) < static_cast<uint32_t>(a.kv.num_blocks)) {
-            v[d] = load16(source + id * a.kv.block_stride +
-                          static_cast<int64_t>(key - block * a.kv.block_size) * a.kv.slot_stride +
-                          (at % kRowChunks) * 16);
-          }
-        }
+      for (int e = 0; e < 4; ++e) {
+        h[2 * e] = e4m3_pair(words[e] & 0xffffu);
+        h[2 * e + 1] = e4m3_pair(words[e] >> 16);
       }
-      if (!free_stage) {
-        if (!wait_in(c, &c.bar.empty[stage], (t / S::kStages - 1) & 1)) return;
-        free_stage = true;
-      }
-#pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int at = first + d * kConverters;
-        if (at >= kAll) break;
-        const int row = at / kRowChunks;
-        const int chunk = 2 * (at % kRowChunks);  // of 16 bytes in the stage
-        const uint32_t words[4] = {v[d].x, v[d].y, v[d].z, v[d].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[2 * e] = e4m3_pair(words[e] & 0xffffu);
-          h[2 * e + 1] = e4m3_pair(words[e] >> 16);
-        }
-        unsigned char* box = to + (chunk / 8) * kBoxBytes + row * 128;
-        *reinterpret_cast<uint4*>(box + ((chunk % 8) ^ (row & 7)) * 16) =
-            make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(box + (((chunk + 1) % 8) ^ (row & 7)) * 16) =
-            make_uint4(h[4], h[5], h[6], h[7]);
-      }
+      unsigned char* box = to + (chunk / 8) * kBoxBytes + row * 128;
+      *reinterpret_cast<uint4*>(box + ((chunk % 8) ^ (row & 7)) * 16) =
+          make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(box + (((chunk + 1) % 8) ^ (row & 7)) * 16) =
+          make_uint4(h[4], h[5], h[6], h[7]);
     }
     fence_async_shared();
     __syncwarp();
-    if ((threadIdx.x & (kWarpSize - 1)) == 0) mbarrier_arrive(&c.bar.full[stage]);
+    if ((threadIdx.x & (kWarpSize - 1)) == 0) {
+      mbarrier_arrive(&c.bar.full[stage]);
+      mbarrier_arrive(&c.bar.raw_empty[slot]);
+    }
   }
 }
 
@@ -313,6 +295,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
   const int warp = __shfl_sync(kFullMask, threadIdx.x / kWarpSize, 0);  // known to be uniform
   const int lane = threadIdx.x & (kWarpSize - 1);
   unsigned char* stages = smem + kTiles * S::kQBytes;
+  unsigned char* raw_tiles = stages + kStages * S::kTileBytes;
 
   // key tiles of each row tile
   int n[2] = {0, 0};
@@ -660,50 +643,63 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         }
       }
       if (elect_lane()) mma_commit(&c.bar.done);
-    } else if (kFp8) {
-      if constexpr (kFp8) {
-        convert_tiles<S, D>(a, w, c, stages, tiles, (warp - S::kLoadWarp) * kWarpSize + lane);
-      }
     } else if (warp == S::kLoadWarp) {
       for (int t = 0; t < 2 * tiles; ++t) {
-        const int stage = t % kStages;
+        const int ring = kFp8 ? S::kRawTiles : kStages;
+        const int slot = t % ring;
+        uint64_t* loaded = kFp8 ? &c.bar.raw_full[slot] : &c.bar.full[slot];
+        uint64_t* emptied = kFp8 ? &c.bar.raw_empty[slot] : &c.bar.empty[slot];
         if (*reinterpret_cast<volatile int*>(&c.aborted)) break;
-        if (t >= kStages && !wait_in(c, &c.bar.empty[stage], (t / kStages - 1) & 1)) break;
-        unsigned char* to = stages + stage * S::kTileBytes;
+        if (t >= ring && !wait_in(c, emptied, (t / ring - 1) & 1)) break;
         const CUtensorMap* map = t & 1 ? value_map : key_map;
         const int key0 = (t / 2) * kTileKeys;
         if constexpr (kPass == kPrompt) {
+          unsigned char* to = stages + slot * S::kTileBytes;
           if (elect_lane()) {
-            mbarrier_arrive_expect_tx(&c.bar.full[stage], S::kTileBytes);
+            mbarrier_arrive_expect_tx(loaded, S::kTileBytes);
 #pragma unroll
             for (int h = 0; h < D / 64; ++h) {
               tma_load_2d(to + h * kBoxBytes, map, w.kv_head * D + 64 * h,
-                          static_cast<int>(w.token0) + key0, &c.bar.full[stage]);
+                          static_cast<int>(w.token0) + key0, loaded);
             }
           }
         } else {
-          // one box to a block of the cache (or 128 slots of a larger one); a
-          // lane to a box. Blocks that do not exist, and what is behind the
-          // end, lie outside the map and arrive as zeros.
-          if (elect_lane()) mbarrier_arrive_expect_tx(&c.bar.full[stage], S::kTileBytes);
-          __syncwarp();
+          // One box to a block of the cache (or 128 slots of a larger one) and
+          // 128 bytes of a row. Lane b finds box b; one lane asks for all of
+          // them. Blocks that do not exist, and what is behind the end, lie
+          // outside the map and arrive as zeros.
+          constexpr int kBoxes = kFp8 ? 1 : D / 64;
+          const int row_bytes = kFp8 ? D : 128;
+          unsigned char* to = kFp8 ? raw_tiles + slot * S::kRawBytes : stages + slot * S::kTileBytes;
           const int box = min(a.kv.block_size, kTileKeys);
-          for (int b = lane; b < kTileKeys / box; b += kWarpSize) {
-            const int64_t key = int64_t{w.key_first} + key0 + b * box;
-            int id = a.kv.num_blocks, slot = 0;
-            if (key < w.key_last) {
-              const int block = static_cast<int>(key / a.kv.block_size);
-              slot = static_cast<int>(key - static_cast<int64_t>(block) * a.kv.block_size);
-              id = a.prefix_blocks[block];
-              if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.kv.num_blocks)) id = a.kv.num_blocks;
+          const int64_t key = int64_t{w.key_first} + key0 + lane * box;
+          int id = a.kv.num_blocks, first_slot = 0;
+          if (lane * box < kTileKeys && key < w.key_last) {
+            const uint32_t block = static_cast<uint32_t>(key) / static_cast<uint32_t>(a.kv.block_size);
+            const int found = a.prefix_blocks[block];
+            if (static_cast<uint32_t>(found) < static_cast<uint32_t>(a.kv.num_blocks)) {
+              id = found;
+              first_slot = static_cast<int>(key - static_cast<int64_t>(block) * a.kv.block_size);
             }
+          }
+          if (elect_lane()) mbarrier_arrive_expect_tx(loaded, kFp8 ? S::kRawBytes : S::kTileBytes);
+          for (int b = 0; b < kTileKeys / box; ++b) {
+            const int block = __shfl_sync(kFullMask, id, b);
+            const int at = __shfl_sync(kFullMask, first_slot, b);
+            if (elect_lane()) {
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-              tma_load_4d(to + h * kBoxBytes + b * box * 128, map, 64 * h, slot, w.kv_head, id,
-                          &c.bar.full[stage]);
+              for (int h = 0; h < kBoxes; ++h) {
+                tma_load_4d(to + h * kBoxBytes + b * box * row_bytes, map, 64 * h, at, w.kv_head,
+                            block, loaded);
+              }
             }
           }
         }
+      }
+    } else if (kFp8) {
+      if constexpr (kFp8) {
+        convert_tiles<S, D>(c, stages, raw_tiles, tiles,
+                            (warp - S::kLoadWarp - 1) * kWarpSize + lane);
       }
     } else if (kPass == kPrompt) {
       // V tiles that reach past the block's first row's last key
@@ -743,8 +739,12 @@ template <typename S>
 __device__ __forceinline__ void open_block(Control& c, bool guarded, bool converted) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbarrier_init(&c.bar.full[s], converted ? S::kConvertWarps : 1);
+      mbarrier_init(&c.bar.full[s], converted ? S::kGuardWarps : 1);
       mbarrier_init(&c.bar.empty[s], S::kIssuers + (guarded && (s & 1) ? S::kGuardWarps : 0));
+    }
+    for (int s = 0; converted && s < S::kRawTiles; ++s) {
+      mbarrier_init(&c.bar.raw_full[s], 1);
+      mbarrier_init(&c.bar.raw_empty[s], S::kGuardWarps);
     }
     mbarrier_init(&c.bar.q_full, S::kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) {
@@ -861,12 +861,12 @@ template <typename T, int D, int kTiles>
 int run_prompt(const PromptArgs& a, const CUtensorMap* maps, cudaStream_t stream) {
   using S = TcShape<D, kTiles>;
   auto kernel = prompt_tc_kernel<T, D, kTiles>;
-  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::smem(false));
   if (rc != SM120N_OK) return rc;
   constexpr int64_t kRows = kTiles * kTileRows;
   const int64_t tiles = (a.tokens * a.group + kRows - 1) / kRows + a.sequences;
   return launch(kernel, dim3(static_cast<unsigned>(tiles * a.key_heads)), dim3(S::kThreads),
-                S::kSmem, stream, maps[0], maps[1], a);
+                S::smem(false), stream, maps[0], maps[1], a);
 }
 
 template <typename T, int D>
@@ -893,19 +893,20 @@ template <typename TQ, typename T, bool kFp8, int D>
 int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
   using S = TcShape<D, 2>;
   CUtensorMap maps[2] = {};
-  for (int i = 0; !kFp8 && i < 2; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const int rc = encode_cache_map(&maps[i], i ? a.kv.value : a.kv.key, a.kv, D, a.key_heads,
-                                    tensor_map_type<T>(), 2, 128, kTileKeys);
+                                    kFp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tensor_map_type<T>(),
+                                    kFp8 ? 1 : 2, kFp8 ? D : 128, kTileKeys, !kFp8);
     if (rc != SM120N_OK) return rc;
   }
   auto kernel = prefix_tc_kernel<TQ, T, kFp8, D>;
-  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::smem(kFp8));
   if (rc != SM120N_OK) return rc;
   const int64_t tiles = (static_cast<int64_t>(a.batch) * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
   return launch(kernel,
                 dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.key_heads),
                      static_cast<unsigned>(a.prefix_splits)),
-                dim3(S::kThreads), S::kSmem, stream, maps[0], maps[1], a);
+                dim3(S::kThreads), S::smem(kFp8), stream, maps[0], maps[1], a);
 }
 
 template <int D>

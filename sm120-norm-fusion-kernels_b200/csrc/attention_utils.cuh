@@ -124,7 +124,7 @@ constexpr CUtensorMapDataType tensor_map_type() {
                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
-// A map whose boxes have rows of `row_bytes` (64 or 128: the swizzle's span).
+// A map whose boxes have rows of `row_bytes` (64 or 128: the swizzle's span; 0: no swizzle).
 inline int encode_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int rank,
                              const cuuint64_t* dims, const cuuint64_t* byte_strides,
                              const cuuint32_t* box, int row_bytes) {
@@ -134,7 +134,9 @@ inline int encode_tensor_map(CUtensorMap* map, const void* base, CUtensorMapData
   const cuuint32_t steps[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims,
                             byte_strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            row_bytes == 0    ? CU_TENSOR_MAP_SWIZZLE_NONE
+                            : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                              : CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(SM120N_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
@@ -146,7 +148,7 @@ inline int encode_tensor_map(CUtensorMap* map, const void* base, CUtensorMapData
 // (at most tile_keys) x row_bytes.
 inline int encode_cache_map(CUtensorMap* map, const void* base, const KvSource& kv, int head_dim,
                             int heads, CUtensorMapDataType type, int elem, int row_bytes,
-                            int tile_keys) {
+                            int tile_keys, bool swizzled) {
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(kv.block_size),
                               static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(kv.num_blocks)};
   // a dimension of one may have no stride of its own
@@ -156,7 +158,7 @@ inline int encode_cache_map(CUtensorMap* map, const void* base, const KvSource& 
   const cuuint64_t strides[3] = {bytes(kv.slot_stride), bytes(kv.head_stride), bytes(kv.block_stride)};
   const cuuint32_t box[4] = {static_cast<cuuint32_t>(row_bytes / elem),
                              static_cast<cuuint32_t>(std::min(kv.block_size, tile_keys)), 1, 1};
-  return encode_tensor_map(map, base, type, 4, dims, strides, box, row_bytes);
+  return encode_tensor_map(map, base, type, 4, dims, strides, box, swizzled ? row_bytes : 0);
 }
 
 }  // namespace sm120n
