@@ -10,12 +10,12 @@
 // the load is even whatever the lengths are, and nothing depends on the order
 // in which blocks run.
 //
-// A block is four warps that compute and one that loads. The loader walks the
-// run tile by tile across the ends of triples, K and V into a ring of stages,
-// with the first tile of a triple also its query rows. Cache blocks that fill a
-// tile of 64 keys evenly come by TMA, one box for each block and 128 bytes of a
-// row; others row by row with cp.async, for which one warp is too slow to keep
-// HBM busy (1600 cycles to issue a tile of 32 KB; 4.4 TB/s). The four warps
+// A block is four warps that compute and two that load, one K and the queries
+// and one V. The loaders walk the run tile by tile across the ends of triples,
+// into a ring of stages, with the first tile of a triple also its query rows.
+// Cache blocks that fill a tile of 64 keys evenly come by TMA, one box for each
+// block and 128 bytes of a row; others row by row with cp.async, which is slower
+// to issue (1600 cycles for 32 KB by one warp; 4.4 TB/s). The four warps
 // share the rows and split the 64 keys of a tile; each keeps its own maximum,
 // sum and values until the triple ends. Keys behind the end, or in a block that
 // does not exist, are masked and their values zeroed, so nothing stored there
@@ -48,7 +48,8 @@ namespace {
 
 constexpr int kTileKeys = 64;
 constexpr int kWarps = 4;  // that compute
-constexpr int kThreads = (kWarps + 1) * kWarpSize;
+constexpr int kLoaders = 2;
+constexpr int kThreads = (kWarps + kLoaders) * kWarpSize;
 constexpr int kWarpKeys = kTileKeys / kWarps;
 constexpr int kMergeColumns = 32;
 
@@ -159,7 +160,8 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   const uint32_t stage_bytes = static_cast<uint32_t>(F::stage_bytes(q_rows));
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbarrier_init(&full[s], kWarpSize + 1);  // copies of every lane, and the masks
+      // of each loader: every lane's copies, and the masks or the bytes to come
+      mbarrier_init(&full[s], kLoaders * (kWarpSize + 1));
       mbarrier_init(&empty[s], kWarps);
     }
     fence_mbarrier_init();
@@ -223,121 +225,124 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   walk.request = found_request;
   walk.request_start = found_start;
 
-  if (warp == kWarps) {
-    // ---- the loader
-    int use = 0;
-    bool ok = true;
-    while (ok && walk.next(a)) {
-      const int32_t* table = a.table + static_cast<int64_t>(walk.request) * a.table_stride;
-      const int64_t head = walk.kv_head * a.kv.head_stride * (kFp8 ? 1 : 2);
-      const unsigned char* key = static_cast<const unsigned char*>(a.kv.key) + head;
-      const unsigned char* value = static_cast<const unsigned char*>(a.kv.value) + head;
-      for (int t = walk.tile0; t < walk.tile1; ++t, ++use) {
-        const int stage = use % kStages;
-        uint32_t bits[2];    // which keys exist
-        int64_t offset[2];   // !kTma: byte offsets of rows `lane` and `lane + 32` within the head
-        const int box = min(a.kv.block_size, kTileKeys);  // kTma: rows; a lane has a box
-        int id = a.kv.num_blocks, slot = 0;               // outside the map: arrives as zeros
-        if constexpr (kTma) {
-          const int within = t * kTileKeys + lane * box;
-          int there = 0;
-          if (lane * box < kTileKeys && within < walk.keys) {
-            const uint32_t j = static_cast<uint32_t>(walk.first_key + within);
-            const uint32_t block = j / static_cast<uint32_t>(a.kv.block_size);
-            const int found = table[block];
-            if (static_cast<uint32_t>(found) < static_cast<uint32_t>(a.kv.num_blocks)) {
-              id = found;
-              slot = static_cast<int>(j - block * a.kv.block_size);
-              there = min(box, walk.keys - within);
-            }
-          }
-          const int mine = lane * box < kTileKeys ? lane * box : kTileKeys;  // first row of the box
-          uint32_t low = 0, high = 0;
-          if (there > 0) {
-            const uint64_t run = (there == 64 ? ~uint64_t{0} : (uint64_t{1} << there) - 1) << mine;
-            low = static_cast<uint32_t>(run);
-            high = static_cast<uint32_t>(run >> 32);
-          }
-          bits[0] = __reduce_or_sync(kFullMask, low);
-          bits[1] = __reduce_or_sync(kFullMask, high);
-        } else {
+  if (warp >= kWarps) {
+    // ---- the loaders: the first brings K and the queries, the second V
+    const bool first_loader = warp == kWarps;
+    const CUtensorMap* map = first_loader ? &key_map : &value_map;
+    const unsigned char* cache =
+        static_cast<const unsigned char*>(first_loader ? a.kv.key : a.kv.value);
+    const uint32_t part = first_loader ? 0 : F::kTileBytes;
+    constexpr int kElem = kFp8 ? 1 : 2;
+    // A tile's rows in the cache. kTma: lane b has box b, the slots of one cache
+    // block (or 64 of a larger one). Otherwise rows `lane` and `lane + 32`. They
+    // are looked up one tile ahead of the wait for its stage.
+    constexpr int kMine = kTma ? 1 : 2;
+    const int box = kTma ? min(a.kv.block_size, kTileKeys) : 1;
+    int block[kMine], slot[kMine], count[kMine];
+    auto look_up = [&](int t) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int within = t * kTileKeys + h * kWarpSize + lane;
-            offset[h] = -1;
-            if (within < walk.keys) {
-              const uint32_t j = static_cast<uint32_t>(walk.first_key + within);
-              const uint32_t block = j / static_cast<uint32_t>(a.kv.block_size);
-              const int found = table[block];
-              if (static_cast<uint32_t>(found) < static_cast<uint32_t>(a.kv.num_blocks)) {
-                offset[h] = (found * a.kv.block_stride +
-                             static_cast<int64_t>(j - block * a.kv.block_size) * a.kv.slot_stride) *
-                            (kFp8 ? 1 : 2);
-              }
-            }
-            bits[h] = __ballot_sync(kFullMask, offset[h] >= 0);
-          }
+      for (int h = 0; h < kMine; ++h) {
+        const int first = (h * kWarpSize + lane) * box;
+        const int within = t * kTileKeys + first;
+        count[h] = first < kTileKeys ? max(min(box, walk.keys - within), 0) : 0;
+        if (count[h] > 0) {
+          const uint32_t j = static_cast<uint32_t>(walk.first_key + within);
+          const uint32_t b = j / static_cast<uint32_t>(a.kv.block_size);
+          slot[h] = static_cast<int>(j - b * a.kv.block_size);
+          block[h] = a.table[static_cast<int64_t>(walk.request) * a.table_stride + b];
         }
-        if (use >= kStages && !mbarrier_wait_bounded(&empty[stage], (use / kStages - 1) & 1)) {
-          if (lane == 0) atomicAdd(&g_decode_expired_waits, 1u);
-          ok = false;
-          break;
+      }
+    };
+    int use = 0;
+    bool more = walk.next(a);
+    int t = walk.tile0;
+    if (more) look_up(t);
+    while (more) {
+      const int stage = use % kStages;
+      int now_block[kMine], now_slot[kMine];
+      uint32_t bits[2] = {0, 0};  // which keys exist
+#pragma unroll
+      for (int h = 0; h < kMine; ++h) {
+        const bool there = count[h] > 0 &&
+                           static_cast<uint32_t>(block[h]) < static_cast<uint32_t>(a.kv.num_blocks);
+        // outside the map: arrives as zeros
+        now_block[h] = there ? block[h] : kTma ? a.kv.num_blocks : -1;
+        now_slot[h] = there ? slot[h] : 0;
+        if constexpr (kTma) {
+          const uint64_t run =
+              !there ? 0 : (count[h] == 64 ? ~uint64_t{0} : (uint64_t{1} << count[h]) - 1) << (lane * box);
+          bits[0] = __reduce_or_sync(kFullMask, static_cast<uint32_t>(run));
+          bits[1] = __reduce_or_sync(kFullMask, static_cast<uint32_t>(run >> 32));
+        } else {
+          bits[h] = __ballot_sync(kFullMask, there);
         }
-        unsigned char* tile = smem + stage * stage_bytes;
-        const uint32_t to = shared_address(tile);
-        if (lane == 0) {
+      }
+      const bool begins = t == walk.tile0;
+      const int kv_head = walk.kv_head;
+      const int rows = min(16, a.group - walk.first_head);
+      const TQ* query = static_cast<const TQ*>(a.query) +
+                        static_cast<int64_t>(walk.request) * a.query_stride +
+                        (static_cast<int64_t>(kv_head) * a.group + walk.first_head) * D;
+      if (++t >= walk.tile1) {
+        more = walk.next(a);
+        t = walk.tile0;
+      }
+      if (more) look_up(t);
+
+      if (use >= kStages && !mbarrier_wait_bounded(&empty[stage], (use / kStages - 1) & 1)) {
+        if (lane == 0) atomicAdd(&g_decode_expired_waits, 1u);
+        break;
+      }
+      unsigned char* tile = smem + stage * stage_bytes;
+      const uint32_t to = shared_address(tile);
+      if (lane == 0) {
+        if (first_loader) {
           live[stage][0] = bits[0];
           live[stage][1] = bits[1];
-          if constexpr (kTma) {
-            mbarrier_arrive_expect_tx(&full[stage], 2 * F::kTileBytes);
-          } else {
-            mbarrier_arrive(&full[stage]);
-          }
         }
-        __syncwarp();
         if constexpr (kTma) {
-          for (int b = 0; b < kTileKeys / box; ++b) {
-            const int block = __shfl_sync(kFullMask, id, b);
-            const int first_slot = __shfl_sync(kFullMask, slot, b);
-            if (elect_lane()) {
-#pragma unroll
-              for (int h = 0; h < F::kBoxes; ++h) {
-                unsigned char* part = tile + h * F::kBoxBytes + b * box * F::kBoxRow;
-                const int x = h * F::kBoxRow / (kFp8 ? 1 : 2);
-                tma_load_4d(part, &key_map, x, first_slot, walk.kv_head, block, &full[stage]);
-                tma_load_4d(part + F::kTileBytes, &value_map, x, first_slot, walk.kv_head, block,
-                            &full[stage]);
-              }
-            }
-          }
+          mbarrier_arrive_expect_tx(&full[stage], F::kTileBytes);
         } else {
+          mbarrier_arrive(&full[stage]);
+        }
+      }
+      __syncwarp();
+      if constexpr (kTma) {
+        for (int b = 0; b < kTileKeys / box; ++b) {
+          const int from = __shfl_sync(kFullMask, now_block[0], b);
+          const int first_slot = __shfl_sync(kFullMask, now_slot[0], b);
+          if (elect_lane()) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll 8
-            for (int i = lane; i < kWarpSize * F::kChunks; i += kWarpSize) {
-              const int r = i / F::kChunks;
-              const int c = i % F::kChunks;
-              const int64_t from = __shfl_sync(kFullMask, offset[h], r);
-              const int64_t at = max(from, int64_t{0}) + c * 16;
-              const uint32_t place = to + F::chunk(h * kWarpSize + r, c);
-              copy16(place, key + at, from >= 0);
-              copy16(place + F::kTileBytes, value + at, from >= 0);
+            for (int h = 0; h < F::kBoxes; ++h) {
+              tma_load_4d(tile + part + h * F::kBoxBytes + b * box * F::kBoxRow, map,
+                          h * F::kBoxRow / kElem, first_slot, kv_head, from, &full[stage]);
             }
           }
         }
-        if (t == walk.tile0) {
-          const TQ* query = static_cast<const TQ*>(a.query) +
-                            static_cast<int64_t>(walk.request) * a.query_stride +
-                            (static_cast<int64_t>(walk.kv_head) * a.group + walk.first_head) * D;
-          const int rows = min(16, a.group - walk.first_head);
-          for (int i = lane; i < q_rows * (D / 8); i += kWarpSize) {
-            const int row = i / (D / 8), c = i % (D / 8);
-            copy16(to + 2 * F::kTileBytes + (row * (D / 8) + (c ^ (row & 7))) * 16,
-                   query + (row < rows ? row * D + c * 8 : 0), row < rows);
+      } else {
+#pragma unroll
+        for (int h = 0; h < kMine; ++h) {
+          const int64_t offset = (now_block[h] * a.kv.block_stride + now_slot[h] * a.kv.slot_stride +
+                                  kv_head * a.kv.head_stride) * kElem;
+#pragma unroll 8
+          for (int i = lane; i < kWarpSize * F::kChunks; i += kWarpSize) {
+            const int r = i / F::kChunks;
+            const int c = i % F::kChunks;
+            const int64_t from = __shfl_sync(kFullMask, offset, r);
+            const bool there = (bits[h] >> r) & 1u;
+            copy16(to + part + F::chunk(h * kWarpSize + r, c), cache + (there ? from : 0) + c * 16, there);
           }
         }
-        mbarrier_arrive_copies(&full[stage]);
       }
+      if (first_loader && begins) {
+        for (int i = lane; i < q_rows * (D / 8); i += kWarpSize) {
+          const int row = i / (D / 8), c = i % (D / 8);
+          copy16(to + 2 * F::kTileBytes + (row * (D / 8) + (c ^ (row & 7))) * 16,
+                 query + (row < rows ? row * D + c * 8 : 0), row < rows);
+        }
+      }
+      mbarrier_arrive_copies(&full[stage]);
+      ++use;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
