@@ -444,7 +444,9 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              Mma<T>::mma(s[n], q[run * 4 + i], e4m3_pair(w[i] & 0xffffu), e4m3_pair(w[i] >> 16));
+              uint32_t b0, b1;
+              e4m3_to_half(w[i], b0, b1);
+              Mma<T>::mma(s[n], q[run * 4 + i], b0, b1);
             }
           }
         }
@@ -528,12 +530,14 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
             w[j] = *reinterpret_cast<const uint32_t*>(
                 tile + F::kTileBytes + F::chunk(r, run * 2 + (g >> 2)) + (g & 3) * 4);
           }
-          const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5140), hi0 = __byte_perm(w[0], w[1], 0x7362);
-          const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5140), hi1 = __byte_perm(w[2], w[3], 0x7362);
-          Mma<T>::mma(o[run * 4], p, e4m3_pair(lo0 & 0xffffu), e4m3_pair(lo1 & 0xffffu));
-          Mma<T>::mma(o[run * 4 + 1], p, e4m3_pair(lo0 >> 16), e4m3_pair(lo1 >> 16));
-          Mma<T>::mma(o[run * 4 + 2], p, e4m3_pair(hi0 & 0xffffu), e4m3_pair(hi1 & 0xffffu));
-          Mma<T>::mma(o[run * 4 + 3], p, e4m3_pair(hi0 >> 16), e4m3_pair(hi1 >> 16));
+          // pairs of neighbouring keys: columns 0, 1 in one word, 2, 3 in the next
+          uint32_t lo[4], hi[4];
+          e4m3_to_half(__byte_perm(w[0], w[1], 0x5140), lo[0], lo[1]);
+          e4m3_to_half(__byte_perm(w[0], w[1], 0x7362), lo[2], lo[3]);
+          e4m3_to_half(__byte_perm(w[2], w[3], 0x5140), hi[0], hi[1]);
+          e4m3_to_half(__byte_perm(w[2], w[3], 0x7362), hi[2], hi[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) Mma<T>::mma(o[run * 4 + i], p, lo[i], hi[i]);
         }
       }
       __syncwarp();

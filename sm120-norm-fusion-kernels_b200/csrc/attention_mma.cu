@@ -228,7 +228,9 @@ struct Worker {
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            Mma<T>::mma(s[n], qa[i], e4m3_pair(w[i] & 0xffffu), e4m3_pair(w[i] >> 16));
+            uint32_t b0, b1;
+            e4m3_to_half(w[i], b0, b1);
+            Mma<T>::mma(s[n], qa[i], b0, b1);
           }
         }
       }
@@ -263,12 +265,14 @@ struct Worker {
             w[j] = *reinterpret_cast<const uint32_t*>(
                 tile + chunk_at<F::kChunks, true>(r, run * 2 + (g >> 2)) * 16 + (g & 3) * 4);
           }
-          const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5140), hi0 = __byte_perm(w[0], w[1], 0x7362);
-          const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5140), hi1 = __byte_perm(w[2], w[3], 0x7362);
-          Mma<T>::mma(o[run * 4], p[kk], e4m3_pair(lo0 & 0xffffu), e4m3_pair(lo1 & 0xffffu));
-          Mma<T>::mma(o[run * 4 + 1], p[kk], e4m3_pair(lo0 >> 16), e4m3_pair(lo1 >> 16));
-          Mma<T>::mma(o[run * 4 + 2], p[kk], e4m3_pair(hi0 & 0xffffu), e4m3_pair(hi1 & 0xffffu));
-          Mma<T>::mma(o[run * 4 + 3], p[kk], e4m3_pair(hi0 >> 16), e4m3_pair(hi1 >> 16));
+          // pairs of neighbouring keys: columns 0, 1 in one word, 2, 3 in the next
+          uint32_t lo[4], hi[4];
+          e4m3_to_half(__byte_perm(w[0], w[1], 0x5140), lo[0], lo[1]);
+          e4m3_to_half(__byte_perm(w[0], w[1], 0x7362), lo[2], lo[3]);
+          e4m3_to_half(__byte_perm(w[2], w[3], 0x5140), hi[0], hi[1]);
+          e4m3_to_half(__byte_perm(w[2], w[3], 0x7362), hi[2], hi[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) Mma<T>::mma(o[run * 4 + i], p[kk], lo[i], hi[i]);
         }
       }
     }

@@ -43,8 +43,6 @@
 //
 // Every wait on an mbarrier is bounded; one that runs out is counted
 // (sm120s_get_device_faults) and ends the block without results.
-#include <cuda_fp8.h>
-
 #include <algorithm>
 
 #include "attention.h"
@@ -239,12 +237,6 @@ __device__ __forceinline__ RowPlace row_place(const Args& a, const Work& w, int 
                   static_cast<int64_t>(w.kv_head) * a.group + (r - step * a.group)};
 }
 
-// Two e4m3 bytes as two fp16 values.
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(b), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-}
-
 // fp8: raw tiles, which TMA has brought, into the swizzled fp16 stages. A thread
 // has 16 bytes of a row at a time, 32 in the stage.
 template <typename S, int D>
@@ -267,10 +259,7 @@ __device__ __forceinline__ void convert_tiles(Control& c, unsigned char* stages,
       const uint32_t words[4] = {v.x, v.y, v.z, v.w};
       uint32_t h[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        h[2 * e] = e4m3_pair(words[e] & 0xffffu);
-        h[2 * e + 1] = e4m3_pair(words[e] >> 16);
-      }
+      for (int e = 0; e < 4; ++e) e4m3_to_half(words[e], h[2 * e], h[2 * e + 1]);
       unsigned char* box = to + (chunk / 8) * kBoxBytes + row * 128;
       *reinterpret_cast<uint4*>(box + ((chunk % 8) ^ (row & 7)) * 16) =
           make_uint4(h[0], h[1], h[2], h[3]);

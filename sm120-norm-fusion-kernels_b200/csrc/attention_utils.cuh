@@ -15,6 +15,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Four e4m3 bytes as two words of two fp16 values, exact: one instruction a
+// word, which takes either half of a register as it is. (Through the header's
+// conversion of a 16-bit pair, taking the pairs apart and putting the halves
+// together again cost more than the conversion.)
+__device__ __forceinline__ void e4m3_to_half(uint32_t bytes, uint32_t& low, uint32_t& high) {
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(low), "=r"(high)
+      : "r"(bytes));
+}
+
 // One row of a prompt by plain arithmetic, one warp, keys one by one: for the
 // rows of a block that has an infinite or NaN value among the keys that some
 // of its rows must not see (a matrix product would multiply it by zero).

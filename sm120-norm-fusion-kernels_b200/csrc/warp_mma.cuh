@@ -2,8 +2,6 @@
 // and the shared-memory layouts of K and V tiles they read.
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include "device_utils.cuh"
 
 namespace sm120n {
@@ -54,12 +52,6 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int kPending>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
-// Two e4m3 bytes (low half of `b`) as two fp16 values.
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(b), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
 
 // Where 16-byte chunk c of a row lies. 16-bit tiles: the 8 rows of a matrix
