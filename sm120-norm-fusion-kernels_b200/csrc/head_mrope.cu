@@ -12,14 +12,16 @@
 // implementation whose roundings would have to be matched here, and one
 // rounding is the more accurate choice.
 //
-// Bound by memory. Work unit, lane layout and loads are those of
-// head_cache_kernel: one head of one token on D/16 lanes, 16-byte accesses,
-// rotation partners in one lane, so only the sum of squares crosses lanes. A
-// lane holds 8 neighbouring trigonometric entries [8p, 8p + 8); the axis of
-// each is fixed for the whole call and kept as 2 bits in a register. Lanes
-// whose entries lie in one section, and all lanes of a token whose positions
-// agree (text), read one table row with 16-byte loads; the others pick each
-// entry from its axis's row.
+// Bound by memory. Lane layout and loads are those of head_cache_kernel: a head
+// on D/16 lanes, 16-byte accesses, rotation partners in one lane, so only the
+// sum of squares crosses lanes. A unit of work is a run of heads of one token
+// on one warp: positions, slot and table entries are read once for the run (a
+// head's table row is twice the bytes of the head). A lane holds 8 neighbouring
+// trigonometric entries [8p, 8p + 8); the axis of each is fixed for the whole
+// call and kept as 2 bits in a register. Lanes whose entries lie in one section,
+// and all lanes of a token whose positions agree (text), read one table row
+// with 16-byte loads; the others pick each entry from its axis's row (8191
+// tokens, 64/8 heads: 72 us against 71).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -72,7 +74,9 @@ struct MropeArgs {
   bool in_turns;
   bool interleaved;
   float epsilon;
-  HeadDivisor heads_div;
+  uint32_t parts;   // units of a token
+  int part_heads;   // heads of a unit
+  HeadDivisor parts_div;
 };
 
 // Axis whose position turns pair i.
@@ -99,8 +103,10 @@ __device__ __forceinline__ void store_fp8_half(uint8_t* p, const float2* f, floa
   store_fp8_chunk<kVector>(p, make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16)));
 }
 
+// Three blocks to an SM: with four the loads ahead spill (8191 tokens, 64/8
+// heads: 65.5 us against 70.2), with two too few bytes are in flight (90.7).
 template <typename T, int D, int kCache, bool kVector>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) head_mrope_kernel(MropeArgs<T> a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) head_mrope_kernel(MropeArgs<T> a) {
   constexpr int kLanes = D / (2 * kChunkElems);
   constexpr int kHeadsPerWarp = kWarpSize / kLanes;
   const int rotary = a.rotary_dim;
@@ -119,8 +125,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) head_mrope_kernel
   }
   const bool one_axis = axes == (axes & 3u) * 0x5555u;
 
-  const uint32_t heads = static_cast<uint32_t>(a.query_heads + a.key_heads);
-  const uint32_t units = static_cast<uint32_t>(a.tokens) * heads;
+  const int heads = a.query_heads + a.key_heads;
+  const uint32_t units = static_cast<uint32_t>(a.tokens) * a.parts;
   const uint32_t warp = (blockIdx.x * blockDim.x + threadIdx.x) / kWarpSize;
   const uint32_t warps = (gridDim.x * blockDim.x) / kWarpSize;
   wait_for_upstream_grid();
@@ -132,133 +138,137 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) head_mrope_kernel
     v_scale = *a.v_scale;
   }
 
-  for (uint32_t first = warp * kHeadsPerWarp; first < units; first += warps * kHeadsPerWarp) {
-    const uint32_t unit = first + head_in_warp;
-    const bool active = unit < units;
-    const uint32_t token = active ? divide(a.heads_div, unit) : 0;
-    const int h = active ? static_cast<int>(unit - token * heads) : 0;
-    const bool is_query = h < a.query_heads;
-    const int kv_head = h - a.query_heads;
-    const T* head = is_query ? a.query + static_cast<int64_t>(token) * a.query_stride +
-                                   static_cast<int64_t>(h) * D
-                             : a.key + static_cast<int64_t>(token) * a.key_stride +
-                                   static_cast<int64_t>(kv_head) * D;
-    Half8<T> x_a{}, x_b{}, v_a{}, v_b{};
-    int64_t position[kMaxAxes];
-    bool valid = active;
-    bool alike = true;  // all axes stand at one position
+  for (uint32_t unit = warp; unit < units; unit += warps) {
+    const uint32_t token = divide(a.parts_div, unit);
+    const int first_head = static_cast<int>(unit - token * a.parts) * a.part_heads;
+    const int last_head = min(first_head + a.part_heads, heads);
+    // the token's rotation, for all heads of the unit
+    const int64_t* places = a.positions + token;
+    const int64_t place = places[static_cast<int64_t>(axes & 3u) * a.axis_stride];
+    int64_t low = place, high = place;
+    for (int k = 0; k < a.axes; ++k) {
+      const int64_t p = places[k * a.axis_stride];
+      low = min(low, p);
+      high = max(high, p);
+    }
     int64_t slot = -1;
-    if (active) {
-      x_a = load_half<T, kVector>(head + off_a);
-      x_b = load_half<T, kVector>(head + off_b);
-#pragma unroll
-      for (int k = 0; k < kMaxAxes; ++k) {
-        position[k] = k < a.axes ? a.positions[k * a.axis_stride + token] : position[0];
-      }
-#pragma unroll
-      for (int k = 0; k < kMaxAxes; ++k) {
-        valid = valid && position[k] >= 0 && position[k] < a.rope_positions;
-        alike = alike && position[k] == position[0];
-      }
-      if (kCache != kNoCache && !is_query) {
-        slot = a.slots[token];
-        if (slot >= 0 && slot < a.cache_slots) {
-          const T* vh = a.value + static_cast<int64_t>(token) * a.value_stride +
-                        static_cast<int64_t>(kv_head) * D;
-          v_a = load_half<T, kVector>(vh + off_a);
-          v_b = load_half<T, kVector>(vh + off_b);
-        } else {
-          slot = -1;
-        }
-      }
-    }
-    const float2 acc = half_sum_squares<T>(x_b, half_sum_squares<T>(x_a, make_float2(0.f, 0.f)));
-    const float total = group_allreduce_sum<kLanes>(__fadd_rn(acc.x, acc.y));  // before any exit
-    if (!valid) continue;
-    const float inv = head_inverse_rms<D>(make_float2(total, 0.0f), a.epsilon);
-    const T* weight = is_query ? a.query_weight : a.key_weight;
-    float2 n_a[4], n_b[4];
-    {
-      float2 w[4];
-      unpack_pairs<T>(x_a, n_a);
-      unpack_pairs<T>(load_half<T, kVector>(weight + off_a), w);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) n_a[i] = make_float2(n_a[i].x * inv * w[i].x, n_a[i].y * inv * w[i].y);
-      unpack_pairs<T>(x_b, n_b);
-      unpack_pairs<T>(load_half<T, kVector>(weight + off_b), w);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) n_b[i] = make_float2(n_b[i].x * inv * w[i].x, n_b[i].y * inv * w[i].y);
-    }
+    if (kCache != kNoCache && last_head > a.query_heads) slot = a.slots[token];
+    if (low < 0 || high >= a.rope_positions) continue;
+    float2 c[4], s[4];
     if (rotates) {
-      float2 c[4], s[4];
-      if (one_axis || alike) {
-        int64_t p = position[0];
-#pragma unroll
-        for (int k = 1; k < kMaxAxes; ++k) p = (axes & 3u) == k ? position[k] : p;
-        const float* row = a.cos_sin + p * rotary;
+      if (one_axis || low == high) {
+        const float* row = a.cos_sin + place * rotary;
         load8_pairs<kVector>(row + trig, c);
         load8_pairs<kVector>(row + rotary / 2 + trig, s);
       } else {
 #pragma unroll
         for (int i = 0; i < kChunkElems; ++i) {
-          const uint32_t axis = (axes >> (2 * i)) & 3u;
-          int64_t p = position[0];
-#pragma unroll
-          for (int k = 1; k < kMaxAxes; ++k) p = axis == k ? position[k] : p;
+          const int64_t p = places[static_cast<int64_t>((axes >> (2 * i)) & 3u) * a.axis_stride];
           const float* entry = a.cos_sin + p * rotary + trig + i;
           (i & 1 ? c[i / 2].y : c[i / 2].x) = entry[0];
           (i & 1 ? s[i / 2].y : s[i / 2].x) = entry[rotary / 2];
         }
       }
-      if (a.interleaved) {  // (x, y) of a float2 are partners, entries 0-3 in n_a and 4-7 in n_b
+    }
+    const T* query = a.query + static_cast<int64_t>(token) * a.query_stride;
+    const T* key = a.key + static_cast<int64_t>(token) * a.key_stride;
+    int64_t cache_at = 0;
+    if (kCache != kNoCache && slot >= 0 && slot < a.cache_slots) {
+      const uint32_t block = static_cast<uint32_t>(slot) / a.block_size;
+      cache_at = static_cast<int64_t>(block) * a.block_stride +
+                 static_cast<int64_t>(static_cast<uint32_t>(slot) - block * a.block_size) * a.slot_stride;
+    } else {
+      slot = -1;
+    }
+    // kHeadsPerWarp heads at a time, the next ones loaded ahead
+    Half8<T> next_a{}, next_b{};
+    auto load_head = [&](int h) {
+      if (h >= last_head) return;
+      const T* head = h < a.query_heads ? query + static_cast<int64_t>(h) * D
+                                        : key + static_cast<int64_t>(h - a.query_heads) * D;
+      next_a = load_half<T, kVector>(head + off_a);
+      next_b = load_half<T, kVector>(head + off_b);
+    };
+    load_head(first_head + head_in_warp);
+    for (int h0 = first_head; h0 < last_head; h0 += kHeadsPerWarp) {
+      const int h = h0 + head_in_warp;
+      const bool active = h < last_head;
+      const bool is_query = h < a.query_heads;
+      const int kv_head = h - a.query_heads;
+      const Half8<T> x_a = next_a, x_b = next_b;
+      load_head(h + kHeadsPerWarp);
+      Half8<T> v_a{}, v_b{};
+      const bool store = kCache != kNoCache && active && !is_query && slot >= 0;
+      if (store) {
+        const T* vh = a.value + static_cast<int64_t>(token) * a.value_stride +
+                      static_cast<int64_t>(kv_head) * D;
+        v_a = load_half<T, kVector>(vh + off_a);
+        v_b = load_half<T, kVector>(vh + off_b);
+      }
+      const float2 acc = half_sum_squares<T>(x_b, half_sum_squares<T>(x_a, make_float2(0.f, 0.f)));
+      const float total = group_allreduce_sum<kLanes>(__fadd_rn(acc.x, acc.y));  // before any exit
+      if (!active) continue;
+      const float inv = head_inverse_rms<D>(make_float2(total, 0.0f), a.epsilon);
+      const T* weight = is_query ? a.query_weight : a.key_weight;
+      float2 n_a[4], n_b[4];
+      {
+        float2 w[4];
+        unpack_pairs<T>(x_a, n_a);
+        unpack_pairs<T>(load_half<T, kVector>(weight + off_a), w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float ca = i & 1 ? c[i / 2].y : c[i / 2].x;
-          const float sa = i & 1 ? s[i / 2].y : s[i / 2].x;
-          const float cb = i & 1 ? c[2 + i / 2].y : c[2 + i / 2].x;
-          const float sb = i & 1 ? s[2 + i / 2].y : s[2 + i / 2].x;
-          n_a[i] = make_float2(n_a[i].x * ca - n_a[i].y * sa, n_a[i].y * ca + n_a[i].x * sa);
-          n_b[i] = make_float2(n_b[i].x * cb - n_b[i].y * sb, n_b[i].y * cb + n_b[i].x * sb);
-        }
-      } else {
+        for (int i = 0; i < 4; ++i) n_a[i] = make_float2(n_a[i].x * inv * w[i].x, n_a[i].y * inv * w[i].y);
+        unpack_pairs<T>(x_b, n_b);
+        unpack_pairs<T>(load_half<T, kVector>(weight + off_b), w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u = n_a[i], v = n_b[i];
-          n_a[i] = make_float2(u.x * c[i].x - v.x * s[i].x, u.y * c[i].y - v.y * s[i].y);
-          n_b[i] = make_float2(v.x * c[i].x + u.x * s[i].x, v.y * c[i].y + u.y * s[i].y);
+        for (int i = 0; i < 4; ++i) n_b[i] = make_float2(n_b[i].x * inv * w[i].x, n_b[i].y * inv * w[i].y);
+      }
+      if (rotates) {
+        if (a.interleaved) {  // (x, y) of a float2 are partners, entries 0-3 in n_a and 4-7 in n_b
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float ca = i & 1 ? c[i / 2].y : c[i / 2].x;
+            const float sa = i & 1 ? s[i / 2].y : s[i / 2].x;
+            const float cb = i & 1 ? c[2 + i / 2].y : c[2 + i / 2].x;
+            const float sb = i & 1 ? s[2 + i / 2].y : s[2 + i / 2].x;
+            n_a[i] = make_float2(n_a[i].x * ca - n_a[i].y * sa, n_a[i].y * ca + n_a[i].x * sa);
+            n_b[i] = make_float2(n_b[i].x * cb - n_b[i].y * sb, n_b[i].y * cb + n_b[i].x * sb);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 u = n_a[i], v = n_b[i];
+            n_a[i] = make_float2(u.x * c[i].x - v.x * s[i].x, u.y * c[i].y - v.y * s[i].y);
+            n_b[i] = make_float2(v.x * c[i].x + u.x * s[i].x, v.y * c[i].y + u.y * s[i].y);
+          }
         }
       }
-    }
-    T* out = is_query ? a.query_out + static_cast<int64_t>(token) * a.query_out_stride +
-                            static_cast<int64_t>(h) * D
-                      : a.key_out + static_cast<int64_t>(token) * a.key_out_stride +
-                            static_cast<int64_t>(kv_head) * D;
-    const Half8<T> y_a = pack_pairs<T>(n_a);
-    const Half8<T> y_b = pack_pairs<T>(n_b);
-    store_half<T, kVector>(out + off_a, y_a);
-    store_half<T, kVector>(out + off_b, y_b);
-    if (kCache != kNoCache && slot >= 0) {  // query heads keep slot = -1
-      const uint32_t block = static_cast<uint32_t>(slot) / a.block_size;
-      const uint32_t offset = static_cast<uint32_t>(slot) - block * a.block_size;
-      const int64_t base = static_cast<int64_t>(block) * a.block_stride +
-                           static_cast<int64_t>(offset) * a.slot_stride +
-                           static_cast<int64_t>(kv_head) * a.head_stride;
-      if constexpr (kCache == kSameType) {
-        T* kc = static_cast<T*>(a.key_cache) + base;
-        T* vc = static_cast<T*>(a.value_cache) + base;
-        store_half<T, kVector>(kc + off_a, y_a);
-        store_half<T, kVector>(kc + off_b, y_b);
-        store_half<T, kVector>(vc + off_a, v_a);
-        store_half<T, kVector>(vc + off_b, v_b);
-      } else {
-        uint8_t* kc = static_cast<uint8_t*>(a.key_cache) + base;
-        uint8_t* vc = static_cast<uint8_t*>(a.value_cache) + base;
-        store_fp8_half<T, kVector>(kc + off_a, n_a, k_scale);
-        store_fp8_half<T, kVector>(kc + off_b, n_b, k_scale);
-        unpack_pairs<T>(v_a, n_a);
-        unpack_pairs<T>(v_b, n_b);
-        store_fp8_half<T, kVector>(vc + off_a, n_a, v_scale);
-        store_fp8_half<T, kVector>(vc + off_b, n_b, v_scale);
+      T* out = is_query ? a.query_out + static_cast<int64_t>(token) * a.query_out_stride +
+                              static_cast<int64_t>(h) * D
+                        : a.key_out + static_cast<int64_t>(token) * a.key_out_stride +
+                              static_cast<int64_t>(kv_head) * D;
+      const Half8<T> y_a = pack_pairs<T>(n_a);
+      const Half8<T> y_b = pack_pairs<T>(n_b);
+      store_half<T, kVector>(out + off_a, y_a);
+      store_half<T, kVector>(out + off_b, y_b);
+      if (store) {
+        const int64_t base = cache_at + static_cast<int64_t>(kv_head) * a.head_stride;
+        if constexpr (kCache == kSameType) {
+          T* kc = static_cast<T*>(a.key_cache) + base;
+          T* vc = static_cast<T*>(a.value_cache) + base;
+          store_half<T, kVector>(kc + off_a, y_a);
+          store_half<T, kVector>(kc + off_b, y_b);
+          store_half<T, kVector>(vc + off_a, v_a);
+          store_half<T, kVector>(vc + off_b, v_b);
+        } else {
+          uint8_t* kc = static_cast<uint8_t*>(a.key_cache) + base;
+          uint8_t* vc = static_cast<uint8_t*>(a.value_cache) + base;
+          store_fp8_half<T, kVector>(kc + off_a, n_a, k_scale);
+          store_fp8_half<T, kVector>(kc + off_b, n_b, k_scale);
+          unpack_pairs<T>(v_a, n_a);
+          unpack_pairs<T>(v_b, n_b);
+          store_fp8_half<T, kVector>(vc + off_a, n_a, v_scale);
+          store_fp8_half<T, kVector>(vc + off_b, n_b, v_scale);
+        }
       }
     }
   }
@@ -288,9 +298,28 @@ int run_mrope(MropeArgs<T> a, cudaStream_t stream) {
   int rc = current_device_info(&dev);
   if (rc != SM120N_OK) return rc;
   const int64_t heads = a.query_heads + a.key_heads;
-  a.heads_div = make_head_divisor(static_cast<uint32_t>(heads));
-  // tokens * heads < 2^31 per launch (32-bit unit indices)
-  const int64_t max_tokens = ((int64_t{1} << 31) - 1) / heads;
+  const int threads = 256;
+  int resident = 1;
+  rc = max_resident_ctas(reinterpret_cast<const void*>(kernel), threads, 0, &resident);
+  if (rc != SM120N_OK) return rc;
+  const int64_t most_warps = int64_t{dev.sm_count} * resident * (threads / kWarpSize);
+  // Units of `per` groups of heads: the warps run over them in rounds, and a
+  // unit's start (positions, table entries) costs about as much as 1.5 groups.
+  // The fewest parts of a token with the least of rounds x (per + 1.5).
+  const int64_t groups = (heads + kHeadsPerWarp - 1) / kHeadsPerWarp;
+  int64_t least = INT64_MAX;
+  for (int64_t parts = 1; parts <= std::min<int64_t>(groups, 64); ++parts) {
+    const int64_t per = (groups + parts - 1) / parts;
+    const int64_t rounds = (a.tokens * parts + most_warps - 1) / most_warps;
+    if (rounds * (2 * per + 3) < least) {
+      least = rounds * (2 * per + 3);
+      a.parts = static_cast<uint32_t>((groups + per - 1) / per);
+      a.part_heads = static_cast<int>(per * kHeadsPerWarp);
+    }
+  }
+  a.parts_div = make_head_divisor(a.parts);
+  // tokens * parts < 2^31 per launch (32-bit unit indices)
+  const int64_t max_tokens = ((int64_t{1} << 31) - 1) / a.parts;
   const int64_t all_tokens = a.tokens;
   for (int64_t done = 0; done < all_tokens; done += max_tokens) {
     MropeArgs<T> c = a;
@@ -304,16 +333,14 @@ int run_mrope(MropeArgs<T> a, cudaStream_t stream) {
       c.value = a.value + done * a.value_stride;
       c.slots = a.slots + done;
     }
-    const int64_t warps_needed = (c.tokens * heads + kHeadsPerWarp - 1) / kHeadsPerWarp;
-    const int64_t threads = std::min<int64_t>(256, warps_needed * kWarpSize);
-    int resident = 1;
-    rc = max_resident_ctas(reinterpret_cast<const void*>(kernel), static_cast<int>(threads), 0,
-                           &resident);
-    if (rc != SM120N_OK) return rc;
-    const int64_t blocks = std::min<int64_t>((warps_needed * kWarpSize + threads - 1) / threads,
-                                             static_cast<int64_t>(dev.sm_count) * resident);
-    rc = launch(kernel, dim3(static_cast<unsigned>(std::max<int64_t>(blocks, 1))),
-                dim3(static_cast<unsigned>(threads)), 0, stream, c);
+    // few units: small blocks, so that they spread over the SMs
+    const int64_t warps_needed = c.tokens * a.parts;
+    const int64_t block_warps = std::max<int64_t>(
+        1, std::min<int64_t>(threads / kWarpSize, warps_needed / dev.sm_count));
+    const int64_t blocks = std::min<int64_t>((warps_needed + block_warps - 1) / block_warps,
+                                             most_warps / block_warps);
+    rc = launch(kernel, dim3(static_cast<unsigned>(blocks)),
+                dim3(static_cast<unsigned>(block_warps * kWarpSize)), 0, stream, c);
     if (rc != SM120N_OK) return rc;
   }
   return SM120N_OK;

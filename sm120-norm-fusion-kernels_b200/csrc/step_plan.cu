@@ -111,7 +111,7 @@ struct PlanRow {
   int32_t served;
 };
 
-template <int kBlocks>
+template <int kBlocks, int kPer>
 __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     plan_step_kernel(PlanArgs a) {
   __shared__ PlanRow rows[kPlanThreads];
@@ -126,6 +126,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
   wait_for_upstream_grid();
   release_downstream_grid();
   const int count = min(max(*a.free_count, 0), a.pool);
+  const uint32_t block_size = static_cast<uint32_t>(a.block_size);
   int64_t carry_tokens = 0, carry_need = 0;
   if (rank == 0 && tid == 0) a.query_start[0] = 0;
 
@@ -134,8 +135,11 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     const bool live = r < a.requests;
     const int64_t c = live ? max(a.context[r], 0) : 0;
     const int64_t q = live ? max(a.query[r], 0) : 0;
-    const int64_t held = (c + a.block_size - 1) / a.block_size;
-    const int64_t want = (c + q + a.block_size - 1) / a.block_size;
+    const uint32_t c_blocks = static_cast<uint32_t>(c) / block_size;
+    const int64_t held = c_blocks + (static_cast<uint32_t>(c) - c_blocks * block_size != 0);
+    const uint32_t both = static_cast<uint32_t>(c + q);  // below 2^32
+    const uint32_t both_blocks = both / block_size;
+    const int64_t want = int64_t{both_blocks} + (both - both_blocks * block_size != 0);
     bool served = live && want <= a.width && c + q <= INT32_MAX;
     const int64_t need = served ? want - held : 0;
     int64_t end = q, upto = need;
@@ -185,15 +189,14 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
       for (int j = lane; j < n; j += kWarpSize) entry[j] = a.free_blocks[pop - j];
     }
 
-    // Tokens of the chunk, four neighbours to a thread: one search for the
-    // first of them, one block id for each block they touch.
+    // Tokens of the chunk, kPer neighbours to a thread: one search for the first
+    // of them, one block id for each block they touch.
     const int64_t last_token = min(carry_tokens, a.tokens);
     const int in_chunk = min(threads, a.requests - base);
-    const int64_t group0 = first_token / 4;
-    for (int64_t g = group0 + static_cast<int64_t>(rank) * threads + tid; 4 * g < last_token;
-         g += static_cast<int64_t>(kBlocks) * threads) {
-      const int64_t from = max(4 * g, first_token);
-      const int64_t to = min(4 * g + 4, last_token);
+    for (int64_t g = first_token / kPer + static_cast<int64_t>(rank) * threads + tid;
+         kPer * g < last_token; g += static_cast<int64_t>(kBlocks) * threads) {
+      const int64_t from = max(kPer * g, first_token);
+      const int64_t to = min(kPer * g + kPer, last_token);
       int low = 0, high = in_chunk;  // the first row whose end is behind `from`
       while (low < high) {
         const int middle = (low + high) / 2;
@@ -201,40 +204,40 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
       }
       int i = low;
       int64_t begin = i == 0 ? first_token : rows[i - 1].end;
-      int known_row = -1, known_block = -1, id = -1;
-      int64_t p[4];
-      int32_t s[4];
+      int known_row = -1, id = -1;
+      uint32_t known_block = 0;
+      int64_t p[kPer];
+      int32_t s[kPer];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t t = 4 * g + j;
+      for (int j = 0; j < kPer; ++j) {
+        const int64_t t = kPer * g + j;
         if (t < from || t >= to) continue;
         while (rows[i].end <= t) begin = rows[i++].end;
-        const int64_t position = rows[i].first + (t - begin);
-        const int block = static_cast<int>(position / a.block_size);
+        p[j] = rows[i].first + (t - begin);
+        s[j] = -1;
+        if (!rows[i].served) continue;
+        const uint32_t position = static_cast<uint32_t>(p[j]);  // below 2^31 for a served request
+        const uint32_t block = position / block_size;
         if (i != known_row || block != known_block) {
           known_row = i;
           known_block = block;
-          id = -1;
-          if (rows[i].served) {
-            id = block < rows[i].held
-                     ? a.table[static_cast<int64_t>(base + i) * a.table_stride + block]
-                     : a.free_blocks[rows[i].pop - (block - rows[i].held)];
-          }
+          const int fresh = static_cast<int>(block) - rows[i].held;
+          id = fresh < 0 ? a.table[static_cast<int64_t>(base + i) * a.table_stride + block]
+                         : a.free_blocks[rows[i].pop - fresh];
         }
-        p[j] = position;
-        s[j] = id < 0 || id >= a.pool
-                   ? -1
-                   : id * a.block_size + static_cast<int>(position - static_cast<int64_t>(block) * a.block_size);
+        if (id >= 0 && id < a.pool) {
+          s[j] = static_cast<int32_t>(id * block_size + (position - block * block_size));
+        }
       }
-      if (from == 4 * g && to == from + 4 &&
+      if (kPer == 4 && from == kPer * g && to == from + kPer &&
           ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots)) & 15) == 0) {
-        *reinterpret_cast<longlong2*>(a.positions + from) = make_longlong2(p[0], p[1]);
-        *reinterpret_cast<longlong2*>(a.positions + from + 2) = make_longlong2(p[2], p[3]);
-        *reinterpret_cast<int4*>(a.slots + from) = make_int4(s[0], s[1], s[2], s[3]);
+        *reinterpret_cast<longlong2*>(a.positions + from) = make_longlong2(p[0], p[1 % kPer]);
+        *reinterpret_cast<longlong2*>(a.positions + from + 2) = make_longlong2(p[kPer / 2], p[kPer - 1]);
+        *reinterpret_cast<int4*>(a.slots + from) = make_int4(s[0], s[1 % kPer], s[kPer / 2], s[kPer - 1]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t t = 4 * g + j;
+        for (int j = 0; j < kPer; ++j) {
+          const int64_t t = kPer * g + j;
           if (t < from || t >= to) continue;
           a.positions[t] = p[j];
           a.slots[t] = s[j];
@@ -267,19 +270,23 @@ struct ReleaseArgs {
 };
 
 constexpr int kReleaseRows = 128;  // of a block in one round
+constexpr int kRowsOfWarp = kReleaseRows / (kPlanThreads / kWarpSize);
+constexpr int kAhead = 4;  // groups of 32 entries of each row in flight
 
 // Rounds of kReleaseRows rows to a block, the blocks' rows in order. A warp
-// counts the ids of a row that go back; sums over the block's rows and over
-// the blocks before it give every row its place; the warp then writes them.
+// counts the ids of its rows that go back; sums over the block's rows and over
+// the blocks before it give every row its place; the warp then writes them. A
+// warp's rows are read side by side, several groups of entries ahead: one row
+// after the other the loads' latencies add up (19 us against 8 for 1000 rows).
 template <int kBlocks>
 __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     release_blocks_kernel(ReleaseArgs a) {
+  __shared__ int ends[kReleaseRows];   // entries of a row that may go back: up to here
   __shared__ int place[kReleaseRows];  // counts, then exclusive sums
   __shared__ int block_total[2];       // by the parity of the round
   const int tid = threadIdx.x;
   const int lane = tid & (kWarpSize - 1);
   const int warp = tid / kWarpSize;
-  const int warps = blockDim.x / kWarpSize;
   const int rank = block_rank<kBlocks>();
   wait_for_upstream_grid();
   release_downstream_grid();
@@ -288,23 +295,50 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
   int round = 0;
   for (int base = 0; base < a.requests; base += kBlocks * kReleaseRows, round ^= 1) {
     const int first = base + rank * kReleaseRows;
-    auto blocks_of = [&](int r) {
-      if (r >= a.requests || !a.finished[r]) return 0;
-      const int64_t n = (static_cast<int64_t>(max(a.seq_lens[r], 0)) + a.block_size - 1) / a.block_size;
-      return static_cast<int>(min(n, static_cast<int64_t>(a.width)));
+    if (tid < kReleaseRows) {
+      const int r = first + tid;
+      uint32_t n = 0;
+      if (r < a.requests && a.finished[r]) {
+        const uint32_t tokens = static_cast<uint32_t>(max(a.seq_lens[r], 0));
+        n = tokens / static_cast<uint32_t>(a.block_size);
+        n += tokens - n * static_cast<uint32_t>(a.block_size) != 0;
+      }
+      ends[tid] = static_cast<int>(min(n, static_cast<uint32_t>(a.width)));
+    }
+    __syncthreads();
+    // f(row of the warp, entry there and in the pool, id) for the warp's rows
+    // side by side, in the order of the entries for each
+    auto over_entries = [&](auto f) {
+      int most = 0;
+#pragma unroll
+      for (int i = 0; i < kRowsOfWarp; ++i) most = max(most, ends[warp * kRowsOfWarp + i]);
+      for (int j0 = a.shared_blocks; j0 < most; j0 += kAhead * kWarpSize) {
+        int id[kRowsOfWarp][kAhead];
+#pragma unroll
+        for (int i = 0; i < kRowsOfWarp; ++i) {
+          const int n = ends[warp * kRowsOfWarp + i];
+          const int32_t* ids = a.table + static_cast<int64_t>(first + warp * kRowsOfWarp + i) * a.table_stride;
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int j = j0 + k * kWarpSize + lane;
+            id[i][k] = j < n ? ids[j] : -1;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kRowsOfWarp; ++i) {
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            f(i, static_cast<uint32_t>(id[i][k]) < static_cast<uint32_t>(a.pool), id[i][k]);
+          }
+        }
+      }
     };
-    auto returned = [&](const int32_t* ids, int j, int n) {
-      return j < n && static_cast<uint32_t>(ids[j]) < static_cast<uint32_t>(a.pool);
-    };
-    for (int i = warp; i < kReleaseRows; i += warps) {
-      const int r = first + i;
-      const int n = blocks_of(r);
-      int found = 0;
-      const int32_t* ids = a.table + static_cast<int64_t>(r) * a.table_stride;
-#pragma unroll 4
-      for (int j = a.shared_blocks + lane; j < n; j += kWarpSize) found += returned(ids, j, n);
-      found = __reduce_add_sync(kFullMask, found);
-      if (lane == 0) place[i] = found;
+    int found[kRowsOfWarp] = {};
+    over_entries([&](int i, bool back, int) { found[i] += back; });
+#pragma unroll
+    for (int i = 0; i < kRowsOfWarp; ++i) {
+      const int all = __reduce_add_sync(kFullMask, found[i]);
+      if (lane == 0) place[warp * kRowsOfWarp + i] = all;
     }
     __syncthreads();
     if (warp == 0) {
@@ -338,20 +372,16 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
       if (k < rank) before += total;
       carry += total;
     }
-    for (int i = warp; i < kReleaseRows; i += warps) {
-      const int r = first + i;
-      const int n = blocks_of(r);
-      const int32_t* ids = a.table + static_cast<int64_t>(r) * a.table_stride;
-      int64_t at = before + place[i];
-      for (int j = a.shared_blocks; j < n; j += kWarpSize) {
-        const bool back = returned(ids, j + lane, n);
-        const unsigned set = __ballot_sync(kFullMask, back);
-        const int64_t mine = at + __popc(set & ((1u << lane) - 1));
-        if (back && mine < a.pool) a.free_blocks[mine] = ids[j + lane];
-        at += __popc(set);
-      }
-    }
-    __syncthreads();  // the next round's counts follow these reads of place
+    int64_t at[kRowsOfWarp];
+#pragma unroll
+    for (int i = 0; i < kRowsOfWarp; ++i) at[i] = before + place[warp * kRowsOfWarp + i];
+    over_entries([&](int i, bool back, int id) {
+      const unsigned set = __ballot_sync(kFullMask, back);
+      const int64_t mine = at[i] + __popc(set & ((1u << lane) - 1));
+      if (back && mine < a.pool) a.free_blocks[mine] = id;
+      at[i] += __popc(set);
+    });
+    __syncthreads();  // the next round's lengths and counts follow these reads
   }
   // no block leaves while another may still read its total
   step_barrier<kBlocks>();
@@ -414,12 +444,16 @@ extern "C" int sm120s_plan_step(const int32_t* context_lens, const int32_t* quer
                    static_cast<int>(requests), static_cast<int>(table_width),
                    static_cast<int>(pool), static_cast<int>(block_size)};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // One block has four tokens to a thread up to 4096 of them; more go to a cluster.
-  if (tokens <= 4 * kPlanThreads) {
-    return launch(plan_step_kernel<1>, dim3(1),
-                  dim3(plan_threads(std::max(requests, (tokens + 3) / 4))), 0, s, a);
+  // A token to a thread of one block, then four, then four to a thread of a
+  // cluster: 1024 decodes 4.6 us with one token to a thread, 5.6 with four.
+  if (tokens <= kPlanThreads) {
+    return launch(plan_step_kernel<1, 1>, dim3(1), dim3(plan_threads(std::max(requests, tokens))), 0,
+                  s, a);
   }
-  return launch(plan_step_kernel<kPlanCluster>, dim3(kPlanCluster), dim3(kPlanThreads), 0, s, a);
+  if (tokens <= 4 * kPlanThreads) {
+    return launch(plan_step_kernel<1, 4>, dim3(1), dim3(kPlanThreads), 0, s, a);
+  }
+  return launch(plan_step_kernel<kPlanCluster, 4>, dim3(kPlanCluster), dim3(kPlanThreads), 0, s, a);
 }
 
 extern "C" int sm120s_release_blocks(const int32_t* seq_lens, const uint8_t* finished,
@@ -443,8 +477,7 @@ extern "C" int sm120s_release_blocks(const int32_t* seq_lens, const uint8_t* fin
                       static_cast<int>(pool), static_cast<int>(block_size),
                       static_cast<int>(std::min(shared_blocks, table_width))};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // A block counts 32 rows at a time; from there the rows go round a cluster.
-  if (requests <= kPlanThreads / kWarpSize) {
+  if (requests <= kReleaseRows) {
     return launch(release_blocks_kernel<1>, dim3(1), dim3(kPlanThreads), 0, s, a);
   }
   return launch(release_blocks_kernel<kPlanCluster>, dim3(kPlanCluster), dim3(kPlanThreads), 0, s, a);
