@@ -57,17 +57,23 @@ struct PlanArgs {
   int block_size;
 };
 
-// Inclusive sums of two values over the block, for up to 32 full warps.
-__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t (*warp_sums)[2]) {
+// Sums here never fall and matter only up to 2^31 - 2 (tokens, blocks of the
+// pool), so they stop at kCap: 32 bits hold them, whatever the lengths are.
+constexpr uint32_t kCap = 0x7fffffffu;
+__device__ __forceinline__ uint32_t capped(uint32_t a, uint32_t b) { return min(a + b, kCap); }
+
+// Inclusive capped sums of two values over the block, for up to 32 full warps.
+__device__ __forceinline__ void block_scan2(uint32_t& a, uint32_t& b, uint32_t (*warp_sums)[2]) {
   const int lane = threadIdx.x & (kWarpSize - 1);
   const int warp = threadIdx.x / kWarpSize;
+  const int warps = blockDim.x / kWarpSize;
 #pragma unroll
   for (int d = 1; d < kWarpSize; d *= 2) {
-    const int64_t x = __shfl_up_sync(kFullMask, a, d);
-    const int64_t y = __shfl_up_sync(kFullMask, b, d);
+    const uint32_t x = __shfl_up_sync(kFullMask, a, d);
+    const uint32_t y = __shfl_up_sync(kFullMask, b, d);
     if (lane >= d) {
-      a += x;
-      b += y;
+      a = capped(a, x);
+      b = capped(b, y);
     }
   }
   if (lane == kWarpSize - 1) {
@@ -75,17 +81,16 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t (*wa
     warp_sums[warp][1] = b;
   }
   __syncthreads();
-  const int warps = blockDim.x / kWarpSize;
   // every warp sums the totals of the warps before it
-  int64_t x = lane < warps && lane < warp ? warp_sums[lane][0] : 0;
-  int64_t y = lane < warps && lane < warp ? warp_sums[lane][1] : 0;
+  uint32_t x = lane < warps && lane < warp ? warp_sums[lane][0] : 0;
+  uint32_t y = lane < warps && lane < warp ? warp_sums[lane][1] : 0;
 #pragma unroll
   for (int d = kWarpSize / 2; d > 0; d /= 2) {
-    x += __shfl_xor_sync(kFullMask, x, d);
-    y += __shfl_xor_sync(kFullMask, y, d);
+    x = capped(x, __shfl_xor_sync(kFullMask, x, d));
+    y = capped(y, __shfl_xor_sync(kFullMask, y, d));
   }
-  a += x;
-  b += y;
+  a = capped(a, x);
+  b = capped(b, y);
 }
 
 template <int kBlocks>
@@ -102,22 +107,33 @@ __device__ __forceinline__ int block_rank() {
   return kBlocks > 1 ? static_cast<int>(blockIdx.x) : 0;  // the grid is one cluster
 }
 
-// A row of the chunk in work, as the tokens need it.
-struct PlanRow {
-  int64_t end;   // of its tokens
-  int32_t first;  // position of its first token
-  int32_t held;
-  int32_t pop;  // index into free_blocks of its first new block; blocks go down from there
-  int32_t served;
+// Division by the block size: a shift where it is a power of two.
+struct BlockSize {
+  uint32_t size;
+  int shift;  // -1: none
+  static __device__ __forceinline__ BlockSize of(int n) {
+    return BlockSize{static_cast<uint32_t>(n), (n & (n - 1)) == 0 ? __ffs(n) - 1 : -1};
+  }
+  __device__ __forceinline__ uint32_t blocks(uint32_t tokens) const {  // whole ones
+    return shift >= 0 ? tokens >> shift : tokens / size;
+  }
+  __device__ __forceinline__ uint32_t ceil(uint32_t tokens) const {
+    const uint32_t whole = blocks(tokens);
+    return whole + (tokens != whole * size);
+  }
 };
 
 template <int kBlocks, int kPer>
 __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     plan_step_kernel(PlanArgs a) {
-  __shared__ PlanRow rows[kPlanThreads];
-  __shared__ int64_t warp_sums[kPlanThreads / kWarpSize][2];
-  __shared__ int64_t chunk_sums[2];
-  __shared__ int popped;
+  // the rows of the chunk in work
+  __shared__ uint32_t ends[kPlanThreads];   // of their tokens
+  __shared__ uint32_t uptos[kPlanThreads];  // new blocks up to and with the row
+  __shared__ uint32_t firsts[kPlanThreads];  // position of the first token
+  __shared__ int32_t helds[kPlanThreads];   // blocks before the step, -1: not served
+  __shared__ uint32_t warp_sums[kPlanThreads / kWarpSize][2];
+  __shared__ uint32_t chunk_sums[2];
+  __shared__ uint32_t popped;
   const int threads = blockDim.x;
   const int tid = threadIdx.x;
   const int lane = tid & (kWarpSize - 1);
@@ -125,111 +141,110 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
   if (tid == 0) popped = 0;
   wait_for_upstream_grid();
   release_downstream_grid();
-  const int count = min(max(*a.free_count, 0), a.pool);
-  const uint32_t block_size = static_cast<uint32_t>(a.block_size);
-  int64_t carry_tokens = 0, carry_need = 0;
+  const uint32_t count = static_cast<uint32_t>(min(max(*a.free_count, 0), a.pool));
+  const BlockSize block_size = BlockSize::of(a.block_size);
+  const uint32_t tokens = static_cast<uint32_t>(a.tokens);
+  uint32_t carry_tokens = 0, carry_need = 0;
   if (rank == 0 && tid == 0) a.query_start[0] = 0;
+
+  // the first row of the chunk whose running sum is above `index`
+  auto find = [](const uint32_t* sums, int n, uint32_t index) {
+    int low = 0, high = n;
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (sums[middle] > index) high = middle; else low = middle + 1;
+    }
+    return low;
+  };
 
   for (int base = 0; base < a.requests; base += threads) {
     const int r = base + tid;
     const bool live = r < a.requests;
-    const int64_t c = live ? max(a.context[r], 0) : 0;
-    const int64_t q = live ? max(a.query[r], 0) : 0;
-    const uint32_t c_blocks = static_cast<uint32_t>(c) / block_size;
-    const int64_t held = c_blocks + (static_cast<uint32_t>(c) - c_blocks * block_size != 0);
-    const uint32_t both = static_cast<uint32_t>(c + q);  // below 2^32
-    const uint32_t both_blocks = both / block_size;
-    const int64_t want = int64_t{both_blocks} + (both - both_blocks * block_size != 0);
-    bool served = live && want <= a.width && c + q <= INT32_MAX;
-    const int64_t need = served ? want - held : 0;
-    int64_t end = q, upto = need;
+    const uint32_t c = live ? static_cast<uint32_t>(max(a.context[r], 0)) : 0;
+    const uint32_t q = live ? static_cast<uint32_t>(max(a.query[r], 0)) : 0;
+    const uint32_t held = block_size.ceil(c);
+    const uint32_t want = block_size.ceil(c + q);
+    bool served = live && want <= static_cast<uint32_t>(a.width) && c + q <= kCap;
+    const uint32_t need = served ? want - held : 0;
+    uint32_t end = min(q, kCap), upto = need;
     __syncthreads();  // the chunk before is done with the shared arrays
     block_scan2(end, upto, warp_sums);
     if (tid == threads - 1) {
       chunk_sums[0] = end;
       chunk_sums[1] = upto;
     }
-    end += carry_tokens;
-    upto += carry_need;
+    end = capped(end, carry_tokens);
+    upto = capped(upto, carry_need);
     // Requests past the end of the token buffer are the last ones, so leaving
     // them in the sums of need changes nothing for those before them.
-    served = served && end <= a.tokens && (need == 0 || upto <= count);
-    PlanRow row;
-    row.end = end;
-    row.first = static_cast<int32_t>(c);
-    row.held = static_cast<int32_t>(held);
-    row.pop = static_cast<int32_t>(count - 1 - (upto - need));  // not read unless served
-    row.served = served;
-    rows[tid] = row;
-    const int top = __reduce_max_sync(kFullMask, served && need > 0 ? static_cast<int>(upto) : 0);
+    served = served && end <= tokens && (need == 0 || upto <= count);
+    ends[tid] = end;
+    uptos[tid] = upto;
+    firsts[tid] = c;
+    helds[tid] = served ? static_cast<int32_t>(held) : -1;
+    const uint32_t top = __reduce_max_sync(kFullMask, served && need > 0 ? upto : 0);
     if (lane == 0 && top > 0) atomicMax(&popped, top);
     step_barrier<kBlocks>();  // every block has read this chunk and free_count
-    const int64_t first_token = carry_tokens;
-    carry_tokens += chunk_sums[0];
-    carry_need += chunk_sums[1];
+    const uint32_t first_token = carry_tokens, first_need = carry_need;
+    carry_tokens = capped(carry_tokens, chunk_sums[0]);
+    carry_need = capped(carry_need, chunk_sums[1]);
     if (rank == 0 && live) {
-      a.query_start[r + 1] = static_cast<int32_t>(min(end, a.tokens));
+      a.query_start[r + 1] = static_cast<int32_t>(min(end, tokens));
       a.seq_lens[r] = static_cast<int32_t>(served ? c + q : c);
     }
+    const int in_chunk = min(threads, a.requests - base);
 
-    // New table entries: the rows of a warp go round the blocks; few entries
-    // are written by the row's own thread, many by the whole warp.
-    const int mine = served && r % kBlocks == rank ? static_cast<int>(need) : 0;
-    if (mine > 0 && mine <= 2) {
-      for (int j = 0; j < mine; ++j) {
-        a.table[r * a.table_stride + row.held + j] = a.free_blocks[row.pop - j];
-      }
-    }
-    for (unsigned many = __ballot_sync(kFullMask, mine > 2); many; many &= many - 1) {
-      const int source = __ffs(many) - 1;
-      const int n = __shfl_sync(kFullMask, mine, source);
-      const int pop = __shfl_sync(kFullMask, row.pop, source);
-      const int at = __shfl_sync(kFullMask, row.held, source);
-      int32_t* entry = a.table + static_cast<int64_t>(r - lane + source) * a.table_stride + at;
-      for (int j = lane; j < n; j += kWarpSize) entry[j] = a.free_blocks[pop - j];
+    // New table entries: the e-th block taken is the e-th from the top, whoever
+    // takes it; those taken end at `popped`.
+    const uint32_t last_need = min(carry_need, popped);
+    for (uint32_t e = first_need + static_cast<uint32_t>(rank * threads + tid); e < last_need;
+         e += static_cast<uint32_t>(kBlocks * threads)) {
+      const int i = find(uptos, in_chunk, e);
+      const uint32_t before = i == 0 ? first_need : uptos[i - 1];
+      a.table[static_cast<int64_t>(base + i) * a.table_stride + helds[i] + (e - before)] =
+          a.free_blocks[count - 1 - e];
     }
 
     // Tokens of the chunk, kPer neighbours to a thread: one search for the first
     // of them, one block id for each block they touch.
-    const int64_t last_token = min(carry_tokens, a.tokens);
-    const int in_chunk = min(threads, a.requests - base);
-    for (int64_t g = first_token / kPer + static_cast<int64_t>(rank) * threads + tid;
-         kPer * g < last_token; g += static_cast<int64_t>(kBlocks) * threads) {
-      const int64_t from = max(kPer * g, first_token);
-      const int64_t to = min(kPer * g + kPer, last_token);
-      int low = 0, high = in_chunk;  // the first row whose end is behind `from`
-      while (low < high) {
-        const int middle = (low + high) / 2;
-        if (rows[middle].end > from) high = middle; else low = middle + 1;
-      }
-      int i = low;
-      int64_t begin = i == 0 ? first_token : rows[i - 1].end;
+    const uint32_t last_token = min(carry_tokens, tokens);
+    for (uint32_t g = first_token / kPer + static_cast<uint32_t>(rank * threads + tid);
+         kPer * g < last_token; g += static_cast<uint32_t>(kBlocks * threads)) {
+      const uint32_t from = max(kPer * g, first_token);
+      const uint32_t to = min(kPer * g + kPer, last_token);
+      int i = find(ends, in_chunk, from);
+      uint32_t begin = i == 0 ? first_token : ends[i - 1];
+      uint32_t taken = i == 0 ? first_need : uptos[i - 1];  // blocks before the row's new ones
       int known_row = -1, id = -1;
       uint32_t known_block = 0;
       int64_t p[kPer];
       int32_t s[kPer];
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const int64_t t = kPer * g + j;
+        const uint32_t t = kPer * g + j;
         if (t < from || t >= to) continue;
-        while (rows[i].end <= t) begin = rows[i++].end;
-        p[j] = rows[i].first + (t - begin);
+        while (ends[i] <= t) {
+          begin = ends[i];
+          taken = uptos[i++];
+        }
+        const uint32_t position = firsts[i] + (t - begin);  // below 2^32
+        p[j] = position;
         s[j] = -1;
-        if (!rows[i].served) continue;
-        const uint32_t position = static_cast<uint32_t>(p[j]);  // below 2^31 for a served request
-        const uint32_t block = position / block_size;
+        const int held_blocks = helds[i];
+        if (held_blocks < 0) continue;
+        const uint32_t block = block_size.blocks(position);
         if (i != known_row || block != known_block) {
           known_row = i;
           known_block = block;
-          const int fresh = static_cast<int>(block) - rows[i].held;
+          const int fresh = static_cast<int>(block) - held_blocks;
           id = fresh < 0 ? a.table[static_cast<int64_t>(base + i) * a.table_stride + block]
-                         : a.free_blocks[rows[i].pop - fresh];
+                         : a.free_blocks[count - 1 - (taken + fresh)];
         }
         if (id >= 0 && id < a.pool) {
-          s[j] = static_cast<int32_t>(id * block_size + (position - block * block_size));
+          s[j] = static_cast<int32_t>(id * block_size.size + (position - block * block_size.size));
         }
       }
-      if (kPer == 4 && from == kPer * g && to == from + kPer &&
+      if (kPer == 4 && to == from + kPer &&
           ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots)) & 15) == 0) {
         *reinterpret_cast<longlong2*>(a.positions + from) = make_longlong2(p[0], p[1 % kPer]);
         *reinterpret_cast<longlong2*>(a.positions + from + 2) = make_longlong2(p[kPer / 2], p[kPer - 1]);
@@ -237,7 +252,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
       } else {
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-          const int64_t t = kPer * g + j;
+          const uint32_t t = kPer * g + j;
           if (t < from || t >= to) continue;
           a.positions[t] = p[j];
           a.slots[t] = s[j];
@@ -246,8 +261,8 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     }
   }
   if (a.requests == 0) step_barrier<kBlocks>();
-  if (rank == 0 && tid == 0) *a.free_count_out = count - popped;
-  for (int64_t t = carry_tokens + static_cast<int64_t>(rank) * threads + tid; t < a.tokens;
+  if (rank == 0 && tid == 0) *a.free_count_out = static_cast<int32_t>(count - popped);
+  for (int64_t t = int64_t{carry_tokens} + static_cast<int64_t>(rank) * threads + tid; t < a.tokens;
        t += static_cast<int64_t>(kBlocks) * threads) {
     a.positions[t] = -1;
     a.slots[t] = -1;
@@ -270,24 +285,26 @@ struct ReleaseArgs {
 };
 
 constexpr int kReleaseRows = 128;  // of a block in one round
-constexpr int kRowsOfWarp = kReleaseRows / (kPlanThreads / kWarpSize);
-constexpr int kAhead = 4;  // groups of 32 entries of each row in flight
+constexpr int kAhead = 8;          // groups of 32 entries of a row in flight
 
-// Rounds of kReleaseRows rows to a block, the blocks' rows in order. A warp
-// counts the ids of its rows that go back; sums over the block's rows and over
-// the blocks before it give every row its place; the warp then writes them. A
-// warp's rows are read side by side, several groups of entries ahead: one row
-// after the other the loads' latencies add up (19 us against 8 for 1000 rows).
+// Rounds of kReleaseRows rows to a block, the blocks' rows in order. The rows
+// that give something back are listed; a warp counts the ids of a row that go
+// back; sums over the list and over the blocks before it give every row its
+// place; the warp then writes them.
 template <int kBlocks>
 __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     release_blocks_kernel(ReleaseArgs a) {
-  __shared__ int ends[kReleaseRows];   // entries of a row that may go back: up to here
-  __shared__ int place[kReleaseRows];  // counts, then exclusive sums
-  __shared__ int block_total[2];       // by the parity of the round
+  __shared__ int listed[kReleaseRows];  // rows of the block, in order
+  __shared__ int ends[kReleaseRows];    // entries of a listed row that may go back: up to here
+  __shared__ int place[kReleaseRows];   // counts, then exclusive sums
+  __shared__ int warp_rows[kReleaseRows / kWarpSize];
+  __shared__ int block_total[2];  // by the parity of the round
   const int tid = threadIdx.x;
   const int lane = tid & (kWarpSize - 1);
   const int warp = tid / kWarpSize;
+  const int warps = blockDim.x / kWarpSize;
   const int rank = block_rank<kBlocks>();
+  const BlockSize block_size = BlockSize::of(a.block_size);
   wait_for_upstream_grid();
   release_downstream_grid();
   const int64_t count = min(max(*a.free_count, 0), a.pool);
@@ -295,50 +312,60 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
   int round = 0;
   for (int base = 0; base < a.requests; base += kBlocks * kReleaseRows, round ^= 1) {
     const int first = base + rank * kReleaseRows;
+    int n = 0;
     if (tid < kReleaseRows) {
       const int r = first + tid;
-      uint32_t n = 0;
-      if (r < a.requests && a.finished[r]) {
-        const uint32_t tokens = static_cast<uint32_t>(max(a.seq_lens[r], 0));
-        n = tokens / static_cast<uint32_t>(a.block_size);
-        n += tokens - n * static_cast<uint32_t>(a.block_size) != 0;
+      const bool there = r < a.requests;
+      const bool done = there && a.finished[r];
+      const int tokens = there ? a.seq_lens[r] : 0;  // beside `finished`, not behind it
+      if (done) {
+        n = static_cast<int>(min(block_size.ceil(static_cast<uint32_t>(max(tokens, 0))),
+                                 static_cast<uint32_t>(a.width)));
       }
-      ends[tid] = static_cast<int>(min(n, static_cast<uint32_t>(a.width)));
+      place[tid] = 0;
+    }
+    const unsigned gives = __ballot_sync(kFullMask, n > a.shared_blocks);
+    if (tid < kReleaseRows && lane == 0) warp_rows[warp] = __popc(gives);
+    __syncthreads();
+    int rows = 0;
+    {
+      int before = 0;
+#pragma unroll
+      for (int w = 0; w < kReleaseRows / kWarpSize; ++w) {
+        if (w < warp) before += warp_rows[w];
+        rows += warp_rows[w];
+      }
+      if (n > a.shared_blocks) {
+        const int at = before + __popc(gives & ((1u << lane) - 1));
+        listed[at] = first + tid;
+        ends[at] = n;
+      }
     }
     __syncthreads();
-    // f(row of the warp, entry there and in the pool, id) for the warp's rows
-    // side by side, in the order of the entries for each
-    auto over_entries = [&](auto f) {
-      int most = 0;
+    // f(entry is in the pool, id) over a listed row, 32 entries at a time in order
+    auto over_entries = [&](int i, auto f) {
+      const int end = ends[i];
+      const int32_t* ids = a.table + static_cast<int64_t>(listed[i]) * a.table_stride;
+      for (int j0 = a.shared_blocks; j0 < end; j0 += kAhead * kWarpSize) {
+        int id[kAhead];
 #pragma unroll
-      for (int i = 0; i < kRowsOfWarp; ++i) most = max(most, ends[warp * kRowsOfWarp + i]);
-      for (int j0 = a.shared_blocks; j0 < most; j0 += kAhead * kWarpSize) {
-        int id[kRowsOfWarp][kAhead];
-#pragma unroll
-        for (int i = 0; i < kRowsOfWarp; ++i) {
-          const int n = ends[warp * kRowsOfWarp + i];
-          const int32_t* ids = a.table + static_cast<int64_t>(first + warp * kRowsOfWarp + i) * a.table_stride;
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            const int j = j0 + k * kWarpSize + lane;
-            id[i][k] = j < n ? ids[j] : -1;
-          }
+        for (int k = 0; k < kAhead; ++k) {
+          const int j = j0 + k * kWarpSize + lane;
+          id[k] = j < end ? ids[j] : -1;
         }
 #pragma unroll
-        for (int i = 0; i < kRowsOfWarp; ++i) {
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            f(i, static_cast<uint32_t>(id[i][k]) < static_cast<uint32_t>(a.pool), id[i][k]);
+        for (int k = 0; k < kAhead; ++k) {
+          if (j0 + k * kWarpSize < end) {
+            f(static_cast<uint32_t>(id[k]) < static_cast<uint32_t>(a.pool), id[k]);
           }
         }
       }
     };
-    int found[kRowsOfWarp] = {};
-    over_entries([&](int i, bool back, int) { found[i] += back; });
-#pragma unroll
-    for (int i = 0; i < kRowsOfWarp; ++i) {
-      const int all = __reduce_add_sync(kFullMask, found[i]);
-      if (lane == 0) place[warp * kRowsOfWarp + i] = all;
+    for (int i = warp; i < rows; i += warps) {
+      int found = 0;
+      over_entries(i, [&](bool back, int) { found += back; });
+      found = __reduce_add_sync(kFullMask, found);
+      if (lane == 0) place[i] = found;
     }
     __syncthreads();
     if (warp == 0) {
@@ -360,28 +387,32 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
       if (lane == kWarpSize - 1) block_total[round] = upto;
     }
     step_barrier<kBlocks>();
-    int64_t before = carry;
-#pragma unroll
-    for (int k = 0; k < kBlocks; ++k) {
-      int total;
+    // a lane reads one block's total
+    int64_t total = 0;
+    if (lane < kBlocks) {
       if constexpr (kBlocks > 1) {
-        total = *cg::this_cluster().map_shared_rank(&block_total[round], k);
+        total = *cg::this_cluster().map_shared_rank(&block_total[round], lane);
       } else {
         total = block_total[round];
       }
-      if (k < rank) before += total;
-      carry += total;
     }
-    int64_t at[kRowsOfWarp];
+    int64_t before = lane < rank ? total : 0;
 #pragma unroll
-    for (int i = 0; i < kRowsOfWarp; ++i) at[i] = before + place[warp * kRowsOfWarp + i];
-    over_entries([&](int i, bool back, int id) {
-      const unsigned set = __ballot_sync(kFullMask, back);
-      const int64_t mine = at[i] + __popc(set & ((1u << lane) - 1));
-      if (back && mine < a.pool) a.free_blocks[mine] = id;
-      at[i] += __popc(set);
-    });
-    __syncthreads();  // the next round's lengths and counts follow these reads
+    for (int d = kWarpSize / 2; d > 0; d /= 2) {
+      before += __shfl_xor_sync(kFullMask, before, d);
+      total += __shfl_xor_sync(kFullMask, total, d);
+    }
+    for (int i = warp; i < rows; i += warps) {
+      int64_t at = carry + before + place[i];
+      over_entries(i, [&](bool back, int id) {
+        const unsigned set = __ballot_sync(kFullMask, back);
+        const int64_t mine = at + __popc(set & ((1u << lane) - 1));
+        if (back && mine < a.pool) a.free_blocks[mine] = id;
+        at += __popc(set);
+      });
+    }
+    carry += total;
+    __syncthreads();  // the next round's lists and counts follow these reads
   }
   // no block leaves while another may still read its total
   step_barrier<kBlocks>();
@@ -392,9 +423,10 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
 
 int check_pool(const void* free_blocks, int64_t pool, const void* free_count, const void* count_out,
                int64_t requests, int64_t width, int64_t table_stride, int64_t block_size) {
-  if (requests < 0 || width < 0 || pool < 0 || requests > INT32_MAX || width > INT32_MAX) {
+  if (requests < 0 || width < 0 || pool < 0 || requests > INT32_MAX || width > INT32_MAX ||
+      pool >= INT32_MAX) {
     return fail(SM120N_ERR_INVALID_ARGUMENT,
-                "requests, table width and pool size must be in [0, 2^31)");
+                "requests, table width and pool size must be in [0, 2^31 - 1)");
   }
   if (block_size < 1 || block_size > INT32_MAX || pool > (int64_t{1} << 31) / block_size) {
     return fail(SM120N_ERR_INVALID_ARGUMENT,
@@ -431,8 +463,8 @@ extern "C" int sm120s_plan_step(const int32_t* context_lens, const int32_t* quer
   int rc = check_pool(free_blocks, pool, free_count, free_count_out, requests, table_width,
                       table_stride, block_size);
   if (rc != SM120N_OK) return rc;
-  if (tokens < 0 || tokens > INT32_MAX) {
-    return fail(SM120N_ERR_INVALID_ARGUMENT, "tokens must be in [0, 2^31)");
+  if (tokens < 0 || tokens >= INT32_MAX) {
+    return fail(SM120N_ERR_INVALID_ARGUMENT, "tokens must be in [0, 2^31 - 1)");
   }
   if (!query_start || (requests > 0 && (!context_lens || !query_lens || !seq_lens)) ||
       (requests > 0 && table_width > 0 && !block_table) ||
