@@ -53,4 +53,7 @@ void fill_qk_cache_args(sm120n_qk_cache_args& a, const torch::Tensor& query,
                         const c10::optional<torch::Tensor>& v_scale, bool is_neox,
                         c10::string_view kv_cache_layout, double epsilon);
 
+// The serving operators as functions of the extension module.
+void define_serving(pybind11::module_& m);
+
 }  // namespace sm120n_binding

@@ -312,3 +312,34 @@ TORCH_LIBRARY_IMPL(sm120_norm_ext, CUDA, m) {
   m.impl("prompt_attention", &b200_prompt_attention);
   m.impl("paged_decode_attention", &b200_paged_decode_attention);
 }
+
+// The same functions on the extension module: a call through it costs the host
+// about half of one through the dispatcher, which is most of a small step.
+void sm120n_binding::define_serving(pybind11::module_& m) {
+  using OptionalTensor = c10::optional<torch::Tensor>;
+  m.def("plan_step_", &b200_plan_step, "Block tables, positions and slot maps of a step (CUDA)");
+  m.def("release_blocks_", &b200_release_blocks, "Blocks of finished requests back to the pool (CUDA)");
+  m.def("qk_norm_mrope_cache_",
+        [](torch::Tensor query, torch::Tensor key, OptionalTensor value, torch::Tensor query_weight,
+           torch::Tensor key_weight, torch::Tensor positions, torch::Tensor cos_sin_cache,
+           std::vector<int64_t> sections, OptionalTensor key_cache, OptionalTensor value_cache,
+           OptionalTensor slot_mapping, OptionalTensor k_scale, OptionalTensor v_scale,
+           bool is_neox, bool interleaved_sections, const std::string& kv_cache_layout,
+           double epsilon, OptionalTensor query_out, OptionalTensor key_out) {
+          b200_qk_norm_mrope_cache(query, key, value, query_weight, key_weight, positions,
+                                   cos_sin_cache, sections, key_cache, value_cache, slot_mapping,
+                                   k_scale, v_scale, is_neox, interleaved_sections,
+                                   kv_cache_layout, epsilon, query_out, key_out);
+        },
+        "Q/K norm + rotation by positions with several axes + KV store (CUDA)");
+  m.def("prompt_attention", &b200_prompt_attention, "Causal attention of packed prompts (CUDA)");
+  m.def("paged_decode_attention",
+        [](torch::Tensor out, torch::Tensor query, torch::Tensor key_cache,
+           torch::Tensor value_cache, torch::Tensor block_table, torch::Tensor seq_lens,
+           OptionalTensor prefix_blocks, OptionalTensor k_scale, OptionalTensor v_scale,
+           const std::string& kv_cache_layout, c10::optional<double> scale) {
+          b200_paged_decode_attention(out, query, key_cache, value_cache, block_table, seq_lens,
+                                      prefix_blocks, k_scale, v_scale, kv_cache_layout, scale);
+        },
+        "Attention of one token per request over a paged cache (CUDA)");
+}

@@ -600,4 +600,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "In-place fused Q/K RMSNorm + RoPE (CUDA)");
   m.def("fused_qk_rms_norm_rope_kv", &b200_fused_qk_rms_norm_rope_kv,
         "In-place fused Q/K RMSNorm + RoPE + paged KV store (CUDA)");
+  define_serving(m);
 }

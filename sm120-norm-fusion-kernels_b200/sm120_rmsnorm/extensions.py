@@ -104,7 +104,7 @@ def qk_norm_mrope_cache_(
     to the activation dtype and separately to an fp8 cache, so a result may
     differ in its last place from :func:`qk_norm_rope_cache_`, which rounds after
     each stage."""
-    _op("qk_norm_mrope_cache_")(
+    _op("qk_norm_mrope_cache_", query)(
         query, key, value, query_weight, key_weight, positions, cos_sin_cache, sections,
         key_cache, value_cache, slot_mapping, k_scale, v_scale, is_neox, interleaved_sections,
         kv_cache_layout, epsilon, query_out, key_out)

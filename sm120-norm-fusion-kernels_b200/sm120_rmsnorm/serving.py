@@ -24,11 +24,18 @@ from .ops import _C, _extension
 
 
 @functools.cache
-def _op(name: str):
-    """The operator itself: small steps are bound by the host, and looking the
-    overload up at every call costs as much as the call."""
-    _extension()
+def _dispatched(name: str):
     return getattr(torch.ops.sm120_norm_ext, name).default
+
+
+def _op(name: str, tensor: torch.Tensor):
+    """The operator: the extension's function for ordinary tensors (small steps
+    are bound by the host, and the dispatcher costs as much again), the
+    registered operator for tracing and for tensor subclasses."""
+    if type(tensor) is torch.Tensor and not torch.compiler.is_compiling():
+        return getattr(_extension(), name)
+    _extension()
+    return _dispatched(name)
 
 
 def plan_step_(
@@ -59,7 +66,7 @@ def plan_step_(
     behind the last token, which the Q/K norm operators leave untouched.
     ``free_count`` (int32 [1]) is updated in place, or left as it is with the new
     count in ``free_count_out``."""
-    _op("plan_step_")(
+    _op("plan_step_", context_lens)(
         context_lens, query_lens, block_table, free_blocks, free_count, block_size, query_start,
         seq_lens, positions, slot_mapping, free_count_out)
 
@@ -79,9 +86,8 @@ def release_blocks_(
     ``shared_blocks`` of every row (a prefix that others still use) stay out.
     Table entries outside the pool are skipped. The table and ``seq_lens`` are
     not written: a row given back must not be given back again."""
-    _op("release_blocks_")(seq_lens, finished, block_table, free_blocks,
-                                             free_count, block_size, shared_blocks,
-                                             free_count_out)
+    _op("release_blocks_", seq_lens)(seq_lens, finished, block_table, free_blocks, free_count,
+                                     block_size, shared_blocks, free_count_out)
 
 
 def prompt_attention(
@@ -101,7 +107,7 @@ def prompt_attention(
     lengths need not be known on the host. Rows of ``out`` behind the last
     sequence are left as they were. ``scale`` defaults to 1 / sqrt(D) and must be
     positive."""
-    _op("prompt_attention")(out, query, key, value, query_start, scale)
+    _op("prompt_attention", out)(out, query, key, value, query_start, scale)
 
 
 def paged_decode_attention(
@@ -132,7 +138,7 @@ def paged_decode_attention(
     request of at least ``P * block_size`` tokens reads its first P blocks from
     there instead of from its row, and they are read once for the whole batch;
     a shorter one is read through its row alone."""
-    _op("paged_decode_attention")(
+    _op("paged_decode_attention", out)(
         out, query, key_cache, value_cache, block_table, seq_lens, prefix_blocks, k_scale,
         v_scale, kv_cache_layout, scale)
 
