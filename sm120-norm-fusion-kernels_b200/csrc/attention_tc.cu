@@ -407,7 +407,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         }
       }
       if constexpr (kPass == kPrefix) {
-        if (c.holes) {
+        if (*reinterpret_cast<volatile int*>(&c.holes)) {
 #pragma unroll
           for (int k = 0; k < kTileKeys; ++k) {
             const int64_t key = min(w.key_first + key0 + k, int64_t{a.prefix_tokens} - 1);
@@ -669,8 +669,11 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
             if (static_cast<uint32_t>(found) < static_cast<uint32_t>(a.kv.num_blocks)) {
               id = found;
               first_slot = static_cast<int>(key - static_cast<int64_t>(block) * a.kv.block_size);
+            } else {
+              *reinterpret_cast<volatile int*>(&c.holes) = 1;  // before the tile can arrive
             }
           }
+          __syncwarp();
           if (elect_lane()) mbarrier_arrive_expect_tx(loaded, kFp8 ? S::kRawBytes : S::kTileBytes);
           for (int b = 0; b < kTileKeys / box; ++b) {
             const int block = __shfl_sync(kFullMask, id, b);
@@ -824,13 +827,6 @@ __global__ void __launch_bounds__(TcShape<D, 2>::kThreads, 1)
   w.key_first = static_cast<int>(tiles * w.split / a.prefix_splits * kTileKeys);
   w.key_last = static_cast<int>(min(tiles * (w.split + 1) / a.prefix_splits * kTileKeys,
                                     int64_t{a.prefix_tokens}));
-  bool holes = false;
-  for (int b = w.key_first / a.kv.block_size + threadIdx.x;
-       b <= (w.key_last - 1) / a.kv.block_size; b += S::kThreads) {
-    holes |= static_cast<uint32_t>(a.prefix_blocks[b]) >= static_cast<uint32_t>(a.kv.num_blocks);
-  }
-  if (__syncthreads_or(holes) && threadIdx.x == 0) control.holes = 1;
-  __syncthreads();
   attend<TQ, T, kFp8, D, 2, kPrefix>(a, w, &key_map, &value_map, control,
                                      aligned_tiles(dynamic_smem));
   close_block<S>(control);
