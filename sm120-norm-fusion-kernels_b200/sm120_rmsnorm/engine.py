@@ -18,6 +18,11 @@ projection on the tensor cores with the Q/K norm + RoPE + KV store in its
 epilogue (``extensions.qkv_proj_norm_rope_cache_``; bf16, head_dim 128, dense
 NHD caches), bit-identical to that kernel's plain GEMM followed by step 3.
 
+:class:`PagedSteps` keeps the block tables of a batch and plans its steps on the
+GPU, and :class:`Qwen3Attention` runs a layer's whole attention on such a plan:
+the prologue, then the attention of whole prompts or of one token per request
+over the paged cache.
+
 :class:`DecodeGraph` captures the prologues of all layers of one decode step
 into a single CUDA graph, so the host launches one graph per step; the B200
 kernels additionally overlap each launch with the tail of the previous kernel
@@ -30,7 +35,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import extensions, ops
+from . import extensions, ops, serving
 
 
 @dataclass(frozen=True)
@@ -42,6 +47,9 @@ class Qwen3AttentionShape:
     rope_theta: float = 1e6
     max_positions: int = 32768
     epsilon: float = 1e-6
+    # pairs of a head that turn by time, height and width (positions [3, tokens])
+    rope_sections: tuple[int, ...] = (16, 24, 24)
+    rope_sections_interleaved: bool = False
 
     @property
     def qkv_width(self) -> int:
@@ -98,11 +106,107 @@ class Qwen3AttentionPrologue:
             return self.split(qkv_out)
         torch.matmul(hidden, self.qkv_weight.t(), out=qkv_out)
         q, k, v = self.split(qkv_out)
+        if positions.dim() == 2:  # [axes, tokens]: time, height, width
+            extensions.qk_norm_mrope_cache_(
+                q, k, v, self.query_norm_weight, self.key_norm_weight, positions, cos_sin_cache,
+                list(s.rope_sections), key_cache, value_cache, slot_mapping, k_scale, v_scale, True,
+                s.rope_sections_interleaved, kv_cache_layout, s.epsilon)
+            return q, k, v
         extensions.qk_norm_rope_cache_(
             q, k, v, self.query_norm_weight, self.key_norm_weight, positions, cos_sin_cache,
             key_cache, value_cache, slot_mapping, k_scale, v_scale, True, kv_cache_layout,
             s.epsilon)
         return q, k, v
+
+
+class PagedSteps:
+    """Block tables and step plans of up to ``requests`` requests over a cache of
+    ``num_blocks`` blocks, all on the GPU: no length has to come back to the host.
+
+    ``context_lens`` is what the cache holds for each request and follows every
+    :meth:`plan`; ``query_start``, ``positions`` and ``slot_mapping`` are those of the
+    step planned last. ``prefix_blocks`` blocks, taken off the pool here, are
+    the first of every request's row; a request that begins behind them starts
+    with ``context_lens`` at their length.
+    """
+
+    def __init__(self, requests: int, num_blocks: int, max_blocks: int, max_tokens: int, device,
+                 block_size: int = 16, prefix_blocks: int = 0):
+        def ints(*shape, dtype=torch.int32):
+            return torch.zeros(*shape, device=device, dtype=dtype)
+
+        self.block_size = block_size
+        self.free_blocks = torch.arange(num_blocks - 1, -1, -1, device=device, dtype=torch.int32)
+        self.free_count = torch.full((1,), num_blocks - prefix_blocks, device=device,
+                                     dtype=torch.int32)
+        # the top of the stack, block 0 first
+        self.prefix = self.free_blocks[num_blocks - prefix_blocks:].flip(0).clone()
+        self.block_table = torch.full((requests, max_blocks), -1, device=device, dtype=torch.int32)
+        self.block_table[:, :prefix_blocks] = self.prefix
+        self.context_lens = ints(requests)
+        self.query_start = ints(requests + 1)
+        self.positions = ints(max_tokens, dtype=torch.int64)
+        self.slot_mapping = ints(max_tokens)
+
+    def plan(self, query_lens: torch.Tensor) -> None:
+        """The next step, with ``query_lens`` (int32 [requests]) new tokens."""
+        serving.plan_step_(self.context_lens, query_lens, self.block_table, self.free_blocks,
+                           self.free_count, self.block_size, self.query_start, self.context_lens,
+                           self.positions, self.slot_mapping)
+
+    def release(self, finished: torch.Tensor) -> None:
+        """Gives the blocks of the requests in ``finished`` (bool [requests]) back,
+        all but the shared ones, and sets their lengths to zero."""
+        serving.release_blocks_(self.context_lens, finished, self.block_table, self.free_blocks,
+                                self.free_count, self.block_size, self.prefix.numel())
+        self.context_lens.masked_fill_(finished, 0)
+
+
+class Qwen3Attention:
+    """A layer's attention on a planned step: prologue, K and V into the paged
+    cache, attention. Returns [tokens, query_heads, head_dim], the input of the
+    output projection. ``positions`` default to the plan's; [3, tokens] for
+    images and video."""
+
+    def __init__(self, prologue: Qwen3AttentionPrologue, key_cache: torch.Tensor,
+                 value_cache: torch.Tensor, cos_sin_cache: torch.Tensor, k_scale=None,
+                 v_scale=None, kv_cache_layout: str = "NHD"):
+        self.prologue = prologue
+        self.key_cache, self.value_cache = key_cache, value_cache
+        self.cos_sin_cache = cos_sin_cache
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self.kv_cache_layout = kv_cache_layout
+
+    def _queries(self, hidden, residual, steps, positions, qkv):
+        tokens = hidden.shape[0]
+        if qkv is None:
+            qkv = torch.empty(tokens, self.prologue.shape.qkv_width, device=hidden.device,
+                              dtype=hidden.dtype)
+        positions = steps.positions[:tokens] if positions is None else positions
+        return self.prologue.forward(hidden, residual, positions, self.cos_sin_cache,
+                                     self.key_cache, self.value_cache,
+                                     steps.slot_mapping[:tokens], qkv, self.k_scale, self.v_scale,
+                                     self.kv_cache_layout)
+
+    def prompts(self, hidden: torch.Tensor, residual: torch.Tensor, steps: PagedSteps,
+                positions: torch.Tensor | None = None, qkv: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+        """Whole prompts, packed as ``steps`` planned them from empty contexts."""
+        q, k, v = self._queries(hidden, residual, steps, positions, qkv)
+        out = torch.zeros(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+        serving.prompt_attention(out, q, k, v, steps.query_start)
+        return out
+
+    def decode(self, hidden: torch.Tensor, residual: torch.Tensor, steps: PagedSteps,
+               positions: torch.Tensor | None = None, qkv: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """One token for every request, as ``steps`` planned them."""
+        q, _, _ = self._queries(hidden, residual, steps, positions, qkv)
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+        serving.paged_decode_attention(out, q, self.key_cache, self.value_cache,
+                                       steps.block_table, steps.context_lens, steps.prefix,
+                                       self.k_scale, self.v_scale, self.kv_cache_layout)
+        return out
 
 
 class DecodeGraph:
