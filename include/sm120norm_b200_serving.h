@@ -66,7 +66,7 @@ SM120N_API int sm120s_reset_device_faults(void);
  * free_blocks [pool] is a stack whose top is free_blocks[free_count - 1]; it is
  * not written. free_count_out may be free_count and seq_lens may be
  * context_lens; other buffers may not overlap. tokens is the length of
- * positions (int64) and slot_mapping (int32). A total of 2^31 tokens or more is
+ * positions (int64) and slot_mapping (int32). A request of 2^31 tokens or more is
  * not served.
  */
 SM120N_API int sm120s_plan_step(const int32_t* context_lens, const int32_t* query_lens,
@@ -177,7 +177,7 @@ SM120N_API int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
  *   out[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_b . k_j)
  * fp32 scores, sums and values, p rounded to 16 bits for the second product;
  * zeros where there is no key. Blocks outside [0, num_blocks) hold no keys. The
- * prefix is read once for all requests.
+ * prefix is read once for all requests. out may not overlap query.
  * query, out [batch, query_heads, head_dim], heads adjacent; caches as
  * sm120n_qk_cache_args (one shape and stride for both), rows 16-byte aligned;
  * fp8 caches stand for code * k_scale[0] / code * v_scale[0]. dtype f16 or bf16.

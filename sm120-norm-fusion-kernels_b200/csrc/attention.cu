@@ -19,9 +19,9 @@ int check_heads(int dtype, int64_t query_heads, int64_t key_heads, int64_t head_
     return fail(SM120N_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256 (got %lld)",
                 static_cast<long long>(head_dim));
   }
-  if (key_heads < 1 || query_heads < 1 || query_heads % key_heads != 0 || query_heads > (1 << 16)) {
+  if (key_heads < 1 || query_heads < 1 || query_heads % key_heads != 0 || query_heads >= (1 << 16)) {
     return fail(SM120N_ERR_INVALID_ARGUMENT,
-                "query_heads must be a positive multiple of key_heads, at most 2^16");
+                "query_heads must be a positive multiple of key_heads, below 2^16");
   }
   if (!(scale > 0.0f) || !std::isfinite(scale * kLog2e)) {
     return fail(SM120N_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
@@ -46,7 +46,7 @@ int check_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int
 // Whether the prefix runs on tensor memory: 256 rows and 128 keys to a tile
 // there, 64 and 64 otherwise.
 bool prefix_on_tensor_memory(const sm120s_decode_args& a) {
-  return a.head_dim <= 128 && a.num_blocks > 0 && block_fills_tiles(a.block_size, 128);
+  return a.head_dim <= 128 && block_fills_tiles(a.block_size, 128);
 }
 
 struct Plan {
@@ -73,6 +73,9 @@ int check_decode_sizes(const sm120s_decode_args* a) {
       a->num_blocks < 0) {
     return fail(SM120N_ERR_INVALID_ARGUMENT,
                 "batch must be in [0, 2^20], table and prefix lengths non-negative");
+  }
+  if (a->batch * a->query_heads > INT32_MAX) {
+    return fail(SM120N_ERR_INVALID_ARGUMENT, "batch * query_heads must be below 2^31");
   }
   if (a->block_size < 1 || a->block_size > INT32_MAX ||
       a->num_blocks > (int64_t{1} << 31) / a->block_size) {
@@ -104,7 +107,7 @@ int plan_decode(const sm120s_decode_args& a, Plan* plan) {
       1, std::min<int64_t>(own_blocks_per_sm(static_cast<int>(a.head_dim)) * dev.sm_count,
                            triples * most_tiles)));
   plan->prefix_splits = 0;
-  if (a.prefix_blocks_count > 0) {
+  if (a.prefix_blocks_count > 0 && a.num_blocks > 0) {
     const bool tc = prefix_on_tensor_memory(a);
     const int64_t tile_rows = tc ? 256 : 64, tile_keys = tc ? 128 : 64;
     const int64_t row_tiles = (a.batch * group + tile_rows - 1) / tile_rows;
@@ -113,7 +116,7 @@ int plan_decode(const sm120s_decode_args& a, Plan* plan) {
     plan->prefix_splits = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>(tiles, (tc ? 1 : 2) * dev.sm_count / blocks)));
   }
-  size_t at = (static_cast<size_t>(a.batch + 1) * sizeof(int32_t) + 15) / 16 * 16;
+  size_t at = (static_cast<size_t>(a.batch + 1) * sizeof(int64_t) + 15) / 16 * 16;
   const size_t own_rows = static_cast<size_t>(triples + plan->own_grid) * 16;
   const size_t prefix_rows = static_cast<size_t>(plan->prefix_splits) * a.batch * a.query_heads;
   plan->own_state = at;
@@ -250,8 +253,9 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
   a.out_stride = in.out_token_stride;
   a.table_stride = in.table_stride;
   a.batch = static_cast<int32_t>(in.batch);
-  a.table_width = static_cast<int32_t>(in.table_width);
-  a.prefix_tokens = static_cast<int32_t>(in.prefix_blocks_count * in.block_size);
+  // a cache without blocks holds no keys, whatever the tables say
+  a.table_width = in.num_blocks > 0 ? static_cast<int32_t>(in.table_width) : 0;
+  a.prefix_tokens = in.num_blocks > 0 ? static_cast<int32_t>(in.prefix_blocks_count * in.block_size) : 0;
   a.query_heads = static_cast<int32_t>(in.query_heads);
   a.key_heads = static_cast<int32_t>(in.key_heads);
   a.group = static_cast<int32_t>(in.query_heads / in.key_heads);
@@ -259,7 +263,7 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
   a.own_grid = plan.own_grid;
   a.prefix_splits = plan.prefix_splits;
   a.scale_log2 = in.scale * kLog2e;
-  a.tile_start = reinterpret_cast<int32_t*>(space);
+  a.tile_start = reinterpret_cast<int64_t*>(space);
   a.own_state = reinterpret_cast<float2*>(space + plan.own_state);
   a.own_values = reinterpret_cast<float*>(space + plan.own_values);
   a.prefix_state = reinterpret_cast<float2*>(space + plan.prefix_state);

@@ -63,7 +63,7 @@ struct DecodeArgs {
   int32_t own_grid;       // thread blocks of the pass over each request's own tokens
   int32_t prefix_splits;  // parts of the prefix
   float scale_log2;
-  int32_t* tile_start;  // [batch + 1] key tiles of the requests before, per key head and row tile
+  int64_t* tile_start;  // [batch + 1] key tiles of the requests before, per key head and row tile
   float2* own_state;    // [(batch * key_heads * row_tiles + own_grid) * 16] (maximum, sum)
   float* own_values;    // the same rows x head_dim
   float2* prefix_state;  // [prefix_splits, batch, query_heads]

@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
     return before;
   };
   const int64_t total = over_requests([&](int i, int64_t start, int) {
-                          if (blockIdx.x == 0) a.tile_start[i] = static_cast<int32_t>(start);
+                          if (blockIdx.x == 0) a.tile_start[i] = start;
                         }) * triples;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = static_cast<int32_t>(total / triples);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = total / triples;
   const int64_t runs = min(total, int64_t{a.own_grid});
   if (blockIdx.x >= runs) {
     if (beside_prefix && blockIdx.x == 0) wait_for_upstream_grid();
@@ -639,9 +639,9 @@ __global__ void __launch_bounds__(kWarps* kWarpSize) merge_kernel(DecodeArgs a) 
   if (keys > 0) {
     const int triples = a.key_heads * a.row_tiles;
     const int triple = kv_head * a.row_tiles + in_group / 16;
-    const int64_t total = static_cast<int64_t>(a.tile_start[a.batch]) * triples;
+    const int64_t total = a.tile_start[a.batch] * triples;
     const int64_t n = a.tile_start[request + 1] - a.tile_start[request];
-    const int64_t t0 = static_cast<int64_t>(a.tile_start[request]) * triples + triple * n;
+    const int64_t t0 = a.tile_start[request] * triples + triple * n;
     const int64_t runs = min(total, int64_t{a.own_grid});
     // the runs that hold the triple's first and last tile
     const int64_t from = ((t0 + 1) * runs - 1) / total;
@@ -731,7 +731,7 @@ int run_own(const DecodeArgs& a, cudaStream_t stream) {
 
 template <typename TQ, typename T, bool kFp8, int D>
 int run_own(const DecodeArgs& a, cudaStream_t stream) {
-  return block_fills_tiles(a.kv.block_size, kTileKeys) && a.kv.num_blocks > 0
+  return block_fills_tiles(a.kv.block_size, kTileKeys) && a.table_width > 0
              ? run_own<TQ, T, kFp8, D, true>(a, stream)
              : run_own<TQ, T, kFp8, D, false>(a, stream);
 }

@@ -48,6 +48,13 @@ int32_t* count_after(const torch::Tensor& count, const c10::optional<torch::Tens
   return out->data_ptr<int32_t>();
 }
 
+void check_apart(const torch::Tensor& out, const torch::Tensor& in, const char* out_name,
+                 const char* name) {
+  const auto status = at::get_overlap_status(out, in);
+  TORCH_CHECK(status != at::MemOverlapStatus::Full && status != at::MemOverlapStatus::Partial,
+              out_name, " may not overlap ", name);
+}
+
 double default_scale(c10::optional<double> scale, int64_t head_dim) {
   return scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(head_dim));
 }
@@ -145,6 +152,9 @@ void b200_qk_norm_mrope_cache(torch::Tensor query, torch::Tensor key,
     TORCH_CHECK(out->sizes() == in.sizes() && out->scalar_type() == in.scalar_type(), name,
                 " must have its input's shape and dtype");
     TORCH_CHECK(out->device() == in.device(), "all tensors must be on the same CUDA device");
+    if (out->data_ptr() != in.data_ptr() || out->strides() != in.strides()) {
+      check_apart(*out, in, name, "its input");
+    }
     *pointer = out->data_ptr();
     *stride = token_stride(*out);
   };
@@ -173,9 +183,9 @@ void b200_prompt_attention(torch::Tensor out, torch::Tensor query, torch::Tensor
               "all tensors must be on the same CUDA device");
   check_vector(query_start, torch::kInt, -1, device, "query_start");
   TORCH_CHECK(query_start.numel() >= 1, "query_start must have one entry per sequence and one more");
-  at::assert_no_overlap(out, query);
-  at::assert_no_overlap(out, key);
-  at::assert_no_overlap(out, value);
+  check_apart(out, query, "out", "query");
+  check_apart(out, key, "out", "key");
+  check_apart(out, value, "out", "value");
   sm120s_prompt_args a{};
   a.struct_size = sizeof(a);
   a.dtype = dtype_code(query);
@@ -231,7 +241,7 @@ void b200_paged_decode_attention(torch::Tensor out, torch::Tensor query, torch::
               "all tensors must be on the same CUDA device");
   check_table(block_table, query.size(0), device);
   check_vector(seq_lens, torch::kInt, query.size(0), device, "seq_lens");
-  at::assert_no_overlap(out, query);
+  check_apart(out, query, "out", "query");
   sm120s_decode_args a{};
   a.struct_size = sizeof(a);
   a.dtype = dtype_code(query);

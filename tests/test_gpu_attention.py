@@ -409,3 +409,63 @@ def test_two_graphs_replayed_side_by_side():
     c = cases[0]
     w, bound = ref.decode(c.q, c.kc, c.vc, c.table, [16 * 30 + 5] * len(RAGGED), c.prefix)
     assert_within(c.out, w, bound)
+
+
+def test_a_cache_without_blocks_and_an_empty_table():
+    c = Decode([5, 0, 90], 2, seed=12)
+    c.kc, c.vc = c.kc[:0], c.vc[:0]
+    assert (c.run() == 0).all()
+    c = Decode([5, 0, 90], seed=13)
+    c.table = c.table[:, :0]
+    assert (c.run() == 0).all()
+
+
+def test_large_blocks():
+    """Blocks that span several tiles of keys, and are not filled."""
+    for d in (64, 128, 256):
+        Decode([700, 129, 64, 1000, 256], 1, d=d, block_size=256, seed=14).check()
+        Decode([700, 129, 64, 1000], 0, d=d, block_size=1024, layout="HND", cache="fp8", seed=15).check()
+
+
+def test_refusals_of_the_binding():
+    c = Decode([50, 60], 2, seed=16)
+    p = Prompt([40], seed=16)
+    good = (c.out, c.q, c.kc, c.vc, c.table, ints(c.lens), c.prefix)
+
+    def decode(message, **change):
+        names = ("out", "query", "key_cache", "value_cache", "block_table", "seq_lens", "prefix_blocks")
+        args = dict(zip(names, good)) | change
+        with pytest.raises(RuntimeError, match=message):
+            serving.paged_decode_attention(**args)
+
+    decode("dtype", query=c.q.half())
+    decode("float16 and bfloat16", query=c.q.float(), out=c.out.float(), key_cache=c.kc.float(),
+           value_cache=c.vc.float())
+    decode("one row per request", block_table=c.table[:1])
+    decode("int32", block_table=c.table.long())
+    decode("seq_lens", seq_lens=ints(c.lens).long())
+    decode("entries", seq_lens=ints([1, 2, 3]))
+    decode("4-D", value_cache=c.vc[1:])
+    decode("k_scale", key_cache=c.kc.to(torch.float8_e4m3fn), value_cache=c.vc.to(torch.float8_e4m3fn))
+    decode("multiple of key_heads", query=c.q[:, :3].contiguous(), out=c.out[:, :3].contiguous())
+    decode("layout", kv_cache_layout="DNH")
+    decode("past the prefix", prefix_blocks=ints([0] * 50))
+    decode("overlap", out=c.q)
+    decode("scale", scale=-1.0)
+    decode("16-byte", query=torch.zeros(2 * 8 * 128 + 1, dtype=c.q.dtype, device=DEV)[1:].view(2, 8, 128))
+
+    def prompt(message, **change):
+        args = dict(out=p.out, query=p.q, key=p.k, value=p.v, query_start=ints([0, 40])) | change
+        with pytest.raises(RuntimeError, match=message):
+            serving.prompt_attention(**args)
+
+    prompt("int32|Int", query_start=ints([0, 40]).long())
+    prompt("one more", query_start=ints([]))
+    prompt("key and value", key=p.k[:30])
+    prompt("dtypes must match", key=p.k.half())
+    prompt("out shape", out=p.out[:, :2])
+    prompt("head_dim", **{k: torch.zeros(40, 2, 96, dtype=torch.bfloat16, device=DEV)
+                          for k in ("out", "query", "key", "value")})
+    prompt("scale", scale=0.0)
+    same = p.q.contiguous()
+    prompt("overlap", out=same, query=same)
