@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   __shared__ __align__(8) uint64_t empty[kStages];
   __shared__ uint32_t live[kStages][2];  // which keys of a tile exist, one bit each
   __shared__ float2 states[kWarps][16];
-  __shared__ int32_t warp_totals[kThreads / kWarpSize];
+  __shared__ int64_t warp_totals[kThreads / kWarpSize];
   __shared__ int64_t found_start;
   __shared__ int found_request;
   const int warp = __shfl_sync(kFullMask, threadIdx.x / kWarpSize, 0);
@@ -176,21 +176,29 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   release_downstream_grid();
 
   const int triples = a.key_heads * a.row_tiles;  // of one request
-  // Sums of the requests' tiles, kThreads requests at a step; f(request, tiles before, tiles).
+  // Sums of the requests' tiles, kPer * kThreads requests at a step, kPer
+  // neighbours to a thread; f(first request, tiles before it, tiles of each).
+  constexpr int kPer = 4;
   auto over_requests = [&](auto f) {
     int64_t before = 0;
-    for (int base = 0; base < a.batch; base += kThreads) {
-      const int i = base + threadIdx.x;
-      int first;
-      const int mine = i < a.batch ? (own_tokens(a, i, &first) + kTileKeys - 1) / kTileKeys : 0;
-      int64_t upto = mine;
+    for (int base = 0; base < a.batch; base += kPer * kThreads) {
+      const int i = base + kPer * static_cast<int>(threadIdx.x);
+      int mine[kPer];
+      int64_t all_mine = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        int first;
+        mine[k] = i + k < a.batch ? (own_tokens(a, i + k, &first) + kTileKeys - 1) / kTileKeys : 0;
+        all_mine += mine[k];
+      }
+      int64_t upto = all_mine;
 #pragma unroll
       for (int d = 1; d < kWarpSize; d *= 2) {
         const int64_t x = __shfl_up_sync(kFullMask, upto, d);
         if (lane >= d) upto += x;
       }
       __syncthreads();
-      if (lane == kWarpSize - 1) warp_totals[warp] = static_cast<int32_t>(upto);
+      if (lane == kWarpSize - 1) warp_totals[warp] = upto;
       __syncthreads();
       int64_t all = 0;
 #pragma unroll
@@ -198,13 +206,32 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
         if (k < warp) upto += warp_totals[k];
         all += warp_totals[k];
       }
-      if (i < a.batch) f(i, before + upto - mine, mine);
+      f(i, before + upto - all_mine, mine);
       before += all;
     }
     return before;
   };
-  const int64_t total = over_requests([&](int i, int64_t start, int) {
-                          if (blockIdx.x == 0) a.tile_start[i] = start;
+  auto find = [&](int64_t at, int first, int64_t start, const int* n) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (at >= start * triples && at < (start + n[k]) * triples) {
+        found_request = first + k;
+        found_start = start * triples;
+      }
+      start += n[k];
+    }
+  };
+  // what the first step of the scan found, for batches that need no other
+  int64_t my_start = 0;
+  int my_tiles[kPer] = {};
+  const int64_t total = over_requests([&](int first, int64_t start, const int* n) {
+                          my_start = start;
+#pragma unroll
+                          for (int k = 0; k < kPer; ++k) {
+                            my_tiles[k] = n[k];
+                            if (blockIdx.x == 0 && first + k < a.batch) a.tile_start[first + k] = start;
+                            start += n[k];
+                          }
                         }) * triples;
   if (blockIdx.x == 0 && threadIdx.x == 0) a.tile_start[a.batch] = total / triples;
   const int64_t runs = min(total, int64_t{a.own_grid});
@@ -215,12 +242,11 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   Walk walk;
   walk.at = total * blockIdx.x / runs;
   walk.end = total * (blockIdx.x + 1) / runs;
-  over_requests([&](int i, int64_t start, int n) {
-    if (walk.at >= start * triples && walk.at < (start + n) * triples) {
-      found_request = i;
-      found_start = start * triples;
-    }
-  });
+  if (a.batch <= kPer * kThreads) {
+    find(walk.at, kPer * static_cast<int>(threadIdx.x), my_start, my_tiles);
+  } else {
+    over_requests([&](int first, int64_t start, const int* n) { find(walk.at, first, start, n); });
+  }
   __syncthreads();
   walk.request = found_request;
   walk.request_start = found_start;
@@ -682,23 +708,34 @@ __global__ void __launch_bounds__(kWarps* kWarpSize) merge_kernel(DecodeArgs a) 
     for (int i = 0; i < kPer; ++i) acc[i] *= keep;
     const unsigned those = __ballot_sync(kFullMask, seen);
     const int count = min(parts - first, kWarpSize);
-#pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-      const float f = __shfl_sync(kFullMask, factor, k);
-      const float* from = reinterpret_cast<const float*>(
-          __shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(values), k));
-      if ((those >> k) & 1u) {
-        float x[kPer];
-        if constexpr (kPer % 4 == 0) {
+    constexpr int kAhead = 32 / kPer;  // parts whose values are on their way at once
+    for (int k0 = 0; k0 < count; k0 += kAhead) {
+      float x[kAhead][kPer];
 #pragma unroll
-          for (int i = 0; i < kPer; i += 4) {
-            *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(from + lane * kPer + i);
+      for (int k = 0; k < kAhead; ++k) {
+        const float* from = reinterpret_cast<const float*>(
+            __shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(values), (k0 + k) & 31));
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[k][i] = 0.0f;
+        if (k0 + k < count && ((those >> (k0 + k)) & 1u)) {
+          if constexpr (kPer % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < kPer; i += 4) {
+              *reinterpret_cast<float4*>(x[k] + i) =
+                  *reinterpret_cast<const float4*>(from + lane * kPer + i);
+            }
+          } else {
+            *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from + lane * kPer);
           }
-        } else {
-          *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from + lane * kPer);
         }
+      }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] += x[i] * f;
+      for (int k = 0; k < kAhead; ++k) {
+        const float f = __shfl_sync(kFullMask, factor, (k0 + k) & 31);  // 0 for what was not seen
+        if (k0 + k < count) {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) acc[i] += x[k][i] * f;
+        }
       }
     }
   }
