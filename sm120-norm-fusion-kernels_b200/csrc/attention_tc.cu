@@ -66,7 +66,7 @@ enum Pass : int { kPrompt, kPrefix };
 // A block of one or two row tiles. Two share K and V and fill the SM. One
 // leaves room for a second block: half the rows to a block and twice as many
 // blocks, which spread more evenly over the SMs.
-template <int D, int kTiles>
+template <int D, int kTiles, bool kFp8 = false>
 struct TcShape {
   static constexpr int kStages =  // K and V tiles alternate: even
       kTiles == 2 ? (D == 64 ? 8 : 4) : (D == 64 ? 4 : 2);
@@ -74,9 +74,8 @@ struct TcShape {
   static constexpr uint32_t kQBytes = kTileRows * D * 2;
   static constexpr int kRawTiles = D == 64 ? 4 : 2;  // fp8 tiles on their way to be converted
   static constexpr uint32_t kRawBytes = kTileKeys * D;
-  static constexpr size_t smem(bool fp8) {
-    return kTiles * kQBytes + kStages * kTileBytes + (fp8 ? kRawTiles * kRawBytes : 0) + 1024;
-  }
+  static constexpr size_t kSmem =
+      kTiles * kQBytes + kStages * kTileBytes + (kFp8 ? kRawTiles * kRawBytes : 0) + 1024;
   static constexpr uint32_t kOutColumn = kTiles * kTileKeys;  // of tile 0; tile 1 is D further
   static constexpr bool kOwnP = D == 64;  // P beside S, 64 columns for each tile
   static constexpr uint32_t kPColumn = kOwnP ? kOutColumn + kTiles * D : 0;
@@ -85,13 +84,14 @@ struct TcShape {
   static constexpr int kSoftmaxWarps = 4 * kTiles;
   static constexpr int kIssuers = D == 64 ? kTiles : 1;
   static constexpr int kLoadWarp = kSoftmaxWarps + kIssuers;
-  static constexpr int kWarps = kSoftmaxWarps + 4;
+  static constexpr int kWarps = kSoftmaxWarps + (kFp8 ? 8 : 4);
   static constexpr int kThreads = kWarps * kWarpSize;
   static constexpr int kGuardWarps = kWarps - kLoadWarp - 1;  // look on, or convert
-  // Registers at launch: 168 for 384 threads, 128 for each of two blocks of
-  // 256; 2 x 208 + 88 = 3 x 168 and 208 + 48 = 2 x 128.
+  // Registers at launch: 168 for 384 threads, 128 for 512 and for each of two
+  // blocks of 256; 2 x 208 + 88 = 3 x 168, 2 x 208 + 2 x 48 = 4 x 128 and
+  // 208 + 48 = 2 x 128.
   static constexpr int kSoftmaxRegisters = 208;
-  static constexpr int kOtherRegisters = kTiles == 2 ? 88 : 48;
+  static constexpr int kOtherRegisters = kTiles == 2 && !kFp8 ? 88 : 48;
 };
 
 // Instruction descriptor of tcgen05.mma.kind::f16: fp32 accumulator (bit 4), the
@@ -279,7 +279,7 @@ __device__ __forceinline__ void convert_tiles(Control& c, unsigned char* stages,
 template <typename TQ, typename T, bool kFp8, int D, int kTiles, int kPass, typename Args>
 __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUtensorMap* key_map,
                                        const CUtensorMap* value_map, Control& c, unsigned char* smem) {
-  using S = TcShape<D, kTiles>;
+  using S = TcShape<D, kTiles, kFp8>;
   constexpr int kStages = S::kStages;
   const int warp = __shfl_sync(kFullMask, threadIdx.x / kWarpSize, 0);  // known to be uniform
   const int lane = threadIdx.x & (kWarpSize - 1);
@@ -808,11 +808,11 @@ __global__ void __launch_bounds__(TcShape<D, kTiles>::kThreads, 3 - kTiles)
 }
 
 template <typename TQ, typename T, bool kFp8, int D>
-__global__ void __launch_bounds__(TcShape<D, 2>::kThreads, 1)
+__global__ void __launch_bounds__(TcShape<D, 2, kFp8>::kThreads, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap key_map,
                      const __grid_constant__ CUtensorMap value_map,
                      const __grid_constant__ DecodeArgs a) {
-  using S = TcShape<D, 2>;
+  using S = TcShape<D, 2, kFp8>;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ Control control;
   open_block<S>(control, false, kFp8);
@@ -846,12 +846,12 @@ template <typename T, int D, int kTiles>
 int run_prompt(const PromptArgs& a, const CUtensorMap* maps, cudaStream_t stream) {
   using S = TcShape<D, kTiles>;
   auto kernel = prompt_tc_kernel<T, D, kTiles>;
-  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::smem(false));
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
   if (rc != SM120N_OK) return rc;
   constexpr int64_t kRows = kTiles * kTileRows;
   const int64_t tiles = (a.tokens * a.group + kRows - 1) / kRows + a.sequences;
   return launch(kernel, dim3(static_cast<unsigned>(tiles * a.key_heads)), dim3(S::kThreads),
-                S::smem(false), stream, maps[0], maps[1], a);
+                S::kSmem, stream, maps[0], maps[1], a);
 }
 
 template <typename T, int D>
@@ -876,7 +876,7 @@ int run_prompt_tiles(const PromptArgs& a, cudaStream_t stream) {
 
 template <typename TQ, typename T, bool kFp8, int D>
 int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
-  using S = TcShape<D, 2>;
+  using S = TcShape<D, 2, kFp8>;
   CUtensorMap maps[2] = {};
   for (int i = 0; i < 2; ++i) {
     const int rc = encode_cache_map(&maps[i], i ? a.kv.value : a.kv.key, a.kv, D, a.key_heads,
@@ -885,13 +885,13 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
     if (rc != SM120N_OK) return rc;
   }
   auto kernel = prefix_tc_kernel<TQ, T, kFp8, D>;
-  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::smem(kFp8));
+  const int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem);
   if (rc != SM120N_OK) return rc;
   const int64_t tiles = (static_cast<int64_t>(a.batch) * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
   return launch(kernel,
                 dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.key_heads),
                      static_cast<unsigned>(a.prefix_splits)),
-                dim3(S::kThreads), S::smem(kFp8), stream, maps[0], maps[1], a);
+                dim3(S::kThreads), S::kSmem, stream, maps[0], maps[1], a);
 }
 
 template <int D>
