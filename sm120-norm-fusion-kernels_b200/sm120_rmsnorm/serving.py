@@ -57,7 +57,9 @@ def plan_step_(
     cache and new ones. ``block_table`` (int32 [R, blocks], any row stride) gets
     the blocks that the new tokens need, from the top of the stack
     ``free_blocks[:free_count]`` downwards, in the order of the requests; a
-    request gets all it needs or none. ``query_start`` (int32 [R + 1]): where
+    request gets all it needs or none. ``free_blocks`` (int32 [blocks of the
+    cache]) has room for every block; table entries outside [0, its length) are
+    no blocks. ``query_start`` (int32 [R + 1]): where
     each request's tokens begin in the step's packed tokens. ``seq_lens`` (int32
     [R], may be ``context_lens`` itself): context + query, or the context alone
     for a request that got no blocks, whose table row is too short or whose
@@ -84,8 +86,9 @@ def release_blocks_(
     """Pushes the blocks of the rows with ``finished`` (bool [R]) back on the
     stack ``free_blocks[:free_count]``, row after row; the first
     ``shared_blocks`` of every row (a prefix that others still use) stay out.
-    Table entries outside the pool are skipped. The table and ``seq_lens`` are
-    not written: a row given back must not be given back again."""
+    Table entries outside [0, length of ``free_blocks``) are skipped. The table
+    and ``seq_lens`` are not written: a row given back must not be given back
+    again."""
     _op("release_blocks_", seq_lens)(seq_lens, finished, block_table, free_blocks, free_count,
                                      block_size, shared_blocks, free_count_out)
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import serving_reference as ref
-from sm120_rmsnorm import serving
+from sm120_rmsnorm import serving, serving_capi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -286,6 +286,14 @@ def test_decode_batches(batch, prefix):
            seed=batch).check()
 
 
+@pytest.mark.parametrize("batch", [768, 769, 1601])
+@pytest.mark.parametrize("prefix", [0, 2])
+def test_batches_that_are_scanned_in_several_steps(batch, prefix):
+    # 768 requests to a step; the last step's among them with tokens and without
+    lens = [(37 * i) % 90 if i % 5 else 0 for i in range(batch)]
+    Decode(lens, prefix, hq=2, hk=1, d=64, seed=batch).check()
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_one_long_request_and_a_long_prefix(d):
     Decode([30000], hq=4, hk=2, d=d, seed=1).check()
@@ -425,6 +433,11 @@ def test_large_blocks():
     for d in (64, 128, 256):
         Decode([700, 129, 64, 1000, 256], 1, d=d, block_size=256, seed=14).check()
         Decode([700, 129, 64, 1000], 0, d=d, block_size=1024, layout="HND", cache="fp8", seed=15).check()
+
+
+def test_no_wait_ran_out():
+    torch.cuda.synchronize()
+    assert serving_capi.device_faults() == 0
 
 
 def test_refusals_of_the_binding():
