@@ -24,16 +24,19 @@
 // (4096 tokens: 110 us with two issuers, 116 with one; at D = 128, where the
 // tiles take turns, 158 with two and four more warps, 146 with one). The next
 // warp loads K and V tiles by TMA into kStages shared-memory stages. The rest of
-// the 12 warps (prompts) look for infinite or NaN values in the V tiles that
+// the warps (prompts) look for infinite or NaN values in the V tiles that
 // some rows must not see, where a product would multiply them by zero; a block
-// that meets one does its rows by plain arithmetic instead. Q and O go through shared memory so that global
-// accesses are whole rows: a thread reading or writing its own row touches 32
-// lines in every instruction of its warp (4000 cycles for a block's rows).
+// that meets one does its rows by plain arithmetic instead. Q and O go through
+// shared memory so that global accesses are whole rows: a thread reading or
+// writing its own row touches 32 lines in every instruction of its warp (4000
+// cycles for a block's rows).
 //
 // Prefixes in fp8 caches run as fp16: TMA brings raw tiles to a ring of their
-// own, and the warps that look on otherwise convert them into the stages (exact), each row of q is scaled by a power of two into [1, 2) first (exact
-// but for elements 2^14 below the row's largest) and the power goes into the
-// row's score scale.
+// own, and six warps (five at D = 64) convert them into the stages, exactly (two
+// warps took 3.5 us to a pair of tiles, where the products and exponentials
+// take 2). Each row of q is scaled by a power of two into [1, 2) first (exact but
+// for elements 2^14 below the row's largest) and the power goes into the row's
+// score scale.
 //
 // The running maximum of a row follows the true one only when that has grown
 // by more than 2^8 (kSlack): p then stays below 256, exact enough in 16 bits

@@ -21,7 +21,7 @@
 // call and kept as 2 bits in a register. Lanes whose entries lie in one section,
 // and all lanes of a token whose positions agree (text), read one table row
 // with 16-byte loads; the others pick each entry from its axis's row (8191
-// tokens, 64/8 heads: 72 us against 71).
+// tokens, 64/8 heads: 65.0 us against 64.5).
 #include <cuda_fp8.h>
 
 #include <algorithm>
