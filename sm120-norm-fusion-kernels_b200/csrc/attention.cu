@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cmath>
 
 namespace sm120n {
 namespace {
@@ -95,6 +96,36 @@ int check_decode_sizes(const sm120s_decode_args* a) {
   return SM120N_OK;
 }
 
+// Parts of a prefix on tensor memory, at most `most` (a block to an SM). More of
+// them are shorter, but each takes SMs from the own tokens' pass for its start,
+// and is read again when the parts are joined: step * tiles / parts + cost *
+// parts is least at the root below. A few parts fewer are taken where that
+// leaves half of the SMs to the own tokens, whose blocks, two to an SM, then run
+// in two waves beside the prefix. Measured (graph, 61 requests of 1-600 own
+// tokens, 32/8 heads, D = 128, bf16), `most` against this: prefixes of 2048
+// tokens 43.5 us (16 parts) against 36.5 (4), 8192 52 (18) against 42 (8),
+// 16384 61 (18) against 50 (9); with 1-32 own tokens and 8192 33.6 against 30.7.
+// Where a part has many blocks, there are few parts, and all of them won: 300
+// requests, 1024 tokens, 82 us with 3 parts against 87.6 with 2; 128 requests, D =
+// 64, 4096 tokens, 62.7 with 9 against 67.5 with 4.
+int prefix_parts(const sm120s_decode_args& a, int most, int64_t blocks, int64_t tiles,
+                 int64_t triples, int sm_count) {
+  if (12 * blocks > sm_count) return most;
+  const double step = (a.cache_dtype == SM120N_CACHE_FP8_E4M3 ? 2.2 : 1.8) *  // us, 128 keys
+                      (a.head_dim == 64 ? 0.72 : 1.0);
+  const double start = 16.0, join_bytes = 1.5e6;  // us of an SM; bytes in a us
+  const int own_room = own_blocks_per_sm(static_cast<int>(a.head_dim)) * sm_count;
+  const double wanted = std::min(1.0, static_cast<double>(triples) / own_room);  // of the SMs
+  const double cost = start * blocks / sm_count * wanted +
+                      static_cast<double>(a.batch) * a.query_heads * a.head_dim * 4 / join_bytes;
+  int64_t parts = std::min<int64_t>(most, std::llround(std::sqrt(step * tiles / cost)));
+  const int64_t beside = sm_count / 2 / blocks;
+  if (triples >= own_room && parts > beside && 10 * beside >= 7 * parts) parts = beside;
+  parts = std::max<int64_t>(parts, 1);
+  const int64_t steps = (tiles + parts - 1) / parts;
+  return static_cast<int>((tiles + steps - 1) / steps);  // no more than take as many steps
+}
+
 int plan_decode(const sm120s_decode_args& a, Plan* plan) {
   DeviceInfo dev;
   const int rc = current_device_info(&dev);
@@ -113,8 +144,9 @@ int plan_decode(const sm120s_decode_args& a, Plan* plan) {
     const int64_t row_tiles = (a.batch * group + tile_rows - 1) / tile_rows;
     const int64_t tiles = (a.prefix_blocks_count * a.block_size + tile_keys - 1) / tile_keys;
     const int64_t blocks = std::max<int64_t>(1, row_tiles * a.key_heads);
-    plan->prefix_splits = static_cast<int>(std::max<int64_t>(
+    const int most = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>(tiles, (tc ? 1 : 2) * dev.sm_count / blocks)));
+    plan->prefix_splits = tc ? prefix_parts(a, most, blocks, tiles, triples, dev.sm_count) : most;
   }
   size_t at = (static_cast<size_t>(a.batch + 1) * sizeof(int64_t) + 15) / 16 * 16;
   const size_t own_rows = static_cast<size_t>(triples + plan->own_grid) * 16;
