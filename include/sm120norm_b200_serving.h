@@ -179,7 +179,8 @@ SM120N_API int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
  * zeros where there is no key. Blocks outside [0, num_blocks) hold no keys. The
  * prefix is read once for all requests. out may not overlap query.
  * query, out [batch, query_heads, head_dim], heads adjacent; caches as
- * sm120n_qk_cache_args (one shape and stride for both), rows 16-byte aligned;
+ * sm120n_qk_cache_args (one shape and stride for both), rows 16-byte aligned and
+ * at least head_dim elements apart in every dimension;
  * fp8 caches stand for code * k_scale[0] / code * v_scale[0]. dtype f16 or bf16.
  * workspace: sm120s_paged_decode_workspace bytes, 16-byte aligned, written and
  * read by this call alone: calls that may run at the same time, or graphs that

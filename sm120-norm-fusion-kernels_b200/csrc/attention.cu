@@ -115,7 +115,8 @@ int prefix_parts(const sm120s_decode_args& a, int most, int64_t blocks, int64_t 
                       (a.head_dim == 64 ? 0.72 : 1.0);
   const double start = 16.0, join_bytes = 1.5e6;  // us of an SM; bytes in a us
   const int own_room = own_blocks_per_sm(static_cast<int>(a.head_dim)) * sm_count;
-  const double wanted = std::min(1.0, static_cast<double>(triples) / own_room);  // of the SMs
+  const double wanted =  // of the SMs
+      std::min(1.0, static_cast<double>(std::max<int64_t>(triples, 1)) / own_room);
   const double cost = start * blocks / sm_count * wanted +
                       static_cast<double>(a.batch) * a.query_heads * a.head_dim * 4 / join_bytes;
   int64_t parts = std::min<int64_t>(most, std::llround(std::sqrt(step * tiles / cost)));
@@ -256,6 +257,12 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
   if (!aligned16(in.key_cache) || !aligned16(in.value_cache) || in.cache_block_stride % pack != 0 ||
       in.cache_slot_stride % pack != 0 || in.cache_head_stride % pack != 0) {
     return fail(SM120N_ERR_INVALID_ARGUMENT, "cache rows must be 16-byte aligned");
+  }
+  if ((in.num_blocks > 1 && in.cache_block_stride < in.head_dim) ||
+      (in.block_size > 1 && in.cache_slot_stride < in.head_dim) ||
+      (in.key_heads > 1 && in.cache_head_stride < in.head_dim)) {
+    return fail(SM120N_ERR_INVALID_ARGUMENT,
+                "cache strides must cover head_dim elements (rows may not overlap)");
   }
   Plan plan;
   rc = plan_decode(in, &plan);

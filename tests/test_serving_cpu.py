@@ -198,3 +198,10 @@ def test_plan_reference_hands_out_whole_requests_in_order():
 def test_sections_of_the_rotation():
     assert ref.axis_of([1, 2, 3], False) == [0, 1, 1, 2, 2, 2]
     assert ref.axis_of([4, 1, 1], True) == [0, 1, 2, 0, 0, 0]
+
+
+@pytest.mark.parametrize("stride", ["cache_block_stride", "cache_slot_stride", "cache_head_stride"])
+@pytest.mark.parametrize("value", [0, 8, -256])
+def test_caches_whose_rows_overlap_are_refused(stride, value):
+    with pytest.raises(capi.CApiError, match="may not overlap|non-negative"):
+        decode(**{stride: value})
