@@ -863,7 +863,9 @@ int run_prompt_tiles(const PromptArgs& a, cudaStream_t stream) {
   for (int i = 0; i < 2; ++i) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.key_heads) * D,
                                 static_cast<cuuint64_t>(a.tokens)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(i ? a.value_stride : a.key_stride) * 2};
+    // one token has no stride of its own
+    const int64_t row = a.tokens > 1 ? (i ? a.value_stride : a.key_stride) : int64_t{a.key_heads} * D;
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row) * 2};
     const cuuint32_t box[2] = {64, kTileKeys};
     const int rc = encode_tensor_map(&maps[i], i ? a.value : a.key, tensor_map_type<T>(), 2, dims,
                                      strides, box, 128);

@@ -435,6 +435,20 @@ def test_large_blocks():
         Decode([700, 129, 64, 1000], 0, d=d, block_size=1024, layout="HND", cache="fp8", seed=15).check()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_one_token_needs_no_stride(d):
+    q, k, v = (torch.randn(1, h, d, device=DEV, dtype=torch.bfloat16) for h in (4, 2, 2))
+    out = torch.zeros_like(q)
+    start = ints([0, 1])
+    serving_capi.prompt_attention(serving_capi.PromptArgs(
+        dtype=serving_capi.BF16, tokens=1, sequences=1, query_heads=4, key_heads=2, head_dim=d,
+        query=q.data_ptr(), query_token_stride=4 * d + 1, key=k.data_ptr(),
+        key_token_stride=2 * d + 3, value=v.data_ptr(), value_token_stride=2 * d + 5,
+        out=out.data_ptr(), out_token_stride=4 * d + 7, query_start=start.data_ptr(), scale=0.1),
+        torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(out, v.repeat_interleave(2, dim=1))
+
+
 def test_no_wait_ran_out():
     torch.cuda.synchronize()
     assert serving_capi.device_faults() == 0
