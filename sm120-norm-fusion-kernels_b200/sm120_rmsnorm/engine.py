@@ -125,28 +125,52 @@ class PagedSteps:
 
     ``context_lens`` is what the cache holds for each request and follows every
     :meth:`plan`; ``query_start``, ``positions`` and ``slot_mapping`` are those of the
-    step planned last. ``prefix_blocks`` blocks, taken off the pool here, are
-    the first of every request's row; a request that begins behind them starts
-    with ``context_lens`` at their length.
+    step planned last.
+
+    ``prefix_blocks`` blocks, taken off the pool here, are the first of every
+    request's row, and every request begins behind them: its ``context_lens``
+    starts at their tokens and returns there. :meth:`prefix_writer` plans the
+    prompt that fills them. Requests that do not share the prefix stand in a
+    second ``PagedSteps`` over the same blocks: ``pool`` is then the first one.
     """
 
     def __init__(self, requests: int, num_blocks: int, max_blocks: int, max_tokens: int, device,
-                 block_size: int = 16, prefix_blocks: int = 0):
+                 block_size: int = 16, prefix_blocks: int = 0, pool: PagedSteps | None = None):
         def ints(*shape, dtype=torch.int32):
             return torch.zeros(*shape, device=device, dtype=dtype)
 
+        if not 0 <= prefix_blocks <= min(num_blocks, max_blocks):
+            raise ValueError("prefix_blocks must be in [0, num_blocks] and fit a row of max_blocks")
+        if pool is not None and (prefix_blocks or pool.free_blocks.numel() != num_blocks
+                                 or pool.block_size != block_size):
+            raise ValueError("a batch over another one's pool has its num_blocks and block_size, "
+                             "and no prefix_blocks of its own")
         self.block_size = block_size
-        self.free_blocks = torch.arange(num_blocks - 1, -1, -1, device=device, dtype=torch.int32)
-        self.free_count = torch.full((1,), num_blocks - prefix_blocks, device=device,
-                                     dtype=torch.int32)
+        if pool is None:
+            self.free_blocks = torch.arange(num_blocks - 1, -1, -1, device=device, dtype=torch.int32)
+            self.free_count = torch.full((1,), num_blocks - prefix_blocks, device=device,
+                                         dtype=torch.int32)
+        else:
+            self.free_blocks, self.free_count = pool.free_blocks, pool.free_count
         # the top of the stack, block 0 first
         self.prefix = self.free_blocks[num_blocks - prefix_blocks:].flip(0).clone()
         self.block_table = torch.full((requests, max_blocks), -1, device=device, dtype=torch.int32)
         self.block_table[:, :prefix_blocks] = self.prefix
-        self.context_lens = ints(requests)
+        self.context_lens = ints(requests).fill_(prefix_blocks * block_size)
         self.query_start = ints(requests + 1)
         self.positions = ints(max_tokens, dtype=torch.int64)
         self.slot_mapping = ints(max_tokens)
+
+    def prefix_writer(self) -> PagedSteps:
+        """A batch of one request whose blocks are those of the prefix: plan it with
+        as many tokens as they hold and run :meth:`Qwen3Attention.prompts` on it in
+        every layer, before the first request is decoded."""
+        blocks = self.prefix.numel()
+        writer = PagedSteps(1, self.free_blocks.numel(), blocks, blocks * self.block_size,
+                            self.free_blocks.device, self.block_size)
+        writer.free_blocks[:blocks] = self.prefix.flip(0)
+        writer.free_count.fill_(blocks)
+        return writer
 
     def plan(self, query_lens: torch.Tensor) -> None:
         """The next step, with ``query_lens`` (int32 [requests]) new tokens."""
@@ -156,10 +180,10 @@ class PagedSteps:
 
     def release(self, finished: torch.Tensor) -> None:
         """Gives the blocks of the requests in ``finished`` (bool [requests]) back,
-        all but the shared ones, and sets their lengths to zero."""
+        all but the shared ones, and sets their lengths to those of the prefix."""
         serving.release_blocks_(self.context_lens, finished, self.block_table, self.free_blocks,
                                 self.free_count, self.block_size, self.prefix.numel())
-        self.context_lens.masked_fill_(finished, 0)
+        self.context_lens.masked_fill_(finished, self.prefix.numel() * self.block_size)
 
 
 class Qwen3Attention:
@@ -191,7 +215,11 @@ class Qwen3Attention:
     def prompts(self, hidden: torch.Tensor, residual: torch.Tensor, steps: PagedSteps,
                 positions: torch.Tensor | None = None, qkv: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-        """Whole prompts, packed as ``steps`` planned them from empty contexts."""
+        """Whole prompts, packed as ``steps`` planned them from empty contexts: their
+        tokens see one another and nothing in the cache. So a batch with a prefix
+        has none; its prompts go through :meth:`decode`, a token a step."""
+        if steps.prefix.numel():
+            raise ValueError("prompts behind a shared prefix do not see it: decode their tokens")
         q, k, v = self._queries(hidden, residual, steps, positions, qkv)
         out = torch.zeros(q.shape, device=q.device, dtype=q.dtype) if out is None else out
         serving.prompt_attention(out, q, k, v, steps.query_start)

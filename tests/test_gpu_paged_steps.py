@@ -1,0 +1,125 @@
+"""Batches that live through several requests (engine.PagedSteps and
+engine.Qwen3Attention): what a decode step returns must be the 64-bit attention
+over the keys and values that the request's own tokens had, kept beside the cache
+as they were computed, within the bounds of tests/serving_reference.py."""
+import pytest
+import torch
+
+import serving_reference as ref
+from sm120_rmsnorm.engine import (PagedSteps, Qwen3Attention, Qwen3AttentionPrologue,
+                                  Qwen3AttentionShape, rope_cos_sin_cache)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SHAPE = Qwen3AttentionShape(hidden=512, query_heads=8, key_heads=2, max_positions=4096)
+BLOCKS = 60
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def bools(values):
+    return torch.tensor(values, dtype=torch.bool, device=DEV)
+
+
+class Layer:
+    """A layer with a cache, and each request's keys and values in its own order."""
+
+    def __init__(self, seed):
+        self.g = torch.Generator(device=DEV).manual_seed(seed)
+        caches = [torch.zeros(BLOCKS, 16, SHAPE.key_heads, SHAPE.head_dim, device=DEV,
+                              dtype=torch.bfloat16) for _ in "kv"]
+        self.attention = Qwen3Attention(Qwen3AttentionPrologue(SHAPE, DEV, generator=self.g),
+                                        *caches, rope_cos_sin_cache(SHAPE, DEV))
+        self.seen = {}  # of a request: keys, values
+
+    def rows(self, n):
+        return [torch.randn(n, SHAPE.hidden, device=DEV, generator=self.g).to(torch.bfloat16)
+                for _ in "hr"]
+
+    def qkv(self, n):
+        return torch.empty(n, SHAPE.qkv_width, device=DEV, dtype=torch.bfloat16)
+
+    def remember(self, name, k, v):
+        old = self.seen.get(name)
+        self.seen[name] = (k.clone(), v.clone()) if old is None else \
+            (torch.cat((old[0], k)), torch.cat((old[1], v)))
+
+    def prompt(self, steps, lens, names):
+        """A step of whole prompts, named row by row."""
+        steps.plan(ints(lens))
+        n = sum(lens)
+        qkv = self.qkv(n)
+        out = self.attention.prompts(*self.rows(n), steps, qkv=qkv)
+        q, k, v = self.attention.prologue.split(qkv)
+        starts = steps.query_start.tolist()
+        want, bound = ref.prompt(q, k, v, starts)
+        assert ((out.double() - want).abs() <= bound).all()
+        for name, a, b in zip(names, starts[:-1], starts[1:]):
+            self.remember(name, k[a:b], v[a:b])
+
+    def decode(self, steps, names):
+        """A step of one token for every row whose name is not None."""
+        steps.plan(ints([int(name is not None) for name in names]))
+        qkv = self.qkv(len(names))
+        out = self.attention.decode(*self.rows(len(names)), steps, qkv=qkv)
+        q, k, v = self.attention.prologue.split(qkv)
+        for r, name in enumerate(names):
+            if name is None:
+                assert (out[r] == 0).all()
+                continue
+            self.remember(name, k[r:r + 1], v[r:r + 1])
+            keys, values = (x.double() for x in self.seen[name])
+            for h in range(SHAPE.key_heads):
+                heads = slice(4 * h, 4 * h + 4)
+                want, bound = ref.attention_row_block(
+                    q[r, heads].double(), keys[:, h], values[:, h], SHAPE.head_dim ** -0.5,
+                    torch.bfloat16, torch.bfloat16)
+                assert ((out[r, heads].double() - want).abs() <= bound).all(), (r, name)
+
+
+def begin_behind(layer, prefix_name, *names):
+    for name in names:
+        layer.seen[name] = layer.seen[prefix_name]
+
+
+def test_requests_behind_a_prefix_end_and_make_room():
+    layer = Layer(1)
+    steps = PagedSteps(3, BLOCKS, 20, 3, DEV, prefix_blocks=2)
+    layer.prompt(steps.prefix_writer(), [32], ["prefix"])
+    pool = int(steps.free_count)
+    assert pool == BLOCKS - 2
+    begin_behind(layer, "prefix", "a", "b", "c", "d", "e", "f", "g")
+    for _ in range(35):  # past two blocks of their own
+        layer.decode(steps, ["a", "b", "c"])
+    assert int(steps.free_count) == pool - 9
+    steps.release(bools([False, True, False]))
+    assert int(steps.free_count) == pool - 6
+    assert steps.context_lens.tolist() == [67, 32, 67]
+    for _ in range(40):  # a second request in the row that was given back
+        layer.decode(steps, ["a", "d", "c"])
+    steps.release(bools([True, True, True]))
+    assert int(steps.free_count) == pool
+    assert steps.context_lens.tolist() == [32] * 3
+    for _ in range(3):
+        layer.decode(steps, ["e", "f", "g"])
+
+
+def test_a_batch_without_the_prefix_over_the_same_pool():
+    layer = Layer(2)
+    sharing = PagedSteps(2, BLOCKS, 20, 2, DEV, prefix_blocks=3)
+    alone = PagedSteps(2, BLOCKS, 20, 90, DEV, pool=sharing)
+    layer.prompt(sharing.prefix_writer(), [48], ["prefix"])
+    begin_behind(layer, "prefix", "a", "b", "c")
+    for names in (("p", "q"), ("r", "s")):
+        layer.prompt(alone, [70, 20], names)
+        for _ in range(20):
+            layer.decode(sharing, ["a", "b"])
+            layer.decode(alone, list(names))
+        alone.release(bools([True, True]))
+    sharing.release(bools([True, False]))
+    for _ in range(5):
+        layer.decode(sharing, ["c", "b"])
+    sharing.release(bools([True, True]))
+    assert int(sharing.free_count) == BLOCKS - 3
