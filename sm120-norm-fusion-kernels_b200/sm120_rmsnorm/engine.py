@@ -125,7 +125,10 @@ class PagedSteps:
 
     ``context_lens`` is what the cache holds for each request and follows every
     :meth:`plan`; ``query_start``, ``positions`` and ``slot_mapping`` are those of the
-    step planned last.
+    step planned last, packed request after request. ``row_positions``, ``row_slots``
+    and ``row_lens`` are the same step as decode runs it, entry r for request r:
+    its first token's position and slot and its length with the step, or -1, -1 and 0
+    for a request without a token or without room for it (:attr:`unserved`).
 
     ``prefix_blocks`` blocks, taken off the pool here, are the first of every
     request's row, and every request begins behind them: its ``context_lens``
@@ -159,7 +162,13 @@ class PagedSteps:
         self.context_lens = ints(requests).fill_(prefix_blocks * block_size)
         self.query_start = ints(requests + 1)
         self.positions = ints(max_tokens, dtype=torch.int64)
-        self.slot_mapping = ints(max_tokens)
+        # and one entry more, for requests without a token
+        self._slots = ints(max_tokens + 1).fill_(-1)
+        self.slot_mapping = self._slots[:max_tokens]
+        self.row_positions = ints(requests, dtype=torch.int64)
+        self.row_slots = ints(requests)
+        self.row_lens = ints(requests)
+        self._asked = ints(requests, dtype=torch.bool)
 
     def prefix_writer(self) -> PagedSteps:
         """A batch of one request whose blocks are those of the prefix: plan it with
@@ -177,6 +186,17 @@ class PagedSteps:
         serving.plan_step_(self.context_lens, query_lens, self.block_table, self.free_blocks,
                            self.free_count, self.block_size, self.query_start, self.context_lens,
                            self.positions, self.slot_mapping)
+        torch.gt(query_lens, 0, out=self._asked)
+        first = torch.where(self._asked, self.query_start[:-1], self.slot_mapping.numel())
+        torch.index_select(self._slots, 0, first, out=self.row_slots)
+        torch.mul(self.context_lens, self.row_slots >= 0, out=self.row_lens)
+        torch.sub(self.row_lens, 1, out=self.row_positions)
+
+    @property
+    def unserved(self) -> torch.Tensor:
+        """Requests (bool [requests], on the GPU) that had tokens in the step planned
+        last and got no place for them: their lengths are as before the step."""
+        return self._asked & (self.row_slots < 0)
 
     def release(self, finished: torch.Tensor) -> None:
         """Gives the blocks of the requests in ``finished`` (bool [requests]) back,
@@ -190,7 +210,7 @@ class Qwen3Attention:
     """A layer's attention on a planned step: prologue, K and V into the paged
     cache, attention. Returns [tokens, query_heads, head_dim], the input of the
     output projection. ``positions`` default to the plan's; [3, tokens] for
-    images and video."""
+    images and video, packed for prompts and one column per request for decode."""
 
     def __init__(self, prologue: Qwen3AttentionPrologue, key_cache: torch.Tensor,
                  value_cache: torch.Tensor, cos_sin_cache: torch.Tensor, k_scale=None,
@@ -201,16 +221,13 @@ class Qwen3Attention:
         self.k_scale, self.v_scale = k_scale, v_scale
         self.kv_cache_layout = kv_cache_layout
 
-    def _queries(self, hidden, residual, steps, positions, qkv):
-        tokens = hidden.shape[0]
+    def _queries(self, hidden, residual, positions, slots, qkv):
         if qkv is None:
-            qkv = torch.empty(tokens, self.prologue.shape.qkv_width, device=hidden.device,
-                              dtype=hidden.dtype)
-        positions = steps.positions[:tokens] if positions is None else positions
+            qkv = torch.empty(hidden.shape[0], self.prologue.shape.qkv_width,
+                              device=hidden.device, dtype=hidden.dtype)
         return self.prologue.forward(hidden, residual, positions, self.cos_sin_cache,
-                                     self.key_cache, self.value_cache,
-                                     steps.slot_mapping[:tokens], qkv, self.k_scale, self.v_scale,
-                                     self.kv_cache_layout)
+                                     self.key_cache, self.value_cache, slots, qkv, self.k_scale,
+                                     self.v_scale, self.kv_cache_layout)
 
     def prompts(self, hidden: torch.Tensor, residual: torch.Tensor, steps: PagedSteps,
                 positions: torch.Tensor | None = None, qkv: torch.Tensor | None = None,
@@ -220,7 +237,9 @@ class Qwen3Attention:
         has none; its prompts go through :meth:`decode`, a token a step."""
         if steps.prefix.numel():
             raise ValueError("prompts behind a shared prefix do not see it: decode their tokens")
-        q, k, v = self._queries(hidden, residual, steps, positions, qkv)
+        tokens = hidden.shape[0]
+        positions = steps.positions[:tokens] if positions is None else positions
+        q, k, v = self._queries(hidden, residual, positions, steps.slot_mapping[:tokens], qkv)
         out = torch.zeros(q.shape, device=q.device, dtype=q.dtype) if out is None else out
         serving.prompt_attention(out, q, k, v, steps.query_start)
         return out
@@ -228,11 +247,17 @@ class Qwen3Attention:
     def decode(self, hidden: torch.Tensor, residual: torch.Tensor, steps: PagedSteps,
                positions: torch.Tensor | None = None, qkv: torch.Tensor | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
-        """One token for every request, as ``steps`` planned them."""
-        q, _, _ = self._queries(hidden, residual, steps, positions, qkv)
+        """At most one token for every request, as ``steps`` planned them; row r is
+        request r's. Requests without a token, and those without room for it
+        (``steps.unserved``), store nothing, and their rows come out as zeros."""
+        if hidden.shape[0] != steps.row_lens.numel():
+            raise ValueError(f"decode takes one row per request ({steps.row_lens.numel()}), with or "
+                             f"without a token (got {hidden.shape[0]})")
+        positions = steps.row_positions if positions is None else positions
+        q, _, _ = self._queries(hidden, residual, positions, steps.row_slots, qkv)
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
         serving.paged_decode_attention(out, q, self.key_cache, self.value_cache,
-                                       steps.block_table, steps.context_lens, steps.prefix,
+                                       steps.block_table, steps.row_lens, steps.prefix,
                                        self.k_scale, self.v_scale, self.kv_cache_layout)
         return out
 

@@ -123,3 +123,76 @@ def test_a_batch_without_the_prefix_over_the_same_pool():
         layer.decode(sharing, ["c", "b"])
     sharing.release(bools([True, True]))
     assert int(sharing.free_count) == BLOCKS - 3
+
+
+@pytest.mark.parametrize("prefix", [0, 2])
+def test_idle_rows_keep_every_request_with_its_own_tokens(prefix):
+    layer = Layer(3)
+    steps = PagedSteps(4, BLOCKS, 20, 90, DEV, prefix_blocks=prefix)
+    if prefix:
+        layer.prompt(steps.prefix_writer(), [32], ["prefix"])
+        begin_behind(layer, "prefix", "a", "b", "c", "d", "e")
+    else:
+        layer.prompt(steps, [40, 3, 17, 30], ["a", "b", "c", "d"])
+    pool = int(steps.free_count)
+    layer.decode(steps, ["a", "b", "c", "d"])
+    steps.release(bools([False, True, False, False]))
+    for _ in range(20):  # a middle row without a request takes no block
+        layer.decode(steps, ["a", None, "c", "d"])
+    assert steps.context_lens[1] == prefix * 16
+    layer.decode(steps, [None, "e", None, None])
+    layer.decode(steps, [None, None, None, None])
+    for _ in range(17):
+        layer.decode(steps, ["a", "e", None, "d"])
+    steps.release(bools([True, True, True, True]))
+    assert int(steps.free_count) == (pool if prefix else BLOCKS)
+
+
+def test_a_request_without_room_comes_out_as_zeros():
+    layer = Layer(4)
+    steps = PagedSteps(3, BLOCKS, 20, 3, DEV)
+    steps.free_count.fill_(2)
+    layer.decode(steps, ["a", "b", None])
+    steps.plan(ints([1, 0, 1]))
+    out = layer.attention.decode(*layer.rows(3), steps)
+    assert steps.unserved.tolist() == [False, False, True]
+    assert (out[1:] == 0).all() and out[0].abs().max() > 0
+
+
+def test_a_captured_step_with_rows_that_come_and_go():
+    layer = Layer(5)
+    steps = PagedSteps(3, BLOCKS, 20, 3, DEV)
+    query = ints([1, 1, 1])
+    hidden, residual = layer.rows(3)
+    qkv = layer.qkv(3)
+    out = torch.empty(3, 8, 128, device=DEV, dtype=torch.bfloat16)
+
+    def step():
+        steps.plan(query)
+        layer.attention.decode(hidden, residual, steps, qkv=qkv, out=out)
+
+    step()
+    torch.cuda.synchronize()
+    q, k, v = layer.attention.prologue.split(qkv)
+    for r in range(3):
+        layer.remember(r, k[r:r + 1], v[r:r + 1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(30):
+        there = [int((i + r) % 3 > 0) for r in range(3)]
+        query.copy_(ints(there))
+        for buffer, values in zip((hidden, residual), layer.rows(3)):
+            buffer.copy_(values)
+        graph.replay()
+        for r in range(3):
+            if not there[r]:
+                assert (out[r] == 0).all()
+                continue
+            layer.remember(r, k[r:r + 1], v[r:r + 1])
+            keys, values = (x.double() for x in layer.seen[r])
+            for h in range(2):
+                want, bound = ref.attention_row_block(
+                    q[r, 4 * h:4 * h + 4].double(), keys[:, h], values[:, h], 128 ** -0.5,
+                    torch.bfloat16, torch.bfloat16)
+                assert ((out[r, 4 * h:4 * h + 4].double() - want).abs() <= bound).all()

@@ -106,6 +106,37 @@ def test_rows_that_do_not_share_the_prefix_stand_in_a_batch_over_the_same_pool()
     assert int(sharing.free_count) == 18
 
 
+def rows_of(steps, query):
+    steps.plan(ints(query))
+    lens = steps.row_lens.tolist()
+    assert steps.row_positions.tolist() == [n - 1 for n in lens]
+    return steps.row_slots.tolist(), lens, steps.unserved.nonzero().flatten().tolist()
+
+
+def test_decode_rows_are_requests_whoever_has_a_token():
+    steps = steps_of(requests=4, blocks=4, tokens=4)
+    assert rows_of(steps, [1, 1, 0, 1]) == ([0, 16, -1, 32], [1, 1, 0, 1], [])
+    assert rows_of(steps, [0, 1, 0, 1]) == ([-1, 17, -1, 33], [0, 2, 0, 2], [])
+    steps.release(torch.tensor([False, True, False, False]))
+    assert rows_of(steps, [1, 0, 1, 1]) == ([1, -1, 16, 34], [2, 0, 1, 3], [])
+    # block 3 alone is left, for the second row; the first request waits
+    steps.release(torch.tensor([True, False, False, False]))
+    steps.free_count.fill_(1)
+    assert rows_of(steps, [0, 1, 1, 0]) == ([-1, 48, 17, -1], [0, 1, 2, 0], [])
+    assert rows_of(steps, [1, 1, 0, 1]) == ([-1, 49, -1, 35], [0, 2, 0, 4], [0])
+    assert steps.context_lens.tolist() == [0, 2, 2, 4]
+
+
+def test_tokens_past_the_buffer_are_unserved():
+    steps = steps_of(requests=3, blocks=9, tokens=2)
+    assert rows_of(steps, [1, 1, 1]) == ([0, 16, -1], [1, 1, 0], [2])
+
+
+def test_decode_wants_a_row_per_request():
+    with pytest.raises(ValueError, match="one row per request"):
+        engine.Qwen3Attention(None, None, None, None).decode(torch.zeros(1, 8), None, steps_of())
+
+
 def test_prompts_behind_a_prefix_are_refused():
     """Prompt attention sees the packed tokens alone, not the prefix."""
     with pytest.raises(ValueError, match="prefix"):
