@@ -99,8 +99,9 @@ SM120N_API int sm120s_release_blocks(const int32_t* seq_lens, const uint8_t* fin
  * sections add up to rotary_dim / 2. One after another: the first sections[0]
  * pairs turn by axis 0, the next sections[1] by axis 1, and so on. Interleaved:
  * pair i turns by axis k = i mod axes if k > 0 and i < axes * sections[k], else
- * by axis 0. query_out / key_out: NULL for in place, or dense heads at these
- * token strides (elements), not overlapping the inputs otherwise.
+ * by axis 0. query_out / key_out: NULL for in place, or adjacent heads at these
+ * token strides (elements): the input's own rows, or rows that share nothing with
+ * query, key, value, the caches and one another.
  */
 typedef struct sm120s_mrope_args {
   uint32_t struct_size; /* sizeof(sm120s_mrope_args) */
@@ -177,7 +178,7 @@ SM120N_API int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
  *   out[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_b . k_j)
  * fp32 scores, sums and values, p rounded to 16 bits for the second product;
  * zeros where there is no key. Blocks outside [0, num_blocks) hold no keys. The
- * prefix is read once for all requests. out may not overlap query.
+ * prefix is read once for all requests. out may not overlap query or a cache.
  * query, out [batch, query_heads, head_dim], heads adjacent; caches as
  * sm120n_qk_cache_args (one shape and stride for both), rows 16-byte aligned and
  * at least head_dim elements apart in every dimension;

@@ -5,7 +5,8 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cmath>
+
+#include "row_overlap.h"
 
 namespace sm120n {
 namespace {
@@ -42,6 +43,17 @@ int check_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int
     return fail(SM120N_ERR_INVALID_ARGUMENT, "%s rows must be 16-byte aligned", name);
   }
   return SM120N_OK;
+}
+
+// Rows of `heads` heads at every token, in 16-bit elements.
+RowSet head_rows(const void* p, int64_t stride, int64_t tokens, int64_t heads, int64_t head_dim) {
+  return row_set(p, tokens, stride, heads * head_dim, 2);
+}
+
+int check_apart(const RowSet& out, const RowSet& in, const char* name) {
+  return rows_overlap(out, in)
+             ? fail(SM120N_ERR_INVALID_ARGUMENT, "out may not overlap %s", name)
+             : SM120N_OK;
 }
 
 // Whether the prefix runs on tensor memory: 256 rows and 128 keys to a tile
@@ -196,6 +208,11 @@ extern "C" int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
   if (rc == SM120N_OK) rc = check_rows(in.value, in.value_token_stride, in.tokens, in.key_heads, in.head_dim, "value");
   if (rc == SM120N_OK) rc = check_rows(in.out, in.out_token_stride, in.tokens, in.query_heads, in.head_dim, "out");
   if (rc != SM120N_OK) return rc;
+  const RowSet out = head_rows(in.out, in.out_token_stride, in.tokens, in.query_heads, in.head_dim);
+  rc = check_apart(out, head_rows(in.query, in.query_token_stride, in.tokens, in.query_heads, in.head_dim), "query");
+  if (rc == SM120N_OK) rc = check_apart(out, head_rows(in.key, in.key_token_stride, in.tokens, in.key_heads, in.head_dim), "key");
+  if (rc == SM120N_OK) rc = check_apart(out, head_rows(in.value, in.value_token_stride, in.tokens, in.key_heads, in.head_dim), "value");
+  if (rc != SM120N_OK) return rc;
   PromptArgs a{};
   a.query = in.query;
   a.out = in.out;
@@ -264,6 +281,15 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
     return fail(SM120N_ERR_INVALID_ARGUMENT,
                 "cache strides must cover head_dim elements (rows may not overlap)");
   }
+  const RowSet out = head_rows(in.out, in.out_token_stride, in.batch, in.query_heads, in.head_dim);
+  rc = check_apart(out, head_rows(in.query, in.query_token_stride, in.batch, in.query_heads, in.head_dim), "query");
+  // a cache from its first to its last element
+  const int64_t elems = in.num_blocks < 1 ? 0 : (in.num_blocks - 1) * in.cache_block_stride +
+                                                    (in.block_size - 1) * in.cache_slot_stride +
+                                                    (in.key_heads - 1) * in.cache_head_stride + in.head_dim;
+  if (rc == SM120N_OK) rc = check_apart(out, row_set(in.key_cache, 1, elems, elems, fp8 ? 1 : 2), "key_cache");
+  if (rc == SM120N_OK) rc = check_apart(out, row_set(in.value_cache, 1, elems, elems, fp8 ? 1 : 2), "value_cache");
+  if (rc != SM120N_OK) return rc;
   Plan plan;
   rc = plan_decode(in, &plan);
   if (rc != SM120N_OK) return rc;

@@ -28,6 +28,7 @@
 
 #include "cache_args.h"
 #include "head_utils.cuh"
+#include "row_overlap.h"
 #include "runtime.h"
 #include "sm120norm_b200_serving.h"
 
@@ -447,6 +448,46 @@ int check_mrope_args(const sm120n_qk_cache_args& in, const sm120s_mrope_args* m)
   return SM120N_OK;
 }
 
+// What is written may overlap nothing that another head reads or writes: its own
+// input only as the same rows (in place).
+int check_mrope_overlaps(const sm120n_qk_cache_args& in, const sm120s_mrope_args& m, int cache_kind) {
+  const int64_t elem = dtype_size(in.dtype);
+  auto rows = [&](const void* p, int64_t stride, int64_t heads) {
+    return row_set(p, in.tokens, stride, heads * in.head_dim, elem);
+  };
+  const bool stores = cache_kind != kNoCache && in.key_heads > 0;
+  const RowSet query = rows(in.query, in.query_token_stride, in.query_heads);
+  const RowSet key = rows(in.key, in.key_token_stride, in.key_heads);
+  const RowSet value = rows(stores ? in.value : nullptr, in.value_token_stride, in.key_heads);
+  const RowSet query_out =
+      m.query_out ? rows(m.query_out, m.query_out_token_stride, in.query_heads) : query;
+  const RowSet key_out = m.key_out ? rows(m.key_out, m.key_out_token_stride, in.key_heads) : key;
+  auto same = [](const RowSet& a, const RowSet& b) {
+    return a.data == b.data && (a.count <= 1 || a.stride == b.stride);
+  };
+  auto refuse = [](const char* out, const char* other) {
+    return fail(SM120N_ERR_INVALID_ARGUMENT, "%s may not overlap %s", out, other);
+  };
+  if (!same(query_out, query) && rows_overlap(query_out, query)) return refuse("query_out", "its input");
+  if (!same(key_out, key) && rows_overlap(key_out, key)) return refuse("key_out", "its input");
+  if (rows_overlap(query_out, key)) return refuse(m.query_out ? "query_out" : "query", "key");
+  if (rows_overlap(key_out, query)) return refuse(m.key_out ? "key_out" : "key", "query");
+  if (rows_overlap(query_out, key_out)) return refuse("query_out", "key_out");
+  if (rows_overlap(query_out, value)) return refuse(m.query_out ? "query_out" : "query", "value");
+  if (rows_overlap(key_out, value)) return refuse(m.key_out ? "key_out" : "key", "value");
+  if (!stores || in.num_blocks < 1) return SM120N_OK;
+  // a cache from its first to its last element
+  const int64_t elems = (in.num_blocks - 1) * in.cache_block_stride +
+                        (in.block_size - 1) * in.cache_slot_stride +
+                        (in.key_heads - 1) * in.cache_head_stride + in.head_dim;
+  for (const void* cache : {in.key_cache, in.value_cache}) {
+    const RowSet all = row_set(cache, 1, elems, elems, cache_kind == kFp8 ? 1 : elem);
+    if (rows_overlap(query_out, all)) return refuse(m.query_out ? "query_out" : "query", "the caches");
+    if (rows_overlap(key_out, all)) return refuse(m.key_out ? "key_out" : "key", "the caches");
+  }
+  return SM120N_OK;
+}
+
 }  // namespace
 }  // namespace sm120n
 
@@ -461,6 +502,8 @@ extern "C" int sm120s_qk_norm_mrope_cache(const sm120n_qk_cache_args* args,
   rc = check_mrope_args(*args, mrope);
   if (rc != SM120N_OK) return rc;
   if (args->tokens == 0 || args->query_heads + args->key_heads == 0) return SM120N_OK;
+  rc = check_mrope_overlaps(*args, *mrope, cache_kind);
+  if (rc != SM120N_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (args->dtype) {
     case SM120N_F32: return run_mrope_typed<float>(*args, *mrope, cache_kind, s);

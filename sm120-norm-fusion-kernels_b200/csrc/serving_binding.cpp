@@ -3,8 +3,6 @@
 // behind the C ABI, on the tensors' device and the current PyTorch stream; no
 // host synchronisation. Only paged_decode_attention allocates: its workspace,
 // anew for every call, so that no two calls or graphs share one.
-#include <ATen/MemoryOverlap.h>
-
 #include <cmath>
 
 #include "binding_utils.h"
@@ -46,13 +44,6 @@ int32_t* count_after(const torch::Tensor& count, const c10::optional<torch::Tens
   if (!out.has_value()) return count.data_ptr<int32_t>();
   check_vector(*out, torch::kInt, 1, device, "free_count_out");
   return out->data_ptr<int32_t>();
-}
-
-void check_apart(const torch::Tensor& out, const torch::Tensor& in, const char* out_name,
-                 const char* name) {
-  const auto status = at::get_overlap_status(out, in);
-  TORCH_CHECK(status != at::MemOverlapStatus::Full && status != at::MemOverlapStatus::Partial,
-              out_name, " may not overlap ", name);
 }
 
 double default_scale(c10::optional<double> scale, int64_t head_dim) {
@@ -152,9 +143,6 @@ void b200_qk_norm_mrope_cache(torch::Tensor query, torch::Tensor key,
     TORCH_CHECK(out->sizes() == in.sizes() && out->scalar_type() == in.scalar_type(), name,
                 " must have its input's shape and dtype");
     TORCH_CHECK(out->device() == in.device(), "all tensors must be on the same CUDA device");
-    if (out->data_ptr() != in.data_ptr() || out->strides() != in.strides()) {
-      check_apart(*out, in, name, "its input");
-    }
     *pointer = out->data_ptr();
     *stride = token_stride(*out);
   };
@@ -183,9 +171,6 @@ void b200_prompt_attention(torch::Tensor out, torch::Tensor query, torch::Tensor
               "all tensors must be on the same CUDA device");
   check_vector(query_start, torch::kInt, -1, device, "query_start");
   TORCH_CHECK(query_start.numel() >= 1, "query_start must have one entry per sequence and one more");
-  check_apart(out, query, "out", "query");
-  check_apart(out, key, "out", "key");
-  check_apart(out, value, "out", "value");
   sm120s_prompt_args a{};
   a.struct_size = sizeof(a);
   a.dtype = dtype_code(query);
@@ -241,7 +226,6 @@ void b200_paged_decode_attention(torch::Tensor out, torch::Tensor query, torch::
               "all tensors must be on the same CUDA device");
   check_table(block_table, query.size(0), device);
   check_vector(seq_lens, torch::kInt, query.size(0), device, "seq_lens");
-  check_apart(out, query, "out", "query");
   sm120s_decode_args a{};
   a.struct_size = sizeof(a);
   a.dtype = dtype_code(query);
