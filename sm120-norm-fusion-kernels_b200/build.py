@@ -53,6 +53,10 @@ def _headers() -> list[Path]:
     return sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
 
 
+def _binding_headers() -> list[Path]:
+    return [CSRC / "binding_utils.h", *sorted(INCLUDE.glob("*.h"))]
+
+
 def _stale(target: Path, sources: list[Path]) -> bool:
     if not target.exists():
         return True
@@ -140,7 +144,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     target = PACKAGE / f"_C{suffix}"
     sources = [CSRC / name for name in BINDING_SOURCES]
-    headers = list(INCLUDE.glob("*.h"))
+    headers = _binding_headers()
     if not force and not _stale(target, [*sources, LIBRARY, SERVING_LIBRARY, *headers]):
         return target
     compile_flags, link_flags = _torch_flags()
