@@ -47,6 +47,7 @@
 // Every wait on an mbarrier is bounded; one that runs out is counted
 // (sm120s_get_device_faults) and ends the block without results.
 #include <algorithm>
+#include <cfloat>
 
 #include "attention.h"
 #include "attention_utils.cuh"
@@ -313,6 +314,12 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
     const int live_rows = min(max(w.rows - (row - lane), 0), kWarpSize);  // of the warp
     unsigned char* rows_smem = smem + i * S::kQBytes + warp_row * 128;  // of the warp, in each box
     float scale = a.scale_log2;
+    float sign = 1.0f;  // of the keys' scale: goes into Q, so that larger products are larger scores
+    if constexpr (kFp8) {
+      const float k_scale = *a.k_scale;
+      sign = copysignf(1.0f, k_scale);
+      scale *= fabsf(k_scale);
+    }
     // Q of the warp's rows into the swizzled operand layout, whole rows at a time
     {
       constexpr int kChunks = D / 8;
@@ -343,7 +350,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
             for (int d = 1; d < kChunks; d *= 2) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, d));
             // 2^-e and 2^e with e the exponent of the row's largest, kept normal
             const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 2), 252);
-            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+            const float down = sign * __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] *= down;
             v[t] = Pack<T>::from_f32(f);
@@ -359,7 +366,9 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
                                     ((chunk % 8) ^ (r & 7)) * 16) = v[t];
         }
       }
-      if constexpr (kFp8) scale *= *a.k_scale;
+      // The scores are then zero to every bit, but the first maximum still counts
+      // as larger than none: infinity times zero would not.
+      if (kFp8 && scale < FLT_MIN) scale = FLT_MIN;
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&c.bar.q_full);
