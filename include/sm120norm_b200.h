@@ -96,7 +96,8 @@ SM120N_API int sm120n_reset_device_faults(void);
  * Diagnostic: the number of polls a kernel makes while waiting for its own
  * bulk copies (the row kernels that stage rows in shared memory) to land
  * before it gives up, records an expired wait in the fault counter and
- * leaves its rows unwritten. 0 restores the default (2^22 polls, far
+ * leaves its rows unwritten; the attention kernels of the serving library take
+ * it for every wait on an mbarrier. 0 restores the default (2^22 polls, far
  * beyond any real copy); values above it are clamped to it. Lowering it lets
  * a test make the bound expire without faulting or hanging anything: the
  * kernel still waits, with the full bound, for its copies to land before it

@@ -35,8 +35,11 @@ SM120N_API const char* sm120s_last_error(void);
 
 /*
  * Number of bounded waits that expired in these kernels on the current device
- * since the last reset. Zero in correct operation; a block that gave up left
- * its rows unwritten. Both synchronise the current device.
+ * since the last reset. Zero in correct operation. A block of prompt attention
+ * that gave up left the rows that it had not finished unwritten; in decode
+ * attention the rows that the block had a part of are NaN. The limit is
+ * sm120n_set_wait_limit's, here of every wait on an mbarrier. Both synchronise the
+ * current device.
  */
 SM120N_API int sm120s_get_device_faults(uint32_t* out_count);
 SM120N_API int sm120s_reset_device_faults(void);

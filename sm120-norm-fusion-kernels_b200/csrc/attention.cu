@@ -229,6 +229,7 @@ extern "C" int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
   a.key_heads = static_cast<int32_t>(in.key_heads);
   a.group = static_cast<int32_t>(group);
   a.scale_log2 = in.scale * kLog2e;
+  a.wait_polls = wait_poll_limit();
   const int head_dim = static_cast<int>(in.head_dim);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return head_dim <= 128 ? launch_prompt_tc(a, in.dtype, head_dim, s)
@@ -328,6 +329,7 @@ extern "C" int sm120s_paged_decode_attention(const sm120s_decode_args* args, voi
   a.own_grid = plan.own_grid;
   a.prefix_splits = plan.prefix_splits;
   a.scale_log2 = in.scale * kLog2e;
+  a.wait_polls = wait_poll_limit();
   a.tile_start = reinterpret_cast<int64_t*>(space);
   a.own_state = reinterpret_cast<float2*>(space + plan.own_state);
   a.own_values = reinterpret_cast<float*>(space + plan.own_values);

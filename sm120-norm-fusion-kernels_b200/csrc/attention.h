@@ -37,10 +37,12 @@ struct PromptArgs {
   int32_t key_heads;
   int32_t group;
   float scale_log2;  // scale * log2(e)
+  uint32_t wait_polls;  // limit of every wait on an mbarrier
 };
 
 // Partial results of a row over a part of its keys: maximum of the scaled
-// scores (base 2), sum of exp2, and the weighted values, not yet divided.
+// scores (base 2), sum of exp2, and the weighted values, not yet divided. A part
+// whose block gave up a wait has (-inf, NaN), which makes the joined row NaN.
 struct DecodeArgs {
   const void* query;
   void* out;
@@ -63,6 +65,7 @@ struct DecodeArgs {
   int32_t own_grid;       // thread blocks of the pass over each request's own tokens
   int32_t prefix_splits;  // parts of the prefix
   float scale_log2;
+  uint32_t wait_polls;  // limit of every wait on an mbarrier
   int64_t* tile_start;  // [batch + 1] key tiles of the requests before, per key head and row tile
   float2* own_state;    // [(batch * key_heads * row_tiles + own_grid) * 16] (maximum, sum)
   float* own_values;    // the same rows x head_dim

@@ -131,6 +131,15 @@ __device__ __forceinline__ void mbarrier_arrive_copies(uint64_t* bar) {
                : "memory");
 }
 
+// After an expired wait: a bounded time for the loads of the last uses of the ring
+// to land, `uses` of them begun or skipped, before shared memory goes to another block.
+template <int kStages>
+__device__ __forceinline__ void let_land(uint64_t* full, int uses) {
+  for (int u = max(uses - kStages, 0); u < uses; ++u) {
+    mbarrier_wait_limited(&full[u % kStages], (u / kStages) & 1, 1u << 16);
+  }
+}
+
 // Key of column c of a group of eight scores.
 template <bool kFp8>
 __device__ __forceinline__ int key_of(int c) {
@@ -315,8 +324,10 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
       }
       if (more) look_up(t);
 
-      if (use >= kStages && !mbarrier_wait_bounded(&empty[stage], (use / kStages - 1) & 1)) {
+      if (use >= kStages &&
+          !mbarrier_wait_warp(&empty[stage], (use / kStages - 1) & 1, a.wait_polls)) {
         if (lane == 0) atomicAdd(&g_decode_expired_waits, 1u);
+        let_land<kStages>(full, use);
         break;
       }
       unsigned char* tile = smem + stage * stage_bytes;
@@ -380,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
   const int g = lane >> 2, tq = lane & 3;
   const int key0 = warp * kWarpKeys;
   int use = 0;
-  bool ok = true;  // false after a wait ran out: keep step with the other warps, write nothing
+  bool ok = true;  // false after a wait ran out: keep step with the other warps, mark the rows
   while (walk.next(a)) {
     const int rows = min(16, a.group - walk.first_head);
     uint32_t q[D / 16][4];
@@ -391,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
     for (int t = walk.tile0; t < walk.tile1; ++t, ++use) {
       const int stage = use % kStages;
-      if (ok && !mbarrier_wait_bounded(&full[stage], (use / kStages) & 1)) {
+      if (ok && !mbarrier_wait_warp(&full[stage], (use / kStages) & 1, a.wait_polls)) {
         if (lane == 0) atomicAdd(&g_decode_expired_waits, 1u);
         ok = false;
       }
@@ -578,8 +589,8 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
       l1 += __shfl_xor_sync(kFullMask, l1, d);
     }
     if (tq == 0) {
-      states[warp][g] = make_float2(m0, l0);
-      states[warp][g + 8] = make_float2(m1, l1);
+      states[warp][g] = ok ? make_float2(m0, l0) : make_float2(-INFINITY, NAN);
+      states[warp][g + 8] = ok ? make_float2(m1, l1) : make_float2(-INFINITY, NAN);
     }
     bar_compute();
     float weight[2];  // of this warp's values of rows g and g + 8 in the joint result
@@ -591,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
       weight[half] = exp2_approx((half ? m1 : m0) - (top == -INFINITY ? 0.0f : top));
     }
     const int64_t slot = (static_cast<int64_t>(walk.request) * triples + walk.triple + blockIdx.x) * 16;
-    if (ok && threadIdx.x < rows) {
+    if (threadIdx.x < rows) {
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, states[w][threadIdx.x].x);
@@ -631,13 +642,12 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
           sum.z += x.z;
           sum.w += x.w;
         }
-        if (ok) {
-          *reinterpret_cast<float4*>(a.own_values + (slot + row) * D + c0 * kMergeColumns + 4 * c) = sum;
-        }
+        *reinterpret_cast<float4*>(a.own_values + (slot + row) * D + c0 * kMergeColumns + 4 * c) = sum;
       }
       bar_compute();
     }
   }
+  if (!ok) let_land<kStages>(full, use);
   if (beside_prefix && blockIdx.x == 0) wait_for_upstream_grid();
 }
 

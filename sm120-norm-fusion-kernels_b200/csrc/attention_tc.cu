@@ -45,7 +45,9 @@
 // before it) and the release of P_j.
 //
 // Every wait on an mbarrier is bounded; one that runs out is counted
-// (sm120s_get_device_faults) and ends the block without results.
+// (sm120s_get_device_faults) and ends the block: a prompt's rows that are not
+// finished then are left as they were, a prefix's are marked for the kernel that
+// joins them.
 #include <algorithm>
 #include <cfloat>
 
@@ -219,12 +221,17 @@ struct Control {
   int aborted;
   int unsafe;  // a value that some rows must not see is infinite or NaN
   int holes;   // kPrefix: a block of the prefix does not exist
+  int loads;   // tiles that the loader has asked for
 };
 
-__device__ __forceinline__ bool wait_in(Control& c, uint64_t* bar, uint32_t parity) {
-  if (mbarrier_wait_bounded(bar, parity)) return true;
-  atomicAdd(&g_attention_expired_waits, 1u);
-  atomicExch(&c.aborted, 1);
+// By a whole warp.
+__device__ __forceinline__ bool wait_in(Control& c, uint64_t* bar, uint32_t parity, uint32_t polls) {
+  if (mbarrier_wait_warp(bar, parity, polls)) return true;
+  if ((threadIdx.x & (kWarpSize - 1)) == 0) {
+    atomicAdd(&g_attention_expired_waits, 1u);
+    atomicExch(&c.aborted, 1);
+  }
+  __syncwarp();
   return false;
 }
 
@@ -245,14 +252,15 @@ __device__ __forceinline__ RowPlace row_place(const Args& a, const Work& w, int 
 // has 16 bytes of a row at a time, 32 in the stage.
 template <typename S, int D>
 __device__ __forceinline__ void convert_tiles(Control& c, unsigned char* stages,
-                                              const unsigned char* raw_tiles, int tiles, int thread) {
+                                              const unsigned char* raw_tiles, int tiles, int thread,
+                                              uint32_t polls) {
   constexpr int kRowChunks = D / 16;
   constexpr int kAll = kTileKeys * kRowChunks;
   for (int t = 0; t < 2 * tiles; ++t) {
     const int stage = t % S::kStages;
     const int slot = t % S::kRawTiles;
-    if (!wait_in(c, &c.bar.raw_full[slot], (t / S::kRawTiles) & 1)) return;
-    if (t >= S::kStages && !wait_in(c, &c.bar.empty[stage], (t / S::kStages - 1) & 1)) return;
+    if (!wait_in(c, &c.bar.raw_full[slot], (t / S::kRawTiles) & 1, polls)) return;
+    if (t >= S::kStages && !wait_in(c, &c.bar.empty[stage], (t / S::kStages - 1) & 1, polls)) return;
     const unsigned char* raw = raw_tiles + slot * S::kRawBytes;
     unsigned char* to = stages + stage * S::kTileBytes;
 #pragma unroll 4
@@ -386,7 +394,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         kPass == kPrompt ? row_place(a, w, i * kTileRows).token : limit;
     bool ok = true;
     for (int j = 0; j < n[i]; ++j) {
-      if (!wait_in(c, &c.bar.s_full[i], j & 1)) {
+      if (!wait_in(c, &c.bar.s_full[i], j & 1, a.wait_polls)) {
         ok = false;
         break;
       }
@@ -439,7 +447,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       const float next = fmaxf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), top);
       if constexpr (S::kOwnP) {
         // P and O are free for this tile once the last product is complete
-        if (j > 0 && !wait_in(c, &c.bar.p_free[i], (j - 1) & 1)) {
+        if (j > 0 && !wait_in(c, &c.bar.p_free[i], (j - 1) & 1, a.wait_polls)) {
           ok = false;
           break;
         }
@@ -491,13 +499,19 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&c.bar.p_ready[i]);
     }
-    if (ok && n[i] > 0) ok = wait_in(c, &c.bar.o_full[i], 0);
+    if (ok && n[i] > 0) ok = wait_in(c, &c.bar.o_full[i], 0, a.wait_polls);
     if constexpr (kPass == kPrompt) {
-      if (ok) ok = wait_in(c, &c.bar.guarded, 0);
+      if (ok) ok = wait_in(c, &c.bar.guarded, 0, a.wait_polls);
     }
     ok = ok && !*reinterpret_cast<volatile int*>(&c.aborted);
     ok = __all_sync(kFullMask, ok);
     tc_fence_after();
+    if constexpr (kPass == kPrefix) {
+      if (!ok && lane < live_rows) {
+        a.prefix_state[(static_cast<int64_t>(w.split) * a.batch + place.token) * a.query_heads +
+                       place.head] = make_float2(-INFINITY, NAN);
+      }
+    }
     if (ok && live_rows > 0) {
       if (kPass == kPrompt && *reinterpret_cast<volatile int*>(&c.unsafe)) {
         if constexpr (kPass == kPrompt) {
@@ -578,7 +592,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       const uint32_t tmem = c.tmem;
       const uint64_t first_key = smem_descriptor(stages);
       const uint64_t first_value = value_descriptor(stages);
-      auto full = [&](int t) { return wait_in(c, &c.bar.full[t % kStages], (t / kStages) & 1); };
+      auto full = [&](int t) { return wait_in(c, &c.bar.full[t % kStages], (t / kStages) & 1, a.wait_polls); };
       auto score = [&](int i, int t) {  // with the key tile of stage use t
         const uint64_t q = smem_descriptor(smem + i * S::kQBytes);
         const uint64_t k = first_key + (t % kStages) * (S::kTileBytes >> 4);
@@ -605,7 +619,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       };
       auto mine = [&](int i) { return S::kIssuers == 1 || i == issuer; };
       // A stage is free once every issuer has committed behind its products with it.
-      bool ok = wait_in(c, &c.bar.q_full, 0) && full(0);
+      bool ok = wait_in(c, &c.bar.q_full, 0, a.wait_polls) && full(0);
       tc_fence_after();
       if (ok && elect_lane()) {
 #pragma unroll
@@ -621,7 +635,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
 #pragma unroll
           for (int i = 0; i < kTiles; ++i) {
             if (!ok || !mine(i) || j + 1 >= n[i]) continue;
-            ok = wait_in(c, &c.bar.s_free[i], j & 1);
+            ok = wait_in(c, &c.bar.s_free[i], j & 1, a.wait_polls);
             tc_fence_after();
             if (ok && elect_lane()) score(i, 2 * j + 2);
           }
@@ -631,7 +645,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
           if (!ok || !mine(i) || j >= n[i]) continue;
-          ok = wait_in(c, &c.bar.p_ready[i], j & 1);
+          ok = wait_in(c, &c.bar.p_ready[i], j & 1, a.wait_polls);
           tc_fence_after();
           if (ok && elect_lane()) {
             weigh(i, 2 * j + 1);
@@ -645,13 +659,14 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       }
       if (elect_lane()) mma_commit(&c.bar.done);
     } else if (warp == S::kLoadWarp) {
-      for (int t = 0; t < 2 * tiles; ++t) {
+      int t = 0;
+      for (; t < 2 * tiles; ++t) {
         const int ring = kFp8 ? S::kRawTiles : kStages;
         const int slot = t % ring;
         uint64_t* loaded = kFp8 ? &c.bar.raw_full[slot] : &c.bar.full[slot];
         uint64_t* emptied = kFp8 ? &c.bar.raw_empty[slot] : &c.bar.empty[slot];
         if (*reinterpret_cast<volatile int*>(&c.aborted)) break;
-        if (t >= ring && !wait_in(c, emptied, (t / ring - 1) & 1)) break;
+        if (t >= ring && !wait_in(c, emptied, (t / ring - 1) & 1, a.wait_polls)) break;
         const CUtensorMap* map = t & 1 ? value_map : key_map;
         const int key0 = (t / 2) * kTileKeys;
         if constexpr (kPass == kPrompt) {
@@ -700,10 +715,11 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
           }
         }
       }
+      if (lane == 0) c.loads = t;
     } else if (kFp8) {
       if constexpr (kFp8) {
         convert_tiles<S, D>(c, stages, raw_tiles, tiles,
-                            (warp - S::kLoadWarp - 1) * kWarpSize + lane);
+                            (warp - S::kLoadWarp - 1) * kWarpSize + lane, a.wait_polls);
       }
     } else if (kPass == kPrompt) {
       // V tiles that reach past the block's first row's last key
@@ -712,7 +728,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
       bool bad = false;
       for (int j = 0; j < tiles; ++j) {
         const int stage = (2 * j + 1) % kStages;
-        if (!wait_in(c, &c.bar.full[stage], ((2 * j + 1) / kStages) & 1)) break;
+        if (!wait_in(c, &c.bar.full[stage], ((2 * j + 1) / kStages) & 1, a.wait_polls)) break;
         if (int64_t{j + 1} * kTileKeys - 1 > first_limit) {
           const uint4* v = reinterpret_cast<const uint4*>(stages + stage * S::kTileBytes);
 #pragma unroll 4
@@ -763,6 +779,7 @@ __device__ __forceinline__ void open_block(Control& c, bool guarded, bool conver
     c.aborted = 0;
     c.unsafe = 0;
     c.holes = 0;
+    c.loads = 0;
     fence_mbarrier_init();
   }
   if (threadIdx.x / kWarpSize == S::kSoftmaxWarps) tmem_alloc(&c.tmem, S::kTmemColumns);
@@ -771,7 +788,7 @@ __device__ __forceinline__ void open_block(Control& c, bool guarded, bool conver
   tc_fence_after();
 }
 
-template <typename S>
+template <typename S, bool kFp8 = false>
 __device__ __forceinline__ void close_block(Control& c) {
   tc_fence_before();
   __syncthreads();
@@ -785,9 +802,11 @@ __device__ __forceinline__ void close_block(Control& c) {
     tmem_dealloc(c.tmem, S::kTmemColumns);
   }
   if (c.aborted && threadIdx.x == S::kLoadWarp * kWarpSize) {
-    // an expired wait: give loads that are still on their way a bounded time to land
-    for (int s = 0; s < S::kStages; ++s) {
-      for (uint32_t p = 0; p < 2; ++p) mbarrier_wait_limited(&c.bar.full[s], p, 1u << 16);
+    // an expired wait: the loads that are still on their way land first
+    constexpr int kRing = kFp8 ? S::kRawTiles : S::kStages;
+    uint64_t* landed = kFp8 ? c.bar.raw_full : c.bar.full;
+    for (int t = max(c.loads - kRing, 0); t < c.loads; ++t) {
+      mbarrier_wait_bounded(&landed[t % kRing], (t / kRing) & 1);
     }
   }
 }
@@ -841,7 +860,7 @@ __global__ void __launch_bounds__(TcShape<D, 2, kFp8>::kThreads, 1)
                                     int64_t{a.prefix_tokens}));
   attend<TQ, T, kFp8, D, 2, kPrefix>(a, w, &key_map, &value_map, control,
                                      aligned_tiles(dynamic_smem));
-  close_block<S>(control);
+  close_block<S, kFp8>(control);
 }
 
 // ---- host ----------------------------------------------------------------------

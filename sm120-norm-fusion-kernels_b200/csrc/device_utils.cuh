@@ -354,6 +354,13 @@ __device__ __forceinline__ bool mbarrier_wait_limited(uint64_t* bar, uint32_t pa
   return false;
 }
 
+// The same by a whole converged warp, with one answer for all of its lanes: they
+// poll on their own, and a barrier that completes between two lanes' last polls
+// must not send them different ways.
+__device__ __forceinline__ bool mbarrier_wait_warp(uint64_t* bar, uint32_t parity, uint32_t polls) {
+  return __all_sync(kFullMask, mbarrier_wait_limited(bar, parity, polls));
+}
+
 // Asks L2 for `bytes` (a multiple of 16) at 16-byte-aligned global `p`; no
 // data is returned and nothing waits for it. Kernels issue these for inputs
 // before waiting for the upstream grid (programmatic dependent launch): a

@@ -21,9 +21,10 @@ void clear_error();
 
 bool programmatic_launch_enabled();
 
-// Polls a kernel makes while waiting for its own bulk copies to land before
-// it records an expired wait (sm120n_set_wait_limit; kernels receive it as an
-// argument). The default is far beyond any real copy.
+// Polls a kernel makes in a wait on its own bulk copies (the attention kernels:
+// in any wait on an mbarrier) before it records an expired wait
+// (sm120n_set_wait_limit; kernels receive it as an argument). The default is far
+// beyond any real copy.
 constexpr uint32_t kDefaultWaitPolls = 1u << 22;
 uint32_t wait_poll_limit();
 

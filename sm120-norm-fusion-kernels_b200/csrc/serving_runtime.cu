@@ -1,6 +1,7 @@
 // serving_runtime.cu -- error state and fault counter of the serving library
 // (declared in include/sm120norm_b200_serving.h). Its kernels follow the
-// process-wide switches of the norm library, sm120n_set_programmatic_launch.
+// process-wide switches of the norm library, sm120n_set_programmatic_launch and
+// sm120n_set_wait_limit.
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -26,6 +27,8 @@ int fail(int status, const char* fmt, ...) {
 void clear_error() { g_last_error.clear(); }
 
 bool programmatic_launch_enabled() { return sm120n_get_programmatic_launch() != 0; }
+
+uint32_t wait_poll_limit() { return sm120n_get_wait_limit(); }
 
 }  // namespace sm120n
 
