@@ -962,18 +962,22 @@ using namespace sm120n;
 extern "C" int sm120s_get_device_faults(uint32_t* out_count) {
   clear_error();
   if (!out_count) return fail(SM120N_ERR_INVALID_ARGUMENT, "out_count must be non-null");
+  int rc = wait_for_device();
+  if (rc != SM120N_OK) return rc;
   unsigned int mine = 0, decode = 0;
   const cudaError_t err = cudaMemcpyFromSymbol(&mine, g_attention_expired_waits, sizeof mine);
   if (err != cudaSuccess) {
     return fail(SM120N_ERR_CUDA, "reading the fault counter failed: %s", cudaGetErrorString(err));
   }
-  const int rc = read_decode_faults(&decode);
+  rc = read_decode_faults(&decode);
   if (rc == SM120N_OK) *out_count = mine + decode;
   return rc;
 }
 
 extern "C" int sm120s_reset_device_faults(void) {
   clear_error();
+  const int rc = wait_for_device();
+  if (rc != SM120N_OK) return rc;
   const unsigned int zero = 0;
   const cudaError_t err = cudaMemcpyToSymbol(g_attention_expired_waits, &zero, sizeof zero);
   if (err != cudaSuccess) {

@@ -1,6 +1,6 @@
 // device_caches.cu -- per-device properties, occupancy and shared-memory grants
-// behind csrc/runtime.h, asked of the CUDA runtime once; linked into both
-// libraries.
+// behind csrc/runtime.h, asked of the CUDA runtime once, and the wait for a
+// device; linked into both libraries.
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -41,6 +41,13 @@ int current_device_info(DeviceInfo* info) {
   info->device = device;
   info->sm_count = g_sm_count[device];
   return SM120N_OK;
+}
+
+int wait_for_device() {
+  const cudaError_t err = cudaDeviceSynchronize();
+  return err == cudaSuccess ? SM120N_OK
+                            : fail(SM120N_ERR_CUDA, "waiting for the device failed: %s",
+                                   cudaGetErrorString(err));
 }
 
 int max_resident_ctas(const void* kernel, int threads, size_t smem, int* out) {

@@ -769,13 +769,15 @@ extern "C" int sm120n_fused_add_rms_norm(const void* input, const void* residual
 extern "C" int sm120n_get_device_faults(uint32_t* out_count) {
   clear_error();
   if (out_count == nullptr) return fail(SM120N_ERR_INVALID_ARGUMENT, "out_count must be non-null");
+  int rc = wait_for_device();
+  if (rc != SM120N_OK) return rc;
   unsigned int value = 0;
   const cudaError_t err = cudaMemcpyFromSymbol(&value, g_expired_waits, sizeof value);
   if (err != cudaSuccess) {
     return fail(SM120N_ERR_CUDA, "reading the fault counter failed: %s", cudaGetErrorString(err));
   }
   unsigned int gemm = 0;
-  const int rc = read_gemm_faults(&gemm);
+  rc = read_gemm_faults(&gemm);
   if (rc != SM120N_OK) return rc;
   *out_count = value + gemm;
   return SM120N_OK;
@@ -783,6 +785,8 @@ extern "C" int sm120n_get_device_faults(uint32_t* out_count) {
 
 extern "C" int sm120n_reset_device_faults(void) {
   clear_error();
+  const int rc = wait_for_device();
+  if (rc != SM120N_OK) return rc;
   const unsigned int zero = 0;
   const cudaError_t err = cudaMemcpyToSymbol(g_expired_waits, &zero, sizeof zero);
   if (err != cudaSuccess) {

@@ -72,6 +72,10 @@ int launch(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, size_t smem,
   return SM120N_OK;
 }
 
+// Waits for all streams of the current device, before a fault counter is read or
+// reset: the copies of a symbol wait for blocking streams only.
+int wait_for_device();
+
 // Expired-wait counter of the tensor-core projection kernel (qkv_gemm.cu),
 // read / reset alongside the row kernels' counter.
 int read_gemm_faults(unsigned int* value);
