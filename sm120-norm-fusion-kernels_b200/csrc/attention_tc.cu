@@ -824,11 +824,13 @@ __global__ void __launch_bounds__(TcShape<D, kTiles>::kThreads, 3 - kTiles)
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ Control control;
   wait_for_upstream_grid();
-  release_downstream_grid();
   const SequenceTile tile = find_tile<kTiles * kTileRows>(a.query_start, a.sequences, a.tokens,
                                                           a.group, blockIdx.x / a.key_heads);
   if (tile.tile < 0) return;
   open_block<S>(control, true, false);
+  // Not before this block has its tensor memory: blocks of the next kernel may take
+  // theirs before they wait for this one, and would then hold what it waits for.
+  release_downstream_grid();
   Work w{};
   place_rows<kTiles>(w, tile.tile * kTiles * kTileRows, tile.length * a.group, a.group);
   w.token0 = tile.first_token;
