@@ -70,7 +70,7 @@ SM120N_API int sm120s_reset_device_faults(void);
  * not written. free_count_out may be free_count and seq_lens may be
  * context_lens; other buffers may not overlap. tokens is the length of
  * positions (int64) and slot_mapping (int32). A request of 2^31 tokens or more is
- * not served.
+ * not served. requests and table_width up to 2^30.
  */
 SM120N_API int sm120s_plan_step(const int32_t* context_lens, const int32_t* query_lens,
                      int32_t* block_table, int64_t table_stride, const int32_t* free_blocks,

@@ -193,7 +193,8 @@ extern "C" int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
   int rc = check_heads(in.dtype, in.query_heads, in.key_heads, in.head_dim, in.scale);
   if (rc != SM120N_OK) return rc;
   const int64_t group = in.query_heads / in.key_heads;
-  if (in.tokens < 0 || in.sequences < 0 || in.sequences > INT32_MAX - 1 ||
+  // 32-bit indices that run up to a step of the search past the end
+  if (in.tokens < 0 || in.sequences < 0 || in.sequences > INT32_MAX - 256 ||
       in.tokens > INT32_MAX - 256) {
     return fail(SM120N_ERR_INVALID_ARGUMENT, "tokens and sequences must be in [0, 2^31 - 256)");
   }

@@ -423,10 +423,11 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
 
 int check_pool(const void* free_blocks, int64_t pool, const void* free_count, const void* count_out,
                int64_t requests, int64_t width, int64_t table_stride, int64_t block_size) {
-  if (requests < 0 || width < 0 || pool < 0 || requests > INT32_MAX || width > INT32_MAX ||
+  // row and entry indices are 32-bit and run up to a round past the end
+  if (requests < 0 || width < 0 || pool < 0 || requests > (1 << 30) || width > (1 << 30) ||
       pool >= INT32_MAX) {
     return fail(SM120N_ERR_INVALID_ARGUMENT,
-                "requests, table width and pool size must be in [0, 2^31 - 1)");
+                "requests and table width must be in [0, 2^30], the pool size in [0, 2^31 - 1)");
   }
   if (block_size < 1 || block_size > INT32_MAX || pool > (int64_t{1} << 31) / block_size) {
     return fail(SM120N_ERR_INVALID_ARGUMENT,
