@@ -36,7 +36,7 @@ from __future__ import annotations
 import torch
 
 from .ops import _C, _extension
-from .serving import _op
+from .serving import _call
 
 FP8_MAX = 448.0
 MIN_TOKEN_SCALE = 1.0 / (448.0 * 512.0)
@@ -104,10 +104,9 @@ def qk_norm_mrope_cache_(
     to the activation dtype and separately to an fp8 cache, so a result may
     differ in its last place from :func:`qk_norm_rope_cache_`, which rounds after
     each stage."""
-    _op("qk_norm_mrope_cache_", query)(
-        query, key, value, query_weight, key_weight, positions, cos_sin_cache, sections,
-        key_cache, value_cache, slot_mapping, k_scale, v_scale, is_neox, interleaved_sections,
-        kv_cache_layout, epsilon, query_out, key_out)
+    _call("qk_norm_mrope_cache_", query, key, value, query_weight, key_weight, positions,
+          cos_sin_cache, sections, key_cache, value_cache, slot_mapping, k_scale, v_scale, is_neox,
+          interleaved_sections, kv_cache_layout, epsilon, query_out, key_out)
 
 
 def rms_norm_static_fp8_quant(result: torch.Tensor, input: torch.Tensor, weight: torch.Tensor,

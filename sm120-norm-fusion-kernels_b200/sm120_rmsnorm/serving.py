@@ -28,14 +28,24 @@ def _dispatched(name: str):
     return getattr(torch.ops.sm120_norm_ext, name).default
 
 
-def _op(name: str, tensor: torch.Tensor):
-    """The operator: the extension's function for ordinary tensors (small steps
-    are bound by the host, and the dispatcher costs as much again), the
-    registered operator for tracing and for tensor subclasses."""
-    if type(tensor) is torch.Tensor and not torch.compiler.is_compiling():
-        return getattr(_extension(), name)
-    _extension()
-    return _dispatched(name)
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None), bool, int, float, str, list, tuple))
+_compiling = torch.compiler.is_compiling
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_function_modes = torch._C._len_torch_function_stack
+_transforms = torch._C._functorch.peek_interpreter_stack
+
+
+def _call(name: str, *args) -> None:
+    """The operator: the extension's function where nothing could look on (small
+    steps are bound by the host, and the dispatcher costs as much again), the
+    registered operator for tracing, modes, function transforms and tensor
+    subclasses among the arguments."""
+    extension = _extension()
+    if (not _compiling() and _PLAIN.issuperset(map(type, args))
+            and not _dispatch_modes() and not _function_modes() and _transforms() is None):
+        getattr(extension, name)(*args)
+    else:
+        _dispatched(name)(*args)
 
 
 def plan_step_(
@@ -68,9 +78,8 @@ def plan_step_(
     behind the last token, which the Q/K norm operators leave untouched.
     ``free_count`` (int32 [1]) is updated in place, or left as it is with the new
     count in ``free_count_out``."""
-    _op("plan_step_", context_lens)(
-        context_lens, query_lens, block_table, free_blocks, free_count, block_size, query_start,
-        seq_lens, positions, slot_mapping, free_count_out)
+    _call("plan_step_", context_lens, query_lens, block_table, free_blocks, free_count, block_size,
+          query_start, seq_lens, positions, slot_mapping, free_count_out)
 
 
 def release_blocks_(
@@ -89,8 +98,8 @@ def release_blocks_(
     Table entries outside [0, length of ``free_blocks``) are skipped. The table
     and ``seq_lens`` are not written: a row given back must not be given back
     again."""
-    _op("release_blocks_", seq_lens)(seq_lens, finished, block_table, free_blocks, free_count,
-                                     block_size, shared_blocks, free_count_out)
+    _call("release_blocks_", seq_lens, finished, block_table, free_blocks, free_count, block_size,
+          shared_blocks, free_count_out)
 
 
 def prompt_attention(
@@ -110,7 +119,7 @@ def prompt_attention(
     lengths need not be known on the host. Rows of ``out`` behind the last
     sequence are left as they were. ``scale`` defaults to 1 / sqrt(D) and must be
     positive."""
-    _op("prompt_attention", out)(out, query, key, value, query_start, scale)
+    _call("prompt_attention", out, query, key, value, query_start, scale)
 
 
 def paged_decode_attention(
@@ -141,9 +150,8 @@ def paged_decode_attention(
     request of at least ``P * block_size`` tokens reads its first P blocks from
     there instead of from its row, and they are read once for the whole batch;
     a shorter one is read through its row alone."""
-    _op("paged_decode_attention", out)(
-        out, query, key_cache, value_cache, block_table, seq_lens, prefix_blocks, k_scale,
-        v_scale, kv_cache_layout, scale)
+    _call("paged_decode_attention", out, query, key_cache, value_cache, block_table, seq_lens,
+          prefix_blocks, k_scale, v_scale, kv_cache_layout, scale)
 
 
 if _C is not None:
