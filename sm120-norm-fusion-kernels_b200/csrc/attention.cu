@@ -126,7 +126,8 @@ int prefix_parts(const sm120s_decode_args& a, int most, int64_t blocks, int64_t 
   const double step = (a.cache_dtype == SM120N_CACHE_FP8_E4M3 ? 2.2 : 1.8) *  // us, 128 keys
                       (a.head_dim == 64 ? 0.72 : 1.0);
   const double start = 16.0, join_bytes = 1.5e6;  // us of an SM; bytes in a us
-  const int own_room = own_blocks_per_sm(static_cast<int>(a.head_dim)) * sm_count;
+  const int own_room =
+      own_blocks_per_sm(a.cache_dtype, static_cast<int>(a.head_dim), a.query_heads / a.key_heads) * sm_count;
   const double wanted =  // of the SMs
       std::min(1.0, static_cast<double>(std::max<int64_t>(triples, 1)) / own_room);
   const double cost = start * blocks / sm_count * wanted +
@@ -148,8 +149,9 @@ int plan_decode(const sm120s_decode_args& a, Plan* plan) {
   const int64_t triples = a.batch * a.key_heads * plan->row_tiles;
   const int64_t most_tiles = (a.table_width * a.block_size + 63) / 64;
   plan->own_grid = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(own_blocks_per_sm(static_cast<int>(a.head_dim)) * dev.sm_count,
-                           triples * most_tiles)));
+      1, std::min<int64_t>(
+             own_blocks_per_sm(a.cache_dtype, static_cast<int>(a.head_dim), group) * dev.sm_count,
+             triples * most_tiles)));
   plan->prefix_splits = 0;
   if (a.prefix_blocks_count > 0 && a.num_blocks > 0) {
     const bool tc = prefix_on_tensor_memory(a);

@@ -73,8 +73,8 @@ struct DecodeArgs {
   float* prefix_values;  // the same rows x head_dim
 };
 
-// Blocks per SM of the pass over own tokens.
-int own_blocks_per_sm(int head_dim);
+// Blocks of the pass over own tokens that an SM holds.
+int own_blocks_per_sm(int cache_dtype, int head_dim, int64_t group);
 
 // One launch each; element types as sm120n_dtype, caches as sm120n_cache_dtype.
 int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);

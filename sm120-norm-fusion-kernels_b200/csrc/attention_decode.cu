@@ -66,7 +66,7 @@ struct OwnForm {
     return (c >> 3) * kBoxBytes + r * 128 + ((c & 7) ^ (r & 7)) * 16;
   }
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
-  // About 100 KB of tiles to a block and two blocks to an SM, or 200 KB and one
+  // About 100 KB of tiles to a block and up to two blocks to an SM, or 200 KB and one
   // with heads of 256, whose values and queries fill a thread's registers: well
   // past the 50 KB in flight that latency times bandwidth asks.
   static constexpr int kStages = D == 256 ? (kFp8 ? 5 : 3) : kRowBytes == 256 ? 3 : 5;
@@ -74,6 +74,13 @@ struct OwnForm {
   static constexpr size_t stage_bytes(int q_rows) { return 2 * kTileBytes + q_rows * D * 2; }
   static constexpr size_t smem(int q_rows) {
     return 1024 + kStages * stage_bytes(q_rows) + static_cast<size_t>(kWarps) * q_rows * kMergeColumns * 4;
+  }
+  // With the static part and what the system keeps of 228 KB. More than 8 query
+  // heads to a key head leave room for one block at D = 128 in 16 bits; a grid of
+  // two to an SM then ran in two waves (64/4 heads, 256 requests of 1-1024 tokens,
+  // 96.3 us against 88.1; 4 of up to 8192, 27.3 against 18.5).
+  static constexpr int blocks_per_sm(int q_rows) {
+    return smem(q_rows) + 2048 <= 228 * 1024 / 2 ? kBlocksPerSm : 1;
   }
 };
 
@@ -785,7 +792,6 @@ int run_own(const DecodeArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int own_blocks_per_sm(int head_dim) { return head_dim == 256 ? 1 : 2; }
 
 #define SM120S_BY_HEAD_DIM(CALL)      \
   switch (head_dim) {                 \
@@ -801,6 +807,15 @@ int launch_own(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim, cu
                              : run_own<__half, __half, false, D>(a, stream))          \
                       : (fp8 ? run_own<__nv_bfloat16, __half, true, D>(a, stream)     \
                              : run_own<__nv_bfloat16, __nv_bfloat16, false, D>(a, stream))
+  SM120S_BY_HEAD_DIM(CALL)
+#undef CALL
+}
+
+int own_blocks_per_sm(int cache_dtype, int head_dim, int64_t group) {
+  const int q_rows = group <= 8 ? 8 : 16;
+#define CALL(D)                                                                              \
+  cache_dtype == SM120N_CACHE_FP8_E4M3 ? OwnForm<true, D>::blocks_per_sm(q_rows)             \
+                                       : OwnForm<false, D>::blocks_per_sm(q_rows)
   SM120S_BY_HEAD_DIM(CALL)
 #undef CALL
 }
