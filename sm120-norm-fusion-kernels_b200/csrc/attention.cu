@@ -236,7 +236,7 @@ extern "C" int sm120s_prompt_attention(const sm120s_prompt_args* args, void* str
   const int head_dim = static_cast<int>(in.head_dim);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return head_dim <= 128 ? launch_prompt_tc(a, in.dtype, head_dim, s)
-                         : launch_prompt_mma(a, in.dtype, head_dim, s);
+                         : launch_prompt_mma(a, in.dtype, s);
 }
 
 extern "C" int sm120s_paged_decode_workspace(const sm120s_decode_args* args, size_t* bytes) {

@@ -77,7 +77,7 @@ struct DecodeArgs {
 int own_blocks_per_sm(int cache_dtype, int head_dim, int64_t group);
 
 // One launch each; element types as sm120n_dtype, caches as sm120n_cache_dtype.
-int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream);
+int launch_prompt_mma(const PromptArgs& a, int dtype, cudaStream_t stream);  // head size 256
 int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,
                       cudaStream_t stream);
 // Head sizes 64 and 128; the prefix form wants blocks that fill a tile of 128 keys.

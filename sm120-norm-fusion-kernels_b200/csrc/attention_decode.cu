@@ -129,9 +129,6 @@ __device__ __forceinline__ void bar_compute() {  // the four computing warps
   asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
-__device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
-}
 // One arrival of this thread once its copies so far have landed.
 __device__ __forceinline__ void mbarrier_arrive_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(bar))

@@ -541,11 +541,9 @@ int run_prefix(const DecodeArgs& a, cudaStream_t stream) {
     default: return CALL(256);        \
   }
 
-int launch_prompt_mma(const PromptArgs& a, int dtype, int head_dim, cudaStream_t stream) {
-#define CALL(D) \
-  dtype == SM120N_F16 ? run_prompt<__half, D>(a, stream) : run_prompt<__nv_bfloat16, D>(a, stream)
-  SM120S_BY_HEAD_DIM(CALL)
-#undef CALL
+int launch_prompt_mma(const PromptArgs& a, int dtype, cudaStream_t stream) {
+  return dtype == SM120N_F16 ? run_prompt<__half, 256>(a, stream)
+                             : run_prompt<__nv_bfloat16, 256>(a, stream);
 }
 
 int launch_prefix_mma(const DecodeArgs& a, int dtype, int cache_dtype, int head_dim,

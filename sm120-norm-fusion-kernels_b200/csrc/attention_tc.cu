@@ -168,10 +168,6 @@ __device__ __forceinline__ void tmem_wait_store() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
-}
-
 template <int kRegisters>
 __device__ __forceinline__ void grow_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
