@@ -511,8 +511,9 @@ __global__ void __launch_bounds__(kThreads, OwnForm<kFp8, D>::kBlocksPerSm)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const bool real = (there >> (n * 8 + key_of<kFp8>(2 * tq + c))) & 1u;
-          s[n][c] = real ? s[n][c] * f0 : -INFINITY;
-          s[n][2 + c] = real ? s[n][2 + c] * f1 : -INFINITY;
+          // not merged with the difference to the maximum: both are rounded alike
+          s[n][c] = real ? __fmul_rn(s[n][c], f0) : -INFINITY;
+          s[n][2 + c] = real ? __fmul_rn(s[n][2 + c], f1) : -INFINITY;
           top0 = fmaxf(top0, s[n][c]);
           top1 = fmaxf(top1, s[n][2 + c]);
         }

@@ -363,8 +363,9 @@ struct Worker {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int key = n * 8 + 2 * (lane & 3) + c;
-          s[n][c] *= f0;
-          s[n][2 + c] *= f1;
+          // not merged with the difference to the maximum: both are rounded alike
+          s[n][c] = __fmul_rn(s[n][c], f0);
+          s[n][2 + c] = __fmul_rn(s[n][2 + c], f1);
           const bool there = whole || (((key < 32 ? live0 : live1) >> (key & 31)) & 1u);
           if (!there || (kPass == kPrompt && key0 + key > limit[0])) s[n][c] = -INFINITY;
           if (!there || (kPass == kPrompt && key0 + key > limit[1])) s[n][2 + c] = -INFINITY;

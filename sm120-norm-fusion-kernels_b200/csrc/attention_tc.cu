@@ -44,6 +44,10 @@
 // themselves, between S_j (whose completion implies that of the product
 // before it) and the release of P_j.
 //
+// scale * s - m is one fused operation: the product is not rounded, m is. Past
+// kFar that difference is no longer small against the exponent (2^27: p past fp16,
+// 2^31: infinite); there products are rounded as m was, a step of their own.
+//
 // Every wait on an mbarrier is bounded; one that runs out is counted
 // (sm120s_get_device_faults) and ends the block: a prompt's rows that are not
 // finished then are left as they were, a prefix's are marked for the kernel that
@@ -66,6 +70,7 @@ constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
 constexpr uint32_t kBoxBytes = kTileKeys * 128;  // 64 elements of 128 rows
 constexpr float kSlack = 8.0f;                   // log2 of how far a maximum may lag
+constexpr float kFar = 1u << 22;                 // scaled scores whose last place is 1/2
 
 enum Pass : int { kPrompt, kPrefix };
 
@@ -384,6 +389,7 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
     float top = -INFINITY;  // raw maximum that `base` follows
     float base = 0.0f;      // scale * the maximum in use
     float sum = 0.0f;
+    float step = scale;     // 1 where some row of the warp has |base| > kFar
     // last key of the row, counted from the first key tile's first
     const int64_t limit = kPass == kPrompt ? place.token : int64_t{w.key_last} - w.key_first - 1;
     const int64_t first_limit =  // smallest of the tile: tiles behind it need no mask
@@ -467,8 +473,13 @@ __device__ __forceinline__ void attend(const Args& a, const Work& w, const CUten
         sum *= keep;
         base = moved;
         if (lags) top = next;
+        step = __any_sync(kFullMask, fabsf(base) > kFar) ? 1.0f : scale;
       }
-      const float2 factor = make_float2(scale, scale);
+      if (__builtin_expect(step != scale, 0)) {
+#pragma unroll
+        for (int k = 0; k < kTileKeys; ++k) s[k] = __fmul_rn(s[k], scale);
+      }
+      const float2 factor = make_float2(step, step);
       const float2 shift = make_float2(-base, -base);
       float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
 #pragma unroll

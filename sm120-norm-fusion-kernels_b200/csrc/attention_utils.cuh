@@ -51,7 +51,7 @@ __device__ __noinline__ void plain_prompt_row(const PromptArgs& a, int64_t token
     }
 #pragma unroll
     for (int d = kWarpSize / 2; d > 0; d /= 2) s += __shfl_xor_sync(kFullMask, s, d);
-    s *= a.scale_log2;
+    s = __fmul_rn(s, a.scale_log2);  // not merged with the difference: both are rounded alike
     const float next = fmaxf(top, s);
     const float base = next == -INFINITY ? 0.0f : next;
     const float keep = exp2_approx(top - base);
