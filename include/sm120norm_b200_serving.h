@@ -142,6 +142,9 @@ SM120N_API int sm120s_qk_norm_mrope_cache(const sm120n_qk_cache_args* args,
  * with fp32 scores and sums, p rounded to the activation dtype for the second
  * product, and the result rounded once. Keys behind token i take no part,
  * whatever they hold. Rows behind the last sequence are left as they were.
+ * Sequences may not overlap: after a start that falls, rows of several sequences
+ * may come from any of them, and where the sequences have more than `tokens`
+ * tokens in all, rows of the last ones may be left as they were.
  * query, out [tokens, query_heads, head_dim], key, value [tokens, key_heads,
  * head_dim]: heads adjacent, token strides in elements, rows 16-byte aligned.
  * out may not overlap the inputs. dtype f16 or bf16; head_dim 64, 128 or 256;

@@ -116,8 +116,8 @@ def prompt_attention(
     or 256, Hq a multiple of Hk, heads adjacent, any 16-byte-aligned token
     stride, e.g. views of one projection's output). Sequence s is the tokens
     ``query_start[s] .. query_start[s + 1] - 1`` (int32 [S + 1], on the GPU); its
-    lengths need not be known on the host. Rows of ``out`` behind the last
-    sequence are left as they were. ``scale`` defaults to 1 / sqrt(D) and must be
+    lengths need not be known on the host, and no start below the one before it.
+    Rows of ``out`` behind the last sequence are left as they were. ``scale`` defaults to 1 / sqrt(D) and must be
     positive."""
     _call("prompt_attention", out, query, key, value, query_start, scale)
 
