@@ -873,14 +873,23 @@ __global__ void __launch_bounds__(TcShape<D, 2, kFp8>::kThreads, 1)
 }
 
 // ---- host ----------------------------------------------------------------------
-// Prompts run in single-tile blocks up to this many two-tile blocks per SM.
-// Measured (32/8 heads, D = 128 unless stated; single-tile against two-tile
-// blocks): 64 tokens 7.7 us against 9.8, seven prompts of 66-190 tokens 12.2
-// against 16.9, 1024 tokens 19.4 against 22.6, 4096 tokens 133 against 141, 19
-// prompts of up to 1500 tokens 172 against 177 and at D = 64 132 against 149;
-// 16384 tokens (13.8 blocks per SM) 2044 against 2008 in a long run: there
-// loading K and V once per block and not twice counts, and the ends do not.
-constexpr int kSingleTileWaves = 12;
+// Blocks of one row tile spread evenly over the SMs and waste less where sequences
+// end; blocks of two load K and V once for both. Two are taken behind
+// kTwoTileHalfWaves two-tile blocks per SM, in halves, and at D = 128 for sequences
+// of kTwoTiles of them on average. Measured (graph, 32/8 heads unless stated;
+// one tile against two, two-tile blocks per SM in brackets):
+// D = 128: 512 tokens 12.9 us against 14.8, 1024 (0.9) 19.5 against 22.1, 2500 (2.1)
+// 60.8 against 61.9, but 2048 (1.7) 43.5 against 41.2; 4096 (3.5) 139.5 against 134.6,
+// 64/8 heads 4096 (6.9) 288 against 278, 8192 (6.9) 507 against 491, 16384 (13.8) 1932
+// against 1870. 64 prompts of 1-200 tokens (5.4; 1.6 tiles each) 70 against 78, 30 of
+// 1-500 (6.3; 3.9) 85 against 89, 19 of 1-1500 (12; 12) even, 8 of 1-2000 (6.8; 16) 128
+// against 126.
+// D = 64: 1024 tokens 16.1 against 20.4, 4096 (3.5) even, 64 of 1-200 52 against 63, 19
+// of 1-1500 (12) 145 against 161, 8192 (6.9) even; 16384 (13.8) 1383 against 1316.
+template <int D>
+constexpr int kTwoTileHalfWaves = D == 64 ? 24 : 5;
+template <int D>
+constexpr int kTwoTiles = D == 64 ? 0 : 10;
 
 template <typename T, int D, int kTiles>
 int run_prompt(const PromptArgs& a, const CUtensorMap* maps, cudaStream_t stream) {
@@ -912,8 +921,9 @@ int run_prompt_tiles(const PromptArgs& a, cudaStream_t stream) {
   const int rc = current_device_info(&dev);
   if (rc != SM120N_OK) return rc;
   const int64_t pairs = (a.tokens * a.group + 2 * kTileRows - 1) / (2 * kTileRows) * a.key_heads;
-  return pairs <= kSingleTileWaves * dev.sm_count ? run_prompt<T, D, 1>(a, maps, stream)
-                                                  : run_prompt<T, D, 2>(a, maps, stream);
+  const bool two = 2 * pairs > kTwoTileHalfWaves<D> * int64_t{dev.sm_count} &&
+                   a.tokens * a.group >= int64_t{kTwoTiles<D>} * 2 * kTileRows * a.sequences;
+  return two ? run_prompt<T, D, 2>(a, maps, stream) : run_prompt<T, D, 1>(a, maps, stream);
 }
 
 template <typename TQ, typename T, bool kFp8, int D>
