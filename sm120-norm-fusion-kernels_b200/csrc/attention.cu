@@ -120,6 +120,12 @@ int check_decode_sizes(const sm120s_decode_args* a) {
 // Where a part has many blocks, there are few parts, and all of them won: 300
 // requests, 1024 tokens, 82 us with 3 parts against 87.6 with 2; 128 requests, D =
 // 64, 4096 tokens, 62.7 with 9 against 67.5 with 4.
+// Held against each number of parts from 1 to `most` on 100 batches (8 to 256 requests,
+// prefixes of 1024 to 32768 tokens, own tokens up to 64, 600 and 2048, groups of 2, 4
+// and 8, D = 64 and 128, fp8): in the median it took 1.03 times the best one's time, 23
+// batches lay above 1.1 and the worst at 1.33 (100 requests with prefixes of 1024
+// tokens, 32/4 heads, 38.5 us against 29 in one part). What it lacks is the lengths,
+// which are not on the host.
 int prefix_parts(const sm120s_decode_args& a, int most, int64_t blocks, int64_t tiles,
                  int64_t triples, int sm_count) {
   if (12 * blocks > sm_count) return most;
