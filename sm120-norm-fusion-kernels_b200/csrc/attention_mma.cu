@@ -19,6 +19,11 @@
 // these run the fp16 instruction, with each row of q scaled by a power of two
 // into [1, 2) first (exact but for elements 2^14 below the row's largest) and
 // the power folded into the row's score scale.
+//
+// Bound by instructions and their latencies: with heads of 256 a warp's 16 rows of o
+// and a tile's scores fill its 255 registers, so that one block of four warps runs on
+// an SM, and every tile of 64 keys has two barriers. One prompt of 4096 tokens, 32/8
+// heads of 256, takes 1945 us (0.14 PFLOP/s), where products alone would take 166.
 #include <algorithm>
 
 #include "attention.h"
