@@ -104,7 +104,7 @@ SM120N_API int sm120s_release_blocks(const int32_t* seq_lens, const uint8_t* fin
  * pair i turns by axis k = i mod axes if k > 0 and i < axes * sections[k], else
  * by axis 0. query_out / key_out: NULL for in place, or adjacent heads at these
  * token strides (elements): the input's own rows, or rows that share nothing with
- * query, key, value, the caches and one another.
+ * query, key, value, the caches and one another. (value may be key's own rows.)
  */
 typedef struct sm120s_mrope_args {
   uint32_t struct_size; /* sizeof(sm120s_mrope_args) */

@@ -474,7 +474,10 @@ int check_mrope_overlaps(const sm120n_qk_cache_args& in, const sm120s_mrope_args
   if (rows_overlap(key_out, query)) return refuse(m.key_out ? "key_out" : "key", "query");
   if (rows_overlap(query_out, key_out)) return refuse("query_out", "key_out");
   if (rows_overlap(query_out, value)) return refuse(m.query_out ? "query_out" : "query", "value");
-  if (rows_overlap(key_out, value)) return refuse(m.key_out ? "key_out" : "key", "value");
+  // a head's value is read by the threads that write its key, before they do
+  if (!same(key_out, value) && rows_overlap(key_out, value)) {
+    return refuse(m.key_out ? "key_out" : "key", "value");
+  }
   if (!stores || in.num_blocks < 1) return SM120N_OK;
   // a cache from its first to its last element
   const int64_t elems = (in.num_blocks - 1) * in.cache_block_stride +

@@ -83,3 +83,23 @@ def test_rotation_beside_and_over_its_inputs():
             run(q, k, **kw)
     run(q, k, query_out=q, key_out=k)  # in place, said twice
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rotation_of_keys_that_are_the_values_too(d):
+    """In place, with value the same rows as key: the cache gets the values as they were."""
+    (q, k, v), whole = columns(20, (4, 2, 2), d)
+    w = torch.ones(d, device=DEV, dtype=torch.bfloat16)
+    places = torch.arange(20, device=DEV).expand(3, -1)
+    table = torch.randn(64, d, device=DEV)
+    slots = torch.randperm(48, device=DEV)[:20].to(torch.int32)
+    results = []
+    for shared in (False, True):
+        key = k.clone()
+        caches = [torch.zeros(3, 16, 2, d, device=DEV, dtype=torch.bfloat16) for _ in "kv"]
+        extensions.qk_norm_mrope_cache_(q.clone(), key, key if shared else k, w, w, places, table,
+                                        [d // 4, d // 8, d // 8], *caches, slots)
+        results.append((key, *caches))
+    for apart, together in zip(*results):
+        assert torch.equal(apart, together)
+    assert torch.equal(results[1][2].view(48, 2, d)[slots.long()], k)
