@@ -80,6 +80,22 @@ SM120N_API int sm120s_plan_step(const int32_t* context_lens, const int32_t* quer
                      int64_t tokens, void* stream);
 
 /*
+ * The same, and the step with one row per request, as decode attention takes it
+ * whoever has a token. For r with q > 0 whose first token got a place:
+ *   row_positions[r] = c, row_slots[r] = its slot, row_lens[r] = c + q
+ * and otherwise row_positions[r] = -1, row_lens[r] = 0 and row_slots[r] = -1 for a
+ * request without a token, -2 for one whose token got no place. Each [requests],
+ * all three or none (NULL).
+ */
+SM120N_API int sm120s_plan_step_rows(const int32_t* context_lens, const int32_t* query_lens,
+                     int32_t* block_table, int64_t table_stride, const int32_t* free_blocks,
+                     const int32_t* free_count, int32_t* free_count_out, int32_t* query_start,
+                     int32_t* seq_lens, int64_t* positions, int32_t* slot_mapping,
+                     int64_t* row_positions, int32_t* row_slots, int32_t* row_lens,
+                     int64_t requests, int64_t table_width, int64_t pool, int64_t block_size,
+                     int64_t tokens, void* stream);
+
+/*
  * Gives the blocks of finished requests back: the entries
  * block_table[r, shared_blocks .. ceil(seq_lens[r] / block_size)) of every row
  * with finished[r] != 0, row after row, go to free_blocks[free_count ...];

@@ -61,7 +61,9 @@ void check_one_float(const torch::Tensor& t, const c10::Device& device) {
 void b200_plan_step(torch::Tensor context_lens, torch::Tensor query_lens, torch::Tensor block_table,
                     torch::Tensor free_blocks, torch::Tensor free_count, int64_t block_size,
                     torch::Tensor query_start, torch::Tensor seq_lens, torch::Tensor positions,
-                    torch::Tensor slot_mapping, c10::optional<torch::Tensor> free_count_out) {
+                    torch::Tensor slot_mapping, c10::optional<torch::Tensor> free_count_out,
+                    c10::optional<torch::Tensor> row_positions,
+                    c10::optional<torch::Tensor> row_slots, c10::optional<torch::Tensor> row_lens) {
   const auto device = context_lens.device();
   const int64_t requests = context_lens.numel();
   check_vector(context_lens, torch::kInt, -1, device, "context_lens");
@@ -73,14 +75,22 @@ void b200_plan_step(torch::Tensor context_lens, torch::Tensor query_lens, torch:
   check_vector(seq_lens, torch::kInt, requests, device, "seq_lens");
   check_vector(positions, torch::kInt64, -1, device, "positions");
   check_vector(slot_mapping, torch::kInt, positions.numel(), device, "slot_mapping");
+  if (row_positions.has_value()) {
+    check_vector(*row_positions, torch::kInt64, requests, device, "row_positions");
+  }
+  if (row_slots.has_value()) check_vector(*row_slots, torch::kInt, requests, device, "row_slots");
+  if (row_lens.has_value()) check_vector(*row_lens, torch::kInt, requests, device, "row_lens");
   c10::cuda::CUDAGuard guard(device);
-  raise_if_failed(sm120s_plan_step(
+  raise_if_failed(sm120s_plan_step_rows(
       context_lens.data_ptr<int32_t>(), query_lens.data_ptr<int32_t>(),
       block_table.data_ptr<int32_t>(), table_stride(block_table), free_blocks.data_ptr<int32_t>(),
       free_count.data_ptr<int32_t>(), count_after(free_count, free_count_out, device),
       query_start.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
-      slot_mapping.data_ptr<int32_t>(), requests, block_table.size(1), free_blocks.numel(),
-      block_size, positions.numel(), current_stream()));
+      slot_mapping.data_ptr<int32_t>(),
+      row_positions.has_value() ? row_positions->data_ptr<int64_t>() : nullptr,
+      row_slots.has_value() ? row_slots->data_ptr<int32_t>() : nullptr,
+      row_lens.has_value() ? row_lens->data_ptr<int32_t>() : nullptr, requests, block_table.size(1),
+      free_blocks.numel(), block_size, positions.numel(), current_stream()));
 }
 
 void b200_release_blocks(torch::Tensor seq_lens, torch::Tensor finished, torch::Tensor block_table,
@@ -277,7 +287,8 @@ TORCH_LIBRARY_FRAGMENT(sm120_norm_ext, m) {
       "plan_step_(Tensor(a!) context_lens, Tensor query_lens, Tensor(b!) block_table, "
       "Tensor free_blocks, Tensor(c!) free_count, int block_size, Tensor(d!) query_start, "
       "Tensor(e!) seq_lens, Tensor(f!) positions, Tensor(g!) slot_mapping, "
-      "Tensor(h!)? free_count_out=None) -> ()");
+      "Tensor(h!)? free_count_out=None, Tensor(i!)? row_positions=None, "
+      "Tensor(j!)? row_slots=None, Tensor(k!)? row_lens=None) -> ()");
   m.def(
       "release_blocks_(Tensor seq_lens, Tensor finished, Tensor block_table, "
       "Tensor(a!) free_blocks, Tensor(b!) free_count, int block_size, int shared_blocks=0, "

@@ -55,6 +55,9 @@ struct PlanArgs {
   int width;
   int pool;
   int block_size;
+  int64_t* row_positions;  // all three or none
+  int32_t* row_slots;
+  int32_t* row_lens;
 };
 
 // Sums here never fall and matter only up to 2^31 - 2 (tokens, blocks of the
@@ -123,8 +126,11 @@ struct BlockSize {
   }
 };
 
-template <int kBlocks, int kPer>
-__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
+// kRows: also the step with one row per request (one request 2.24 us against 2.03,
+// 1001 5.0 against 4.6). At least one block to an SM is asked for: without it the
+// compiler kept to 32 registers (a prompt step 8.05 us against 7.75).
+template <int kBlocks, int kPer, bool kRows>
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads, 1)
     plan_step_kernel(PlanArgs a) {
   // the rows of the chunk in work
   __shared__ uint32_t ends[kPlanThreads];   // of their tokens
@@ -191,6 +197,22 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     if (rank == 0 && live) {
       a.query_start[r + 1] = static_cast<int32_t>(min(end, tokens));
       a.seq_lens[r] = static_cast<int32_t>(served ? c + q : c);
+      if constexpr (kRows) {
+        // the request's first token, as the loop over the tokens below finds it
+        int slot = q == 0 ? -1 : -2;
+        if (served && q > 0) {
+          const uint32_t block = block_size.blocks(c);
+          const int id = block == held
+                             ? a.free_blocks[count - 1 - (upto - need)]
+                             : a.table[static_cast<int64_t>(r) * a.table_stride + block];
+          if (id >= 0 && id < a.pool) {
+            slot = static_cast<int>(id * block_size.size + (c - block * block_size.size));
+          }
+        }
+        a.row_slots[r] = slot;
+        a.row_lens[r] = slot >= 0 ? static_cast<int32_t>(c + q) : 0;
+        a.row_positions[r] = slot >= 0 ? int64_t{c} : -1;
+      }
     }
     const int in_chunk = min(threads, a.requests - base);
 
@@ -460,6 +482,20 @@ extern "C" int sm120s_plan_step(const int32_t* context_lens, const int32_t* quer
                                 int64_t* positions, int32_t* slot_mapping, int64_t requests,
                                 int64_t table_width, int64_t pool, int64_t block_size,
                                 int64_t tokens, void* stream) {
+  return sm120s_plan_step_rows(context_lens, query_lens, block_table, table_stride, free_blocks,
+                               free_count, free_count_out, query_start, seq_lens, positions,
+                               slot_mapping, nullptr, nullptr, nullptr, requests, table_width, pool,
+                               block_size, tokens, stream);
+}
+
+extern "C" int sm120s_plan_step_rows(const int32_t* context_lens, const int32_t* query_lens,
+                                     int32_t* block_table, int64_t table_stride,
+                                     const int32_t* free_blocks, const int32_t* free_count,
+                                     int32_t* free_count_out, int32_t* query_start,
+                                     int32_t* seq_lens, int64_t* positions, int32_t* slot_mapping,
+                                     int64_t* row_positions, int32_t* row_slots, int32_t* row_lens,
+                                     int64_t requests, int64_t table_width, int64_t pool,
+                                     int64_t block_size, int64_t tokens, void* stream) {
   clear_error();
   int rc = check_pool(free_blocks, pool, free_count, free_count_out, requests, table_width,
                       table_stride, block_size);
@@ -472,23 +508,31 @@ extern "C" int sm120s_plan_step(const int32_t* context_lens, const int32_t* quer
       (tokens > 0 && (!positions || !slot_mapping))) {
     return fail(SM120N_ERR_INVALID_ARGUMENT, "tensor pointers must be non-null");
   }
+  if (requests > 0 && (!row_positions || !row_slots || !row_lens) &&
+      (row_positions || row_slots || row_lens)) {
+    return fail(SM120N_ERR_INVALID_ARGUMENT, "row_positions, row_slots and row_lens go together");
+  }
   const PlanArgs a{context_lens, query_lens, block_table, free_blocks, free_count, free_count_out,
                    query_start, seq_lens, positions, slot_mapping, table_stride, tokens,
                    static_cast<int>(requests), static_cast<int>(table_width),
-                   static_cast<int>(pool), static_cast<int>(block_size)};
+                   static_cast<int>(pool), static_cast<int>(block_size), row_positions, row_slots,
+                   row_lens};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // A token to a thread of one block, then four, then four to a thread of a
   // cluster: 1001 decodes take 4.5 us with one token to a thread, 5.4 with four
   // and 5.8 on a cluster, a prompt step of a few thousand tokens 7.75 us with
   // four and 7.9 on a cluster, which is there for those that are longer.
+  const bool rows = row_slots != nullptr;
   if (tokens <= kPlanThreads) {
-    return launch(plan_step_kernel<1, 1>, dim3(1), dim3(plan_threads(std::max(requests, tokens))), 0,
-                  s, a);
+    return launch(rows ? plan_step_kernel<1, 1, true> : plan_step_kernel<1, 1, false>, dim3(1),
+                  dim3(plan_threads(std::max(requests, tokens))), 0, s, a);
   }
   if (tokens <= 4 * kPlanThreads) {
-    return launch(plan_step_kernel<1, 4>, dim3(1), dim3(kPlanThreads), 0, s, a);
+    return launch(rows ? plan_step_kernel<1, 4, true> : plan_step_kernel<1, 4, false>, dim3(1),
+                  dim3(kPlanThreads), 0, s, a);
   }
-  return launch(plan_step_kernel<kPlanCluster, 4>, dim3(kPlanCluster), dim3(kPlanThreads), 0, s, a);
+  return launch(rows ? plan_step_kernel<kPlanCluster, 4, true> : plan_step_kernel<kPlanCluster, 4, false>,
+                dim3(kPlanCluster), dim3(kPlanThreads), 0, s, a);
 }
 
 extern "C" int sm120s_release_blocks(const int32_t* seq_lens, const uint8_t* finished,

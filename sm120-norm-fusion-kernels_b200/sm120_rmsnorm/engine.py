@@ -127,8 +127,9 @@ class PagedSteps:
     :meth:`plan`; ``query_start``, ``positions`` and ``slot_mapping`` are those of the
     step planned last, packed request after request. ``row_positions``, ``row_slots``
     and ``row_lens`` are the same step as decode runs it, entry r for request r:
-    its first token's position and slot and its length with the step, or -1, -1 and 0
-    for a request without a token or without room for it (:attr:`unserved`).
+    its first token's position and slot and its length with the step, or a position
+    and a slot below zero and 0 for a request without a token or without room for it
+    (:attr:`unserved`).
 
     ``prefix_blocks`` blocks, taken off the pool here, are the first of every
     request's row, and every request begins behind them: its ``context_lens``
@@ -162,13 +163,10 @@ class PagedSteps:
         self.context_lens = ints(requests).fill_(prefix_blocks * block_size)
         self.query_start = ints(requests + 1)
         self.positions = ints(max_tokens, dtype=torch.int64)
-        # and one entry more, for requests without a token
-        self._slots = ints(max_tokens + 1).fill_(-1)
-        self.slot_mapping = self._slots[:max_tokens]
+        self.slot_mapping = ints(max_tokens)
         self.row_positions = ints(requests, dtype=torch.int64)
         self.row_slots = ints(requests)
         self.row_lens = ints(requests)
-        self._asked = ints(requests, dtype=torch.bool)
 
     def prefix_writer(self) -> PagedSteps:
         """A batch of one request whose blocks are those of the prefix: plan it with
@@ -185,18 +183,14 @@ class PagedSteps:
         """The next step, with ``query_lens`` (int32 [requests]) new tokens."""
         serving.plan_step_(self.context_lens, query_lens, self.block_table, self.free_blocks,
                            self.free_count, self.block_size, self.query_start, self.context_lens,
-                           self.positions, self.slot_mapping)
-        torch.gt(query_lens, 0, out=self._asked)
-        first = torch.where(self._asked, self.query_start[:-1], self.slot_mapping.numel())
-        torch.index_select(self._slots, 0, first, out=self.row_slots)
-        torch.mul(self.context_lens, self.row_slots >= 0, out=self.row_lens)
-        torch.sub(self.row_lens, 1, out=self.row_positions)
+                           self.positions, self.slot_mapping, None, self.row_positions,
+                           self.row_slots, self.row_lens)
 
     @property
     def unserved(self) -> torch.Tensor:
         """Requests (bool [requests], on the GPU) that had tokens in the step planned
         last and got no place for them: their lengths are as before the step."""
-        return self._asked & (self.row_slots < 0)
+        return self.row_slots == -2
 
     def release(self, finished: torch.Tensor) -> None:
         """Gives the blocks of the requests in ``finished`` (bool [requests]) back,

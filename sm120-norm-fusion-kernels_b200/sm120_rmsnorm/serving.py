@@ -60,6 +60,9 @@ def plan_step_(
     positions: torch.Tensor,
     slot_mapping: torch.Tensor,
     free_count_out: torch.Tensor | None = None,
+    row_positions: torch.Tensor | None = None,
+    row_slots: torch.Tensor | None = None,
+    row_lens: torch.Tensor | None = None,
 ) -> None:
     """Block tables, positions and slots of the next step, in one launch.
 
@@ -77,9 +80,14 @@ def plan_step_(
     [T]): of every packed token; slot -1 where nothing can be stored, both -1
     behind the last token, which the Q/K norm operators leave untouched.
     ``free_count`` (int32 [1]) is updated in place, or left as it is with the new
-    count in ``free_count_out``."""
+    count in ``free_count_out``. ``row_positions`` (int64 [R]), ``row_slots`` and
+    ``row_lens`` (int32 [R]; all three or none) are the step with one row per
+    request, as :func:`paged_decode_attention` takes it: position and slot of each
+    request's first token and its length with the step, or -1, -1, 0 for a request
+    without a token and -1, -2, 0 for one whose token got no place."""
     _call("plan_step_", context_lens, query_lens, block_table, free_blocks, free_count, block_size,
-          query_start, seq_lens, positions, slot_mapping, free_count_out)
+          query_start, seq_lens, positions, slot_mapping, free_count_out, row_positions, row_slots,
+          row_lens)
 
 
 def release_blocks_(
@@ -159,8 +167,8 @@ if _C is not None:
 
     @torch.library.register_fake("sm120_norm_ext::plan_step_")
     def _plan_step_meta(context_lens, query_lens, block_table, free_blocks, free_count, block_size,
-                        query_start, seq_lens, positions, slot_mapping,
-                        free_count_out=None) -> None:
+                        query_start, seq_lens, positions, slot_mapping, free_count_out=None,
+                        row_positions=None, row_slots=None, row_lens=None) -> None:
         return None
 
     @torch.library.register_fake("sm120_norm_ext::release_blocks_")

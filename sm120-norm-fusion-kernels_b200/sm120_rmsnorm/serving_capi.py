@@ -71,6 +71,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "sm120s_reset_device_faults": ([], ctypes.c_int),
     "sm120s_plan_step": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                           _i64, _i64, _i64, _i64, _i64, _vp], ctypes.c_int),
+    "sm120s_plan_step_rows": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                               _i64, _i64, _i64, _i64, _i64, _vp], ctypes.c_int),
     "sm120s_release_blocks": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp],
                               ctypes.c_int),
     "sm120s_qk_norm_mrope_cache": ([ctypes.POINTER(QkCacheArgs), ctypes.POINTER(MropeArgs), _vp],
@@ -126,6 +128,17 @@ def plan_step(context_lens_ptr, query_lens_ptr, block_table_ptr, table_stride, f
         context_lens_ptr, query_lens_ptr, block_table_ptr, table_stride, free_blocks_ptr,
         free_count_ptr, free_count_out_ptr, query_start_ptr, seq_lens_ptr, positions_ptr,
         slot_mapping_ptr, requests, table_width, pool, block_size, tokens, stream))
+
+
+def plan_step_rows(context_lens_ptr, query_lens_ptr, block_table_ptr, table_stride, free_blocks_ptr,
+                   free_count_ptr, free_count_out_ptr, query_start_ptr, seq_lens_ptr, positions_ptr,
+                   slot_mapping_ptr, row_positions_ptr, row_slots_ptr, row_lens_ptr, requests,
+                   table_width, pool, block_size, tokens, stream=0) -> None:
+    _check(load().sm120s_plan_step_rows(
+        context_lens_ptr, query_lens_ptr, block_table_ptr, table_stride, free_blocks_ptr,
+        free_count_ptr, free_count_out_ptr, query_start_ptr, seq_lens_ptr, positions_ptr,
+        slot_mapping_ptr, row_positions_ptr, row_slots_ptr, row_lens_ptr, requests, table_width,
+        pool, block_size, tokens, stream))
 
 
 def release_blocks(seq_lens_ptr, finished_ptr, block_table_ptr, table_stride, free_blocks_ptr,

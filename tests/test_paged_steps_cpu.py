@@ -17,14 +17,19 @@ def ints(values):
 @pytest.fixture(autouse=True)
 def plain_operators(monkeypatch):
     def plan(context, query, table, free, count, block_size, start, lens, positions, slots,
-             count_out=None):
-        rows = table.tolist()
+             count_out, row_positions, row_slots, row_lens):
+        rows, before, asked = table.tolist(), context.tolist(), query.tolist()
         got = ref.plan(context.tolist(), query.tolist(), rows, free.tolist(), int(count),
                        block_size, positions.numel())
         table.copy_(ints(rows).view_as(table))
         for to, values in zip((start, lens, positions, slots), got):
             to.copy_(torch.tensor(values))
         (count if count_out is None else count_out).fill_(got[4])
+        for r, (c, q, first) in enumerate(zip(before, asked, got[0])):
+            fits = q > 0 and sum(asked[:r + 1]) <= positions.numel() and got[3][first] >= 0
+            row_slots[r] = got[3][first] if fits else -2 if q > 0 else -1
+            row_lens[r] = c + q if fits else 0
+            row_positions[r] = c if fits else -1
 
     def release(lens, finished, table, free, count, block_size, shared=0, count_out=None):
         stack = free.tolist()
@@ -110,7 +115,7 @@ def rows_of(steps, query):
     steps.plan(ints(query))
     lens = steps.row_lens.tolist()
     assert steps.row_positions.tolist() == [n - 1 for n in lens]
-    return steps.row_slots.tolist(), lens, steps.unserved.nonzero().flatten().tolist()
+    return [max(s, -1) for s in steps.row_slots.tolist()], lens, steps.unserved.nonzero().flatten().tolist()
 
 
 def test_decode_rows_are_requests_whoever_has_a_token():
