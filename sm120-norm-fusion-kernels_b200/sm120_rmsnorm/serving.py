@@ -28,11 +28,7 @@ def _dispatched(name: str):
     return getattr(torch.ops.sm120_norm_ext, name).default
 
 
-_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None), bool, int, float, str, list, tuple))
 _compiling = torch.compiler.is_compiling
-_dispatch_modes = torch._C._len_torch_dispatch_stack
-_function_modes = torch._C._len_torch_function_stack
-_transforms = torch._C._functorch.peek_interpreter_stack
 
 
 def _call(name: str, *args) -> None:
@@ -41,8 +37,7 @@ def _call(name: str, *args) -> None:
     registered operator for tracing, modes, function transforms and tensor
     subclasses among the arguments."""
     extension = _extension()
-    if (not _compiling() and _PLAIN.issuperset(map(type, args))
-            and not _dispatch_modes() and not _function_modes() and _transforms() is None):
+    if not _compiling() and extension.nothing_looks_on(*args):
         getattr(extension, name)(*args)
     else:
         _dispatched(name)(*args)
