@@ -12,7 +12,12 @@ The order in which a step uses them, with the operators there were before:
 
 All are stream-ordered, never synchronise, and can be captured in a CUDA
 graph; registered as ``torch.ops.sm120_norm_ext.*``. They run forward only:
-none has a gradient. No fallback when the extension is missing.
+none has a gradient. Outputs may not share memory with inputs, but for what is said
+to be in place. No fallback when the extension is missing.
+
+The attention kernels bound every wait of theirs. One that runs out (never in
+correct operation) is counted in ``serving_capi.device_faults()``; decode rows that
+it had a part of are NaN, prompt rows that were not finished are left as they were.
 """
 from __future__ import annotations
 

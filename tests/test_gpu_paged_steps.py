@@ -2,6 +2,8 @@
 engine.Qwen3Attention): what a decode step returns must be the 64-bit attention
 over the keys and values that the request's own tokens had, kept beside the cache
 as they were computed, within the bounds of tests/serving_reference.py."""
+import random
+
 import pytest
 import torch
 
@@ -196,3 +198,59 @@ def test_a_captured_step_with_rows_that_come_and_go():
                     q[r, 4 * h:4 * h + 4].double(), keys[:, h], values[:, h], 128 ** -0.5,
                     torch.bfloat16, torch.bfloat16)
                 assert ((out[r, 4 * h:4 * h + 4].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("prefix", [0, 3])
+@pytest.mark.parametrize("seed", range(4))
+def test_requests_that_come_wait_and_go_at_random(seed, prefix):
+    """Rows take part in a step or not, run out of blocks, end and begin again; the
+    pool is too small for all. Every output against the request's own tokens."""
+    rng = random.Random(seed)
+    layer = Layer(10 + seed)
+    rows = 6
+    steps = PagedSteps(rows, BLOCKS, 20, rows, DEV, prefix_blocks=prefix)
+    if prefix:
+        layer.prompt(steps.prefix_writer(), [16 * prefix], ["prefix"])
+    kept = steps.free_blocks[:rng.randint(5, 7)].clone()
+    steps.free_count.fill_(len(kept))  # the others are somebody else's
+    born = 0
+    names = [None] * rows
+    waited = 0
+    for _ in range(120):
+        for r in range(rows):
+            if names[r] is None and rng.random() < 0.3:
+                names[r] = born
+                born += 1
+                if prefix:
+                    begin_behind(layer, "prefix", names[r])
+        takes = [name is not None and rng.random() < 0.8 for name in names]
+        before = steps.context_lens.tolist()
+        steps.plan(ints([int(t) for t in takes]))
+        qkv = layer.qkv(rows)
+        out = layer.attention.decode(*layer.rows(rows), steps, qkv=qkv)
+        q, k, v = layer.attention.prologue.split(qkv)
+        unserved, after = steps.unserved.tolist(), steps.context_lens.tolist()
+        waited += sum(unserved)
+        for r in range(rows):
+            served = takes[r] and not unserved[r]
+            assert after[r] == before[r] + served and not (unserved[r] and not takes[r])
+            if not served:
+                assert (out[r] == 0).all()
+                continue
+            layer.remember(names[r], k[r:r + 1], v[r:r + 1])
+            keys, values = (x.double() for x in layer.seen[names[r]])
+            assert len(keys) == after[r]
+            for h in range(SHAPE.key_heads):
+                heads = slice(4 * h, 4 * h + 4)
+                want, bound = ref.attention_row_block(
+                    q[r, heads].double(), keys[:, h], values[:, h], SHAPE.head_dim ** -0.5,
+                    torch.bfloat16, torch.bfloat16)
+                assert ((out[r, heads].double() - want).abs() <= bound).all()
+        done = [name is not None and rng.random() < 0.03 for name in names]
+        if any(done):
+            steps.release(bools(done))
+            names = [None if d else name for d, name in zip(done, names)]
+    assert waited > 0 and born > rows
+    steps.release(bools([True] * rows))
+    assert int(steps.free_count) == len(kept)
+    assert sorted(steps.free_blocks[:len(kept)].tolist()) == sorted(kept.tolist())
