@@ -92,3 +92,19 @@ def test_a_limit_between_loses_no_row(one_poll):
             bad = out.isnan().all(-1)
             assert torch.equal(out[~bad], right[~bad])
     recovers(c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens, hq, hk", [([300, 5, 900], 4, 2), ([700] * 12, 64, 8)])
+def test_a_limit_between_leaves_whole_prompt_rows(one_poll, d, lens, hq, hk):
+    c = Prompt(lens, hq=hq, hk=hk, d=d, seed=5)
+    capi.set_wait_limit(0)
+    right = c.run().clone()
+    for polls in (2, 5, 10, 20, 40, 80, 160, 320, 640):
+        capi.set_wait_limit(polls)
+        for _ in range(3):
+            c.out.fill_(3.0)
+            out = c.run()
+            torch.cuda.synchronize()
+            left = (out == 3.0).all(-1)
+            assert torch.equal(out[~left], right[~left])
